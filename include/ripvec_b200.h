@@ -45,6 +45,7 @@ extern "C" {
 #define RV_DTYPE_F32 0
 #define RV_DTYPE_BF16 1
 #define RV_DTYPE_F16 2
+#define RV_DTYPE_E4M3 3 /* 8-bit output of rv_rms_norm */
 
 #define RV_POOL_MEAN 0 /* mean over the sequence (ModernBERT; BASELINE ClassicBert config) */
 #define RV_POOL_CLS 1  /* first token (the reference ClassicBert CPU backend) */
@@ -317,6 +318,79 @@ int rv_index_export(rv_index* idx, int64_t row0, int64_t n, int32_t dst_dtype, v
  * of the max_pairs-th best score, or of the threshold itself). */
 int rv_index_find_duplicates(rv_index* idx, float threshold, int64_t max_pairs, int64_t* out_a, int64_t* out_b,
                              float* out_score, double* out_score64, int64_t* out_count);
+
+/* ---------------------------------------------------------------- decoding steps
+ * Operators of a decoder that reads what a search found: the retrieved text as a prefix that a batch
+ * of answers shares, or as the candidates of a rerank batch behind one query.  No counterpart in the
+ * reference.  Keys and values live in a cache of fixed-size pages that the caller owns.  A step is
+ * planned once on the host (which tokens are new, which pages they go to and read) and the plan then
+ * serves every layer.  rv_step_append, rv_step_attend and rv_rms_norm queue their kernels on `stream`
+ * (0 = the legacy default stream) and return; the tensors they are given must be ready in that
+ * stream's order.  Calls on one step from different streams are ordered by the library, except while
+ * a stream is being captured. */
+
+/* One layer's key and value pools, [num_pages, kv_heads, page_size, head_dim] in any order of memory:
+ * strides in elements, unit stride along head_dim; pools and strides multiples of 16 bytes. */
+typedef struct rv_kv_cache {
+  void* k;
+  void* v;
+  int64_t num_pages;
+  int64_t page_stride, head_stride, slot_stride;
+  int32_t dtype; /* RV_DTYPE_BF16 or RV_DTYPE_F16 */
+  int32_t kv_heads, head_dim, page_size;
+} rv_kv_cache;
+
+typedef struct rv_step rv_step;
+/* q_heads a multiple of kv_heads (query head h reads key/value head h / (q_heads / kv_heads));
+ * head_dim 64 or 128; page_size 16, 32, 64, 128 or 256 tokens. */
+int rv_step_create(int device, int32_t q_heads, int32_t kv_heads, int32_t head_dim, int32_t page_size, rv_step** out);
+void rv_step_destroy(rv_step* step);
+const char* rv_step_last_error(const rv_step* step);
+/* New tokens of the current plan (0 without one). */
+int rv_step_tokens(const rv_step* step);
+/* Plans a step of n_seqs sequences (host arrays, not retained).  Sequence b brings q_lens[b] new
+ * tokens (packed in order in the tensors of the calls below); own_lens[b] keys are its own once they
+ * are appended, in ceil(own_lens[b] / page_size) pages; own_pages lists all sequences' pages one
+ * after the other.  Consecutive sequences form n_groups groups of group_sizes[g]; the sequences of
+ * group g share a prefix of prefix_lens[g] keys in ceil(prefix_lens[g] / page_size) pages of
+ * prefix_pages; a length of 0 is no prefix.  Every page is below num_pages.  A query sees its group's
+ * whole prefix; with causal != 0, token i of q sees its own keys up to own_len - q + i, otherwise all
+ * of them.  A key's position is prefix_len + its place among its sequence's own.  Replaces the
+ * earlier plan once the calls queued with it are done; a failed plan leaves none. */
+int rv_step_plan(rv_step* step, int32_t n_seqs, const int32_t* q_lens, const int32_t* own_lens,
+                 const int32_t* own_pages, int32_t n_groups, const int32_t* group_sizes, const int32_t* prefix_lens,
+                 const int32_t* prefix_pages, int64_t num_pages, int32_t causal, void* stream);
+/* Rotates the new tokens' queries and keys by their positions and writes keys and values to their
+ * pages, the queries to q_out (which may be q itself; q = q_out = NULL appends keys and values only).
+ * q, q_out: [tokens, q_heads, head_dim]; k, v: [tokens, kv_heads, head_dim]; all of the cache's dtype
+ * with strides in elements and unit stride along head_dim.  The first `rot` values of a head turn by
+ * cos / sin [positions, rot / 2] (f32), as pairs (i, i + rot / 2), or (2i, 2i + 1) when interleaved;
+ * f32 arithmetic, rounded once.  RV_E_INVALID where own_lens < q_lens, and where a page that new
+ * tokens go to is also another sequence's or a prefix's. */
+int rv_step_append(rv_step* step, const rv_kv_cache* cache, const void* q, int64_t q_token_stride,
+                   int64_t q_head_stride, const void* k, int64_t k_token_stride, int64_t k_head_stride, const void* v,
+                   int64_t v_token_stride, int64_t v_head_stride, void* q_out, int64_t q_out_token_stride,
+                   int64_t q_out_head_stride, const float* cos, const float* sin, int64_t positions, int32_t rot,
+                   int32_t interleaved, void* stream);
+/* out = softmax(scale q K^T) V over the keys each query sees; out [tokens, q_heads, head_dim] of the
+ * cache's dtype.  lse (optional, f32 [tokens, q_heads], contiguous): the natural logarithm of the
+ * softmax's denominator, with which results over disjoint sets of keys can be joined.  A query that
+ * sees no key gets zeros and -inf.  Softmax statistics and sums are f32; the softmax's weights enter
+ * the second product in the cache's 16-bit type.  What a page holds past the last key is not used.
+ * q and out start on 16 bytes with strides of 16 bytes; scale > 0. */
+int rv_step_attend(rv_step* step, const rv_kv_cache* cache, const void* q, int64_t q_token_stride,
+                   int64_t q_head_stride, void* out, int64_t out_token_stride, int64_t out_head_stride, float* lse,
+                   float scale, void* stream);
+/* h = x + residual (residual may be NULL), residual_out = h rounded to 16 bits (may be NULL, may be
+ * residual or x), out = h / sqrt(mean(h^2) + eps) * weight; h and the statistics in f32, unrounded.
+ * Rows of `hidden` (1..65536) values of act_dtype with strides in elements; weight f32 [hidden].
+ * out_dtype act_dtype: 16-bit rows.  RV_DTYPE_E4M3: 8-bit codes with out ~ code * scale, scales f32
+ * [rows, hidden / group], scale = max(max |out|, 1e-12) / 448 over a group of 32, 64, 128 or 256
+ * values (hidden a multiple of it) or, with group 0, over the row. */
+int rv_rms_norm(int32_t act_dtype, const void* x, int64_t x_stride, const void* residual, int64_t residual_stride,
+                const float* weight, void* residual_out, int64_t residual_out_stride, void* out, int64_t out_stride,
+                int32_t out_dtype, float* scales, int32_t group, int64_t rows, int32_t hidden, float eps,
+                void* stream);
 
 /* ---------------------------------------------------------------- single-kernel entry points
  * Used by the parity tests to check one kernel against the CPU oracle.  Device pointers. */

@@ -26,6 +26,7 @@ RV_ARCH_CLASSICBERT = 2
 RV_DTYPE_F32 = 0
 RV_DTYPE_BF16 = 1
 RV_DTYPE_F16 = 2
+RV_DTYPE_E4M3 = 3
 RV_POOL_MEAN = 0
 RV_POOL_CLS = 1
 RV_KIND_GEMM = 0
@@ -55,6 +56,21 @@ class ModelDesc(C.Structure):
         ("type_vocab", C.c_int32),
         ("pooling", C.c_int32),
         ("max_batch_tokens", C.c_int64),
+    ]
+
+
+class KvCache(C.Structure):
+    _fields_ = [
+        ("k", C.c_void_p),
+        ("v", C.c_void_p),
+        ("num_pages", C.c_int64),
+        ("page_stride", C.c_int64),
+        ("head_stride", C.c_int64),
+        ("slot_stride", C.c_int64),
+        ("dtype", C.c_int32),
+        ("kv_heads", C.c_int32),
+        ("head_dim", C.c_int32),
+        ("page_size", C.c_int32),
     ]
 
 
@@ -116,6 +132,14 @@ SIGNATURES = {
     "rv_cache_decode": (C.c_int, [vp, C.c_uint64, vp, i64, C.POINTER(i64), C.POINTER(i32)]),
     "rv_cache_last_error": (C.c_char_p, []),
     "rv_index_export": (C.c_int, [vp, i64, i64, i32, vp, i32]),
+    "rv_step_create": (C.c_int, [C.c_int, i32, i32, i32, i32, C.POINTER(vp)]),
+    "rv_step_destroy": (None, [vp]),
+    "rv_step_last_error": (C.c_char_p, [vp]),
+    "rv_step_tokens": (C.c_int, [vp]),
+    "rv_step_plan": (C.c_int, [vp, i32, vp, vp, vp, i32, vp, vp, vp, i64, i32, vp]),
+    "rv_step_append": (C.c_int, [vp, vp] + [vp, i64, i64] * 4 + [vp, vp, i64, i32, i32, vp]),
+    "rv_step_attend": (C.c_int, [vp, vp] + [vp, i64, i64] * 2 + [vp, f32, vp]),
+    "rv_rms_norm": (C.c_int, [i32, vp, i64, vp, i64, vp, vp, i64, vp, i64, i32, vp, i32, i64, i32, f32, vp]),
     "rv_op_gemm": (C.c_int, [i32, vp, vp, vp, i32, i32, i32, i32, i32, vp]),
     "rv_op_attention": (C.c_int, [i32, vp, vp, vp, i32, i32, i32, i32, f32, vp]),
     "rv_debug_stall_attention": (C.c_int, [i32, i64]),

@@ -1,0 +1,436 @@
+// Decoding steps over a paged key/value cache: the C entry points, the checks of their arguments and
+// the host plan (which pages a step's tokens write and read) that one upload hands to the kernels of
+// every layer.
+#include "decode.h"
+
+#include <climits>
+#include <cmath>
+#include <cstring>
+#include <exception>
+#include <mutex>
+#include <new>
+#include <string>
+#include <vector>
+
+#include "../../include/ripvec_b200.h"
+#include "tmap.h"
+
+namespace {
+
+struct DeviceGuard {
+  int prev = -1;
+  bool ok = true;
+  explicit DeviceGuard(int d) {
+    cudaGetDevice(&prev);
+    if (prev != d) ok = cudaSetDevice(d) == cudaSuccess;
+    else prev = -1;
+  }
+  ~DeviceGuard() {
+    if (prev >= 0) cudaSetDevice(prev);
+  }
+};
+
+// Pinned staging of one plan's upload; reused once its copy has left it.
+struct Staging {
+  char* p = nullptr;
+  size_t cap = 0;
+  cudaEvent_t done = nullptr;
+};
+
+constexpr int64_t kMaxTokens = int64_t(1) << 24;  // of one step
+constexpr int64_t kMaxKeys = int64_t(1) << 30;    // of one sequence or prefix
+
+bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
+
+}  // namespace
+
+struct rv_step {
+  int device = 0;
+  int q_heads = 0, kv_heads = 0, head_dim = 0, page_size = 0;
+  std::mutex mu;
+  std::string err;
+  // the plan
+  bool planned = false, can_append = false;
+  int n_tokens = 0;
+  int64_t num_pages = 0;
+  int last_pos = -1;  // largest position of a new token
+  char* meta = nullptr;
+  size_t meta_cap = 0;
+  const rv::StepToken* tokens = nullptr;
+  const rv::StepSeq* seqs = nullptr;
+  const int* pages = nullptr;
+  Staging staging[2];
+  int turn = 0;
+  std::vector<char> host;
+  std::vector<int> writer;  // by page: 1 + the sequence that writes to it
+  // Calls on different streams wait for one another: plan, append and attend share the plan's device
+  // records and the workspace.
+  cudaEvent_t last = nullptr;
+  cudaStream_t last_stream = nullptr;
+  bool used = false;
+};
+
+namespace {
+
+int fail(rv_step* s, int code, const std::string& why) {
+  s->err = why;
+  return code;
+}
+
+int cuda_fail(rv_step* s, const char* what, cudaError_t e) {
+  return fail(s, e == cudaErrorMemoryAllocation ? RV_E_NOMEM : RV_E_CUDA, std::string(what) + ": " + cudaGetErrorString(e));
+}
+
+bool capturing(cudaStream_t st) {
+  cudaStreamCaptureStatus cs = cudaStreamCaptureStatusNone;
+  return cudaStreamIsCapturing(st, &cs) == cudaSuccess && cs != cudaStreamCaptureStatusNone;
+}
+
+// Makes st wait for this step's earlier work on another stream.  Under stream capture the order is the
+// caller's: an event of uncaptured work cannot be waited for there.
+cudaError_t enter(rv_step* s, cudaStream_t st) {
+  if (!s->used || st == s->last_stream || capturing(st)) return cudaSuccess;
+  return cudaStreamWaitEvent(st, s->last, 0);
+}
+cudaError_t leave(rv_step* s, cudaStream_t st) {
+  if (capturing(st)) return cudaSuccess;
+  s->used = true;
+  s->last_stream = st;
+  return cudaEventRecord(s->last, st);
+}
+
+// The pools as the kernels take them, checked against the step; an empty string, or what is wrong.
+std::string take_pool(const rv_step* s, const rv_kv_cache* c, rv::KvPool* out, rv::Act* act) {
+  if (!c || !c->k || !c->v) return "null cache";
+  if (c->dtype != RV_DTYPE_BF16 && c->dtype != RV_DTYPE_F16) return "the cache's dtype is neither bf16 nor f16";
+  if (c->kv_heads != s->kv_heads || c->head_dim != s->head_dim || c->page_size != s->page_size)
+    return "the cache's kv_heads, head_dim or page_size are not the step's";
+  if (c->num_pages < s->num_pages) return "the cache has fewer pages than the plan was made for";
+  if (!aligned16(c->k) || !aligned16(c->v) || (c->num_pages > 1 && c->page_stride % 8) || (s->kv_heads > 1 && c->head_stride % 8) ||
+      c->slot_stride % 8)
+    return "the cache's pools and strides must be multiples of 16 bytes";
+  // The stride of an axis of one entry has no meaning (and may be anything).
+  const int64_t page_stride = c->num_pages > 1 ? c->page_stride : s->head_dim;
+  const int64_t head_stride = s->kv_heads > 1 ? c->head_stride : s->head_dim;
+  if (page_stride <= 0 || head_stride <= 0 || c->slot_stride < s->head_dim)
+    return "the cache's strides must be positive, the slot stride at least head_dim";
+  out->k = c->k;
+  out->v = c->v;
+  out->page_stride = page_stride;
+  out->head_stride = head_stride;
+  out->slot_stride = c->slot_stride;
+  out->page_size = c->page_size;
+  *act = c->dtype == RV_DTYPE_BF16 ? rv::Act::kBf16 : rv::Act::kF16;
+  return "";
+}
+
+bool rows_aligned(const void* p, int64_t ts, int64_t hs) { return aligned16(p) && ts % 8 == 0 && hs % 8 == 0; }
+
+int plan(rv_step* s, int32_t n_seqs, const int32_t* q_lens, const int32_t* own_lens, const int32_t* own_pages,
+         int32_t n_groups, const int32_t* group_sizes, const int32_t* prefix_lens, const int32_t* prefix_pages,
+         int64_t num_pages, int32_t causal, cudaStream_t st) {
+  s->planned = false;
+  if (n_seqs < 0 || n_groups < 0 || num_pages < 0 || num_pages > INT_MAX || (n_seqs > 0 && (!q_lens || !own_lens)) ||
+      (n_groups > 0 && (!group_sizes || !prefix_lens)))
+    return fail(s, RV_E_INVALID, "null or negative argument");
+  if (capturing(st)) return fail(s, RV_E_INVALID, "a plan cannot be made on a capturing stream");
+  const int ps = s->page_size;
+  auto count = [ps](int64_t keys) { return (keys + ps - 1) / ps; };
+  int64_t in_groups = 0, n_prefix_pages = 0, n_own_pages = 0, tokens = 0;
+  for (int g = 0; g < n_groups; ++g) {
+    if (group_sizes[g] < 0 || prefix_lens[g] < 0 || prefix_lens[g] > kMaxKeys)
+      return fail(s, RV_E_INVALID, "group sizes and prefix lengths must be from 0 to 2^30");
+    in_groups += group_sizes[g];
+    n_prefix_pages += count(prefix_lens[g]);
+  }
+  if (in_groups != n_seqs) return fail(s, RV_E_INVALID, "the group sizes do not add up to the sequences");
+  bool can_append = true;
+  for (int b = 0; b < n_seqs; ++b) {
+    if (q_lens[b] < 0 || own_lens[b] < 0 || own_lens[b] > kMaxKeys)
+      return fail(s, RV_E_INVALID, "lengths must be from 0 to 2^30");
+    tokens += q_lens[b];
+    n_own_pages += count(own_lens[b]);
+    can_append = can_append && own_lens[b] >= q_lens[b];
+  }
+  if (tokens > kMaxTokens) return fail(s, RV_E_INVALID, "more than 2^24 tokens in one step");
+  if (n_prefix_pages + n_own_pages > INT_MAX / 8) return fail(s, RV_E_INVALID, "too many pages in one step");
+  if ((n_prefix_pages > 0 && !prefix_pages) || (n_own_pages > 0 && !own_pages))
+    return fail(s, RV_E_INVALID, "null page list");
+  for (int64_t i = 0; i < n_prefix_pages; ++i)
+    if (prefix_pages[i] < 0 || prefix_pages[i] >= num_pages) return fail(s, RV_E_INVALID, "prefix page out of range");
+  for (int64_t i = 0; i < n_own_pages; ++i)
+    if (own_pages[i] < 0 || own_pages[i] >= num_pages) return fail(s, RV_E_INVALID, "page out of range");
+
+  const size_t o_tokens = 0, o_seqs = o_tokens + size_t(tokens) * sizeof(rv::StepToken);
+  const size_t o_pages = o_seqs + size_t(n_seqs) * sizeof(rv::StepSeq);
+  const size_t bytes = o_pages + size_t(n_prefix_pages + n_own_pages) * sizeof(int);
+  s->host.resize(bytes ? bytes : 1);
+  auto* tk = reinterpret_cast<rv::StepToken*>(s->host.data() + o_tokens);
+  auto* sq = reinterpret_cast<rv::StepSeq*>(s->host.data() + o_seqs);
+  int* pg = reinterpret_cast<int*>(s->host.data() + o_pages);
+  if (n_prefix_pages) std::memcpy(pg, prefix_pages, size_t(n_prefix_pages) * 4);
+  if (n_own_pages) std::memcpy(pg + n_prefix_pages, own_pages, size_t(n_own_pages) * 4);
+  s->writer.assign(size_t(num_pages), 0);
+  int t = 0, b = 0, last_pos = -1;
+  int64_t pa = 0, pb = n_prefix_pages;
+  for (int g = 0; g < n_groups; ++g) {
+    for (int k = 0; k < group_sizes[g]; ++k, ++b) {
+      const int n = q_lens[b], own = own_lens[b];
+      sq[b] = {t, n, int(pa), prefix_lens[g], int(pb), own, causal ? own - n : INT_MAX / 2, 0};
+      for (int i = 0; i < n; ++i) {
+        const int place = own - n + i;  // negative only when nothing can be appended
+        const int page = place >= 0 ? pg[pb + place / ps] : 0;
+        tk[t++] = {page, place >= 0 ? place % ps : 0, prefix_lens[g] + place, b};
+        if (place < 0) continue;
+        int& w = s->writer[size_t(page)];
+        if (w && w != b + 1) can_append = false;
+        w = b + 1;
+        if (prefix_lens[g] + place > last_pos) last_pos = prefix_lens[g] + place;
+      }
+      pb += count(own);
+    }
+    pa += count(prefix_lens[g]);
+  }
+  // A page that new tokens go to belongs to no prefix.
+  for (int64_t i = 0; i < n_prefix_pages; ++i)
+    if (s->writer[size_t(prefix_pages[i])]) can_append = false;
+
+  Staging& sg = s->staging[s->turn];
+  s->turn ^= 1;
+  cudaError_t e = cudaEventSynchronize(sg.done);  // the copy before last has left this buffer
+  if (e != cudaSuccess) return cuda_fail(s, "waiting for an earlier plan", e);
+  if (sg.cap < bytes) {
+    if (sg.p) cudaFreeHost(sg.p);
+    sg.p = nullptr;
+    sg.cap = 0;
+    const size_t want = bytes + bytes / 2 + 4096;
+    if ((e = cudaMallocHost(reinterpret_cast<void**>(&sg.p), want)) != cudaSuccess)
+      return cuda_fail(s, "pinned staging", e);
+    sg.cap = want;
+  }
+  if (s->meta_cap < bytes) {
+    if (s->meta) cudaFree(s->meta);  // waits for the kernels that still read it
+    s->meta = nullptr;
+    s->meta_cap = 0;
+    const size_t want = bytes + bytes / 2 + 4096;
+    if ((e = cudaMalloc(reinterpret_cast<void**>(&s->meta), want)) != cudaSuccess)
+      return cuda_fail(s, "plan records", e);
+    s->meta_cap = want;
+  }
+  if (bytes) std::memcpy(sg.p, s->host.data(), bytes);
+  if ((e = enter(s, st)) != cudaSuccess) return cuda_fail(s, "ordering streams", e);
+  if (bytes && (e = cudaMemcpyAsync(s->meta, sg.p, bytes, cudaMemcpyHostToDevice, st)) != cudaSuccess)
+    return cuda_fail(s, "plan upload", e);
+  if ((e = cudaEventRecord(sg.done, st)) != cudaSuccess) return cuda_fail(s, "plan upload", e);
+  if ((e = leave(s, st)) != cudaSuccess) return cuda_fail(s, "ordering streams", e);
+  s->tokens = reinterpret_cast<rv::StepToken*>(s->meta + o_tokens);
+  s->seqs = reinterpret_cast<rv::StepSeq*>(s->meta + o_seqs);
+  s->pages = reinterpret_cast<int*>(s->meta + o_pages);
+  s->n_tokens = int(tokens);
+  s->num_pages = num_pages;
+  s->last_pos = last_pos;
+  s->can_append = can_append;
+  s->planned = true;
+  return RV_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+int rv_step_create(int device, int32_t q_heads, int32_t kv_heads, int32_t head_dim, int32_t page_size, rv_step** out) {
+  if (!out) return RV_E_INVALID;
+  *out = nullptr;
+  if (q_heads <= 0 || kv_heads <= 0 || q_heads % kv_heads || q_heads > 1024 || (head_dim != 64 && head_dim != 128) ||
+      (page_size != 16 && page_size != 32 && page_size != 64 && page_size != 128 && page_size != 256))
+    return RV_E_INVALID;
+  rv_step* s = new (std::nothrow) rv_step;
+  if (!s) return RV_E_NOMEM;
+  s->device = device;
+  s->q_heads = q_heads;
+  s->kv_heads = kv_heads;
+  s->head_dim = head_dim;
+  s->page_size = page_size;
+  DeviceGuard g(device);
+  bool ok = g.ok && cudaEventCreateWithFlags(&s->last, cudaEventDisableTiming) == cudaSuccess;
+  for (auto& sg : s->staging) ok = ok && cudaEventCreateWithFlags(&sg.done, cudaEventDisableTiming) == cudaSuccess;
+  if (!ok) {
+    cudaGetLastError();
+    rv_step_destroy(s);
+    return RV_E_CUDA;
+  }
+  *out = s;
+  return RV_OK;
+}
+
+void rv_step_destroy(rv_step* s) {
+  if (!s) return;
+  {
+    DeviceGuard g(s->device);
+    if (s->used) cudaEventSynchronize(s->last);
+    for (auto& sg : s->staging) {
+      if (sg.done) {
+        cudaEventSynchronize(sg.done);
+        cudaEventDestroy(sg.done);
+      }
+      if (sg.p) cudaFreeHost(sg.p);
+    }
+    if (s->meta) cudaFree(s->meta);
+    if (s->last) cudaEventDestroy(s->last);
+  }
+  delete s;
+}
+
+const char* rv_step_last_error(const rv_step* s) { return s ? s->err.c_str() : "null step"; }
+
+int rv_step_tokens(const rv_step* s) { return s && s->planned ? s->n_tokens : 0; }
+
+int rv_step_plan(rv_step* s, int32_t n_seqs, const int32_t* q_lens, const int32_t* own_lens, const int32_t* own_pages,
+                 int32_t n_groups, const int32_t* group_sizes, const int32_t* prefix_lens, const int32_t* prefix_pages,
+                 int64_t num_pages, int32_t causal, void* stream) {
+  if (!s) return RV_E_INVALID;
+  std::lock_guard<std::mutex> lk(s->mu);
+  DeviceGuard g(s->device);
+  if (!g.ok) return fail(s, RV_E_CUDA, "cudaSetDevice failed");
+  try {
+    return plan(s, n_seqs, q_lens, own_lens, own_pages, n_groups, group_sizes, prefix_lens, prefix_pages, num_pages,
+                causal, static_cast<cudaStream_t>(stream));
+  } catch (const std::exception& e) {
+    s->planned = false;
+    return fail(s, RV_E_NOMEM, e.what());
+  }
+}
+
+int rv_step_append(rv_step* s, const rv_kv_cache* cache, const void* q, int64_t q_token, int64_t q_head, const void* k,
+                   int64_t k_token, int64_t k_head, const void* v, int64_t v_token, int64_t v_head, void* q_out,
+                   int64_t q_out_token, int64_t q_out_head, const float* cos, const float* sin, int64_t positions,
+                   int32_t rot, int32_t interleaved, void* stream) {
+  if (!s) return RV_E_INVALID;
+  std::lock_guard<std::mutex> lk(s->mu);
+  try {
+    if (!s->planned) return fail(s, RV_E_NOT_READY, "no plan");
+    if (!s->can_append)
+      return fail(s, RV_E_INVALID, "the plan cannot append: own_lens below q_lens, or a page that new tokens go to is "
+                                   "another sequence's or a prefix's");
+    rv::AppendArgs a{};
+    rv::Act act;
+    const std::string why = take_pool(s, cache, &a.pool, &act);
+    if (!why.empty()) return fail(s, RV_E_INVALID, why);
+    if (rot < 0 || rot > s->head_dim || rot % 2) return fail(s, RV_E_INVALID, "rot must be even, from 0 to head_dim");
+    if (s->n_tokens == 0) return RV_OK;
+    if (!k || !v || !q != !q_out) return fail(s, RV_E_INVALID, "null keys or values, or queries without their output");
+    if (rot > 0 && (!cos || !sin || s->last_pos >= positions))
+      return fail(s, RV_E_INVALID, "the rotation table is missing or shorter than the step's positions");
+    a.tokens = s->tokens;
+    a.n_tokens = s->n_tokens;
+    a.q_heads = s->q_heads;
+    a.kv_heads = s->kv_heads;
+    a.head_dim = s->head_dim;
+    a.q = {q, q_token, q_head};
+    a.k = {k, k_token, k_head};
+    a.v = {v, v_token, v_head};
+    a.q_out = q_out;
+    a.q_out_token = q_out_token;
+    a.q_out_head = q_out_head;
+    a.cos = cos;
+    a.sin = sin;
+    a.rot = rot;
+    a.interleaved = interleaved != 0;
+    a.vec = rows_aligned(q, q_token, q_head) && rows_aligned(k, k_token, k_head) && rows_aligned(v, v_token, v_head) &&
+            rows_aligned(q_out, q_out_token, q_out_head) && aligned16(cos) && aligned16(sin) && rot % 16 == 0;
+    DeviceGuard g(s->device);
+    if (!g.ok) return fail(s, RV_E_CUDA, "cudaSetDevice failed");
+    cudaStream_t st = static_cast<cudaStream_t>(stream);
+    cudaError_t e = enter(s, st);
+    if (e == cudaSuccess) e = rv::kv_append(act, a, st);
+    if (e == cudaSuccess) e = leave(s, st);
+    return e == cudaSuccess ? RV_OK : cuda_fail(s, "rv_step_append", e);
+  } catch (const std::exception& e) {
+    return fail(s, RV_E_NOMEM, e.what());
+  }
+}
+
+int rv_step_attend(rv_step* s, const rv_kv_cache* cache, const void* q, int64_t q_token, int64_t q_head, void* out,
+                   int64_t out_token, int64_t out_head, float* lse, float scale, void* stream) {
+  if (!s) return RV_E_INVALID;
+  std::lock_guard<std::mutex> lk(s->mu);
+  try {
+    if (!s->planned) return fail(s, RV_E_NOT_READY, "no plan");
+    rv::AttendArgs a{};
+    rv::Act act;
+    const std::string why = take_pool(s, cache, &a.pool, &act);
+    if (!why.empty()) return fail(s, RV_E_INVALID, why);
+    if (!(scale > 0.f) || !std::isfinite(scale)) return fail(s, RV_E_INVALID, "scale must be positive and finite");
+    if (s->n_tokens == 0) return RV_OK;
+    if (!q || !out) return fail(s, RV_E_INVALID, "null queries or output");
+    if (s->q_heads == 1) q_head = out_head = s->head_dim;
+    if (s->n_tokens == 1) {
+      q_token = q_head * s->q_heads;
+      out_token = out_head * s->q_heads;
+    }
+    if (!rows_aligned(q, q_token, q_head) || !rows_aligned(out, out_token, out_head))
+      return fail(s, RV_E_INVALID, "queries and output must start on 16 bytes and have strides of 16 bytes");
+    if (q_token <= 0 || q_head <= 0 || out_token <= 0 || out_head <= 0)
+      return fail(s, RV_E_INVALID, "the strides of queries and output must be positive");
+    a.tokens = s->tokens;
+    a.seqs = s->seqs;
+    a.pages = s->pages;
+    a.n_tokens = s->n_tokens;
+    a.q_heads = s->q_heads;
+    a.kv_heads = s->kv_heads;
+    a.head_dim = s->head_dim;
+    a.q = {q, q_token, q_head};
+    a.out = out;
+    a.out_token = out_token;
+    a.out_head = out_head;
+    a.lse = lse;
+    a.scale = scale;
+    DeviceGuard g(s->device);
+    if (!g.ok) return fail(s, RV_E_CUDA, "cudaSetDevice failed");
+    cudaStream_t st = static_cast<cudaStream_t>(stream);
+    cudaError_t e = enter(s, st);
+    if (e == cudaSuccess) e = rv::step_attend(act, a, st);
+    if (e == cudaSuccess) e = leave(s, st);
+    return e == cudaSuccess ? RV_OK : cuda_fail(s, "rv_step_attend", e);
+  } catch (const std::exception& e) {
+    return fail(s, RV_E_NOMEM, e.what());
+  }
+}
+
+int rv_rms_norm(int32_t act_dtype, const void* x, int64_t x_stride, const void* residual, int64_t residual_stride,
+                const float* weight, void* residual_out, int64_t residual_out_stride, void* out, int64_t out_stride,
+                int32_t out_dtype, float* scales, int32_t group, int64_t rows, int32_t hidden, float eps,
+                void* stream) {
+  if (act_dtype != RV_DTYPE_BF16 && act_dtype != RV_DTYPE_F16) return RV_E_INVALID;
+  if (out_dtype != act_dtype && out_dtype != RV_DTYPE_E4M3) return RV_E_INVALID;
+  const bool out8 = out_dtype == RV_DTYPE_E4M3;
+  if (rows < 0 || hidden <= 0 || hidden > 65536 || !(eps >= 0.f) || !std::isfinite(eps)) return RV_E_INVALID;
+  if (group != 0 && (!out8 || (group != 32 && group != 64 && group != 128 && group != 256) || hidden % group))
+    return RV_E_INVALID;
+  if (rows == 0) return RV_OK;
+  if (!x || !weight || !out || (out8 != (scales != nullptr))) return RV_E_INVALID;
+  // Input rows may repeat (stride 0); output rows may not overlap.
+  if (x_stride < 0 || (residual && residual_stride < 0) ||
+      (rows > 1 && (out_stride < hidden || (residual_out && residual_out_stride < hidden))))
+    return RV_E_INVALID;
+  rv::NormArgs a{};
+  a.x = x;
+  a.residual = residual;
+  a.weight = weight;
+  a.rows = rows;
+  a.hidden = hidden;
+  a.x_stride = x_stride;
+  a.residual_stride = residual_stride;
+  a.residual_out_stride = residual_out_stride;
+  a.out_stride = out_stride;
+  a.residual_out = residual_out;
+  a.out = out;
+  a.scales = scales;
+  a.group = group ? group : hidden;
+  a.eps = eps;
+  const cudaError_t e =
+      rv::rms_norm(act_dtype == RV_DTYPE_BF16 ? rv::Act::kBf16 : rv::Act::kF16, a, static_cast<cudaStream_t>(stream));
+  return e == cudaSuccess ? RV_OK : RV_E_CUDA;
+}
+
+}  // extern "C"

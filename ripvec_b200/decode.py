@@ -1,0 +1,228 @@
+"""Decoder-side operators over a paged key/value cache (torch device tensors).
+
+What runs after a search: a decoder reads the retrieved text, either as one prefix that a batch of
+answers shares or as the candidates of a rerank batch behind one query.  ``PagedCache`` describes one
+layer's pools, ``DecodeStep`` plans a step once for all layers and runs ``append`` (rotary positions,
+keys and values into their pages) and ``attend`` (attention of every sequence over its group's shared
+prefix and its own keys), and ``rms_norm`` is the decoder's residual norm with 16-bit or 8-bit output.
+
+Calls queue their kernels on ``stream`` (a CUDA stream handle; by default torch's current stream) and
+return.  The reference has no decoder; there is nothing of it to cite here.
+"""
+
+from __future__ import annotations
+
+import ctypes as C
+from typing import Sequence
+
+import numpy as np
+import torch
+
+from . import _lib as L
+
+_DTYPES = {torch.bfloat16: L.RV_DTYPE_BF16, torch.float16: L.RV_DTYPE_F16}
+
+
+def _stream(stream, device) -> int | None:
+    return (torch.cuda.current_stream(device).cuda_stream if stream is None else stream) or None
+
+
+def _rows(name: str, t, tokens: int, heads: int, dim: int, dtype, device) -> None:
+    if t.shape != (tokens, heads, dim) or t.dtype != dtype or t.device != device or t.stride(2) != 1:
+        raise ValueError(f"{name} must be [{tokens}, {heads}, {dim}] {dtype} on {device} with unit stride along the "
+                         f"last axis, got {tuple(t.shape)} {t.dtype} on {t.device} with strides {t.stride()}")
+
+
+def _i32(values) -> np.ndarray:
+    a = np.asarray(values)
+    if a.size and (a.dtype.kind not in "iu" or a.min() < 0 or a.max() > np.iinfo(np.int32).max):
+        raise ValueError("lengths, sizes and pages are whole numbers from 0 to 2^31 - 1")
+    return np.ascontiguousarray(a, np.int32)
+
+
+class PagedCache:
+    """One layer's key and value pools, ``[pages, kv_heads, page_size, head_dim]`` bf16 or f16 tensors in
+    any order of memory (pass a transposed view of other layouts) with unit stride along ``head_dim`` and
+    the same strides.  The tensors are the caller's and are kept alive by this object."""
+
+    def __init__(self, k: torch.Tensor, v: torch.Tensor):
+        if k.ndim != 4 or k.shape != v.shape or k.dtype not in _DTYPES or v.dtype != k.dtype or not k.is_cuda \
+                or v.device != k.device:
+            raise ValueError("k and v must be 4-D bf16 or f16 tensors of one shape on one CUDA device")
+        if k.stride() != v.stride() or k.stride(3) != 1:
+            raise ValueError("k and v must have the same strides, and unit stride along the last axis")
+        self.k, self.v = k, v
+        self.num_pages, self.kv_heads, self.page_size, self.head_dim = k.shape
+        self.dtype, self.device = k.dtype, k.device
+        sp, sh, ss, _ = k.stride()
+        self.desc = L.KvCache(k.data_ptr(), v.data_ptr(), self.num_pages, sp, sh, ss, _DTYPES[k.dtype], self.kv_heads,
+                              self.head_dim, self.page_size)
+        self._ref = C.addressof(self.desc)
+
+
+class DecodeStep:
+    """A step of a batch: planned once on the host, then run by every layer (``rv_step_*``)."""
+
+    def __init__(self, *, q_heads: int, kv_heads: int, head_dim: int, page_size: int, device: int = 0):
+        self._lib = L.lib()
+        h = C.c_void_p()
+        rc = self._lib.rv_step_create(device, q_heads, kv_heads, head_dim, page_size, C.byref(h))
+        if rc != L.RV_OK:
+            raise L.RvError(rc, "rv_step_create failed (q_heads a multiple of kv_heads, head_dim 64 or 128, page_size "
+                                "16, 32, 64, 128 or 256, a CUDA device)")
+        self._h = h
+        self.q_heads, self.kv_heads, self.head_dim, self.page_size = q_heads, kv_heads, head_dim, page_size
+        self.device = torch.device("cuda", device)
+        self.tokens = None  # of the plan; None without one
+
+    def _check(self, rc: int) -> None:
+        if rc != L.RV_OK:
+            raise L.RvError(rc, self._lib.rv_step_last_error(self._h).decode())
+
+    def _tokens(self) -> int:
+        if self.tokens is None:
+            raise L.RvError(L.RV_E_NOT_READY, "no plan")
+        return self.tokens
+
+    def close(self) -> None:
+        if getattr(self, "_h", None):
+            self._lib.rv_step_destroy(self._h)
+            self._h = None
+
+    def __del__(self):
+        try:
+            self.close()
+        except Exception:
+            pass
+
+    def plan(self, *, q_lens: Sequence[int], own_lens: Sequence[int], own_pages: Sequence[Sequence[int]],
+             num_pages: int, prefix_lens: Sequence[int] = (), prefix_pages: Sequence[Sequence[int]] = (),
+             group_sizes: Sequence[int] | None = None, causal: bool = True, stream: int | None = None) -> None:
+        """``rv_step_plan``: sequence ``b`` brings ``q_lens[b]`` new tokens and has ``own_lens[b]`` keys of
+        its own, these included, in ``own_pages[b]`` (longer lists are cut).  Consecutive sequences form
+        groups that share a prefix; by default one group of all, with no prefix or the one given."""
+        self.tokens = None
+        ps = self.page_size
+        ql, ol, pl = _i32(q_lens), _i32(own_lens), _i32(prefix_lens)
+        if len(ql) != len(ol) or len(own_pages) != len(ol) or len(prefix_pages) != len(pl):
+            raise ValueError("q_lens, own_lens and own_pages (and prefix_lens and prefix_pages) must have equal lengths")
+        if group_sizes is None:
+            if len(pl) > 1:
+                raise ValueError("several prefixes need group_sizes")
+            gs = _i32([len(ql)])
+            if len(pl) == 0:
+                pl, prefix_pages = _i32([0]), [[]]
+        else:
+            gs = _i32(group_sizes)
+            if len(gs) != len(pl):
+                raise ValueError("group_sizes and prefix_lens must have equal lengths")
+
+        def flat(lists, lens):
+            need = -(-lens.astype(np.int64) // ps)
+            if any(len(p) < k for p, k in zip(lists, need)):
+                raise ValueError("a page list is shorter than its length needs")
+            return _i32([x for p, k in zip(lists, need.tolist()) for x in p[:k]])
+
+        op, pp = flat(own_pages, ol), flat(prefix_pages, pl)
+        self._check(self._lib.rv_step_plan(self._h, len(ql), ql.ctypes.data, ol.ctypes.data, op.ctypes.data, len(gs),
+                                           gs.ctypes.data, pl.ctypes.data, pp.ctypes.data, num_pages, bool(causal),
+                                           _stream(stream, self.device)))
+        self.tokens = int(ql.sum())
+
+    def append(self, cache: PagedCache, q, k, v, cos, sin, *, q_out=None, interleaved: bool = False,
+               stream: int | None = None):
+        """``rv_step_append``: rotates ``q [tokens, q_heads, head_dim]`` and ``k [tokens, kv_heads, head_dim]``
+        by ``cos`` / ``sin [positions, rot / 2]`` (f32) and writes keys and values into the cache; returns
+        the rotated queries (``q_out``, a new tensor by default; it may be ``q``).  ``q = None`` appends
+        keys and values only."""
+        t, d = self._tokens(), self.head_dim
+        if q is not None:
+            _rows("q", q, t, self.q_heads, d, cache.dtype, cache.device)
+            if q_out is None:
+                q_out = torch.empty((t, self.q_heads, d), dtype=q.dtype, device=q.device)
+            _rows("q_out", q_out, t, self.q_heads, d, cache.dtype, cache.device)
+            qa = (q.data_ptr(), q.stride(0), q.stride(1))
+            qo = (q_out.data_ptr(), q_out.stride(0), q_out.stride(1))
+        elif q_out is not None:
+            raise ValueError("q_out without q")
+        else:
+            qa = qo = (None, 0, 0)
+        _rows("k", k, t, self.kv_heads, d, cache.dtype, cache.device)
+        _rows("v", v, t, self.kv_heads, d, cache.dtype, cache.device)
+        if cos.shape != sin.shape or cos.ndim != 2 or cos.dtype != torch.float32 or sin.dtype != torch.float32 \
+                or cos.device != cache.device or sin.device != cache.device or not cos.is_contiguous() \
+                or not sin.is_contiguous():
+            raise ValueError("cos and sin must be contiguous [positions, rot / 2] f32 tensors on the cache's device")
+        rc = self._lib.rv_step_append(self._h, cache._ref, *qa, k.data_ptr(), k.stride(0), k.stride(1), v.data_ptr(),
+                                      v.stride(0), v.stride(1), *qo, cos.data_ptr(), sin.data_ptr(), cos.shape[0],
+                                      2 * cos.shape[1], interleaved, _stream(stream, cache.device))
+        if rc:
+            self._check(rc)
+        return q_out
+
+    def attend(self, cache: PagedCache, q, *, out=None, lse=None, scale: float | None = None,
+               stream: int | None = None):
+        """``rv_step_attend``: attention of every query of the step over its group's prefix and its own keys
+        (``scale`` 1 / sqrt(head_dim) by default).  ``lse [tokens, q_heads]`` f32, where given, receives the
+        log of the softmax's denominator.  Returns ``out [tokens, q_heads, head_dim]``."""
+        t, d = self._tokens(), self.head_dim
+        _rows("q", q, t, self.q_heads, d, cache.dtype, cache.device)
+        if out is None:
+            out = torch.empty((t, self.q_heads, d), dtype=q.dtype, device=q.device)
+        else:
+            _rows("out", out, t, self.q_heads, d, cache.dtype, cache.device)
+        if lse is not None and (lse.shape != (t, self.q_heads) or lse.dtype != torch.float32
+                                or lse.device != cache.device or not lse.is_contiguous()):
+            raise ValueError(f"lse must be a contiguous [{t}, {self.q_heads}] f32 tensor on the cache's device")
+        rc = self._lib.rv_step_attend(self._h, cache._ref, q.data_ptr(), q.stride(0), q.stride(1), out.data_ptr(),
+                                      out.stride(0), out.stride(1), None if lse is None else lse.data_ptr(),
+                                      d ** -0.5 if scale is None else scale, _stream(stream, cache.device))
+        if rc:
+            self._check(rc)
+        return out
+
+
+def rms_norm(x, weight, *, residual=None, residual_out=None, out=None, eps: float = 1e-5, out_8bit: bool = False,
+             group: int = 0, scales=None, stream: int | None = None):
+    """``rv_rms_norm`` over the rows of ``x [rows, hidden]`` (bf16 or f16, ``weight`` f32): ``h = x + residual``,
+    ``out = h / sqrt(mean(h^2) + eps) * weight``; ``h`` in 16 bits goes to ``residual_out`` where given (it may
+    be ``residual`` or ``x``).  Returns ``(out, scales)``: 16-bit rows and ``None``, or with ``out_8bit`` e4m3
+    codes and their f32 scales ``[rows, hidden / group]`` (``group = 0``: one scale a row)."""
+    if x.ndim != 2 or x.dtype not in _DTYPES or not x.is_cuda or (x.shape[1] > 1 and x.stride(1) != 1):
+        raise ValueError("x must be a 2-D bf16 or f16 CUDA tensor with unit stride along the last axis")
+    rows, hidden = x.shape
+    if weight.shape != (hidden,) or weight.dtype != torch.float32 or weight.device != x.device \
+            or not weight.is_contiguous():
+        raise ValueError("weight must be a contiguous f32 [hidden] tensor on x's device")
+    for name, t in (("residual", residual), ("residual_out", residual_out)):
+        if t is not None and (t.shape != x.shape or t.dtype != x.dtype or t.device != x.device
+                              or (hidden > 1 and t.stride(1) != 1)):
+            raise ValueError(f"{name} must be like x, with unit stride along the last axis")
+    if group and (not out_8bit or group not in (32, 64, 128, 256) or hidden % group):
+        raise ValueError("group must be 32, 64, 128 or 256, divide hidden, and comes with out_8bit")
+    dt = torch.float8_e4m3fn if out_8bit else x.dtype
+    if out is None:
+        out = torch.empty((rows, hidden), dtype=dt, device=x.device)
+    elif out.shape != x.shape or out.dtype != dt or out.device != x.device or (hidden > 1 and out.stride(1) != 1):
+        raise ValueError(f"out must be [{rows}, {hidden}] {dt} on x's device, with unit stride along the last axis")
+    shape = (rows, hidden // group if group else 1)
+    if not out_8bit:
+        if scales is not None:
+            raise ValueError("scales come with out_8bit")
+    elif scales is None:
+        scales = torch.empty(shape, dtype=torch.float32, device=x.device)
+    elif scales.shape != shape or scales.dtype != torch.float32 or scales.device != x.device \
+            or not scales.is_contiguous():
+        raise ValueError(f"scales must be a contiguous {shape} f32 tensor on x's device")
+    if rows == 0:
+        return out, scales
+    code = _DTYPES[x.dtype]
+    with torch.cuda.device(x.device):
+        rc = L.lib().rv_rms_norm(code, x.data_ptr(), x.stride(0), L.ptr(residual),
+                                 0 if residual is None else residual.stride(0), weight.data_ptr(), L.ptr(residual_out),
+                                 0 if residual_out is None else residual_out.stride(0), out.data_ptr(), out.stride(0),
+                                 L.RV_DTYPE_E4M3 if out_8bit else code, L.ptr(scales), group, rows, hidden, eps,
+                                 _stream(stream, x.device))
+    if rc != L.RV_OK:
+        raise L.RvError(rc, "rv_rms_norm failed (hidden from 1 to 65536, row strides of at least hidden, eps >= 0)")
+    return out, scales
