@@ -1,0 +1,599 @@
+// Attention of many query rows (prompts, rerank batches, and all sequences' rows against a shared prefix) over
+// paged keys, on the 5th-generation tensor cores.
+//
+// Work = (item, group of `fold` query heads): up to two 128-row tiles, rows being the `fold` heads of
+// consecutive tokens, against the item's key tiles of 128 keys (prefix tiles, then the sequence's own).  The
+// kernel is persistent, one CTA per SM; both row tiles share every K and V tile that a CTA loads.  Warp roles:
+//   warps 0..3, 4..7  softmax of row tile 0, 1: one row per thread,
+//   warp 8            TMA of Q and K, warp 9 TMA of V: page by page into rings of 128-key slots,
+//   warp 10           TMEM owner and issuer of the tcgen05.mma.
+// Per key tile and row tile i:
+//   S_i = Q_i K^T     tcgen05.mma M=128 N<=128 into TMEM columns of its own,
+//   softmax           scores by tcgen05.ld, masks, P = exp2(s - m) in 16 bits over S_i (tcgen05.st),
+//   O_i += P V        P from TMEM, V as an MN-major operand, in two halves of 64 keys, so that the first half
+//                     multiplies while the second half's exponentials are computed.
+// While one row tile's softmax runs, the tensor cores work on the other.  The reference maximum m moves only
+// when a row's maximum grows by more than 2^8; then the row's O is rescaled in TMEM.  S of a tile is issued
+// after P V of the tile before it by the same thread, so the barrier that announces S also means that the
+// earlier P V is done: rescaling needs no wait of its own.  An item's O is read out after the next item's
+// first P is written, before that item's first P V.
+#include <algorithm>
+
+#include "step_attend.cuh"
+
+namespace rv {
+
+namespace {
+
+constexpr int kSoftmaxWarps = 8;
+constexpr int kThreads = 384;   // three warpgroups; warp 11 only takes part in the register split
+// Registers a thread: the softmax warpgroups hold a row of 128 scores each and take some of the third's.  The
+// launch must bring what the split adds up to (checked before the first launch): 2 * 208 + 88 = 3 * 168.
+constexpr int kLaunchRegs = 168, kSoftmaxRegs = 208, kOtherRegs = 88;
+static_assert(2 * kSoftmaxRegs + kOtherRegs <= 3 * kLaunchRegs, "register split");
+constexpr int kTmemCols = 512;  // S0, S1 at 0, 128; O0, O1 at 256, 384
+
+template <int D>
+constexpr int kStages = D == 128 ? 2 : 4;  // of K and of V
+template <int D>
+constexpr int kQBytes = kTileRows * D * 2;
+template <int D>
+constexpr int kKeyBytes = kTileKeys * D * 2;
+template <int D>
+constexpr int kSmemBytes = 1024 + 2 * kQBytes<D> + 2 * kStages<D> * kKeyBytes<D> + 512;
+
+// MN-major operand of 64-value blocks with 128-byte swizzling: 8-row groups of 1024 bytes along K, blocks of
+// 64 values `block_bytes` apart along N.
+__device__ __forceinline__ uint64_t desc_mn(uint32_t saddr, uint32_t block_bytes) {
+  uint64_t d = 0;
+  d |= static_cast<uint64_t>((saddr & 0x3FFFFu) >> 4);
+  d |= static_cast<uint64_t>(block_bytes >> 4) << 16;
+  d |= static_cast<uint64_t>(1024u >> 4) << 32;
+  d |= static_cast<uint64_t>(1u) << 46;
+  d |= static_cast<uint64_t>(2u) << 61;
+  return d;
+}
+
+__device__ __forceinline__ void fence_async_shared() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
+
+// Completion wait that ignores the abort flag (bounded by time): lets copies and MMAs in flight finish.
+__device__ __forceinline__ bool wait_done(uint64_t* bar, uint32_t parity) {
+  volatile int no_abort = 0;
+  return mbar_wait(bar, parity, &no_abort);
+}
+
+// The items of one CTA: rounds over all CTAs, every other one backwards, so that items ordered by their work
+// spread evenly.  The next item's record is brought into L1 ahead of its use.
+struct Walk {
+  int w, round;
+  int hg;
+  StepItem it;
+  int tiles;     // key tiles
+  int count[2];  // of which row tile 0, 1 takes this many (0: no tokens)
+
+  __device__ __forceinline__ static int index(int round) {
+    return round * gridDim.x + ((round & 1) ? gridDim.x - 1 - blockIdx.x : blockIdx.x);
+  }
+  __device__ __forceinline__ void load(const AttendParams& p, int total) {
+    if (w >= total) return;
+    const int groups = p.q_heads / p.fold;
+    hg = w % groups;
+    it = p.items[w / groups];
+    const int nw = index(round + 1);
+    if (nw < total) {
+      const char* nx = reinterpret_cast<const char*>(&p.items[nw / groups]);
+      asm volatile("prefetch.global.L1 [%0];" ::"l"(nx));
+      asm volatile("prefetch.global.L1 [%0];" ::"l"(nx + 32));
+    }
+    const int na = (it.a1 - it.a0 + kTileKeys - 1) / kTileKeys;
+    const int per = kTileRows / p.fold;  // tokens of a row tile
+    tiles = 0;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      count[i] = 0;
+      if (i * per >= it.n) continue;
+      // Own keys that the row tile's last token sees; a row tile that sees none still takes one tile, all
+      // masked, which gives its rows their empty result.
+      const int lim = min(it.b1, it.diag + min(it.n, (i + 1) * per));
+      count[i] = max(1, na + (max(0, lim - it.b0) + kTileKeys - 1) / kTileKeys);
+      tiles = max(tiles, count[i]);
+    }
+  }
+  __device__ __forceinline__ void init(const AttendParams& p, int total) {
+    round = 0;
+    w = index(0);
+    load(p, total);
+  }
+  __device__ __forceinline__ void next(const AttendParams& p, int total) {
+    ++round;
+    w = index(round);
+    load(p, total);
+  }
+  // Keys of tile t that row tile i can see, at least 1 (masked then).
+  __device__ __forceinline__ int seen(const AttendParams& p, const KeyTile& t, int i) const {
+    if (!t.own) return t.valid;
+    const int last = min(it.n, (i + 1) * (kTileRows / p.fold));
+    return max(1, min(t.valid, it.diag + last - t.base));
+  }
+};
+
+template <typename T, int D>
+__global__ void __launch_bounds__(kThreads, 1) attend_tiles_kernel(const __grid_constant__ CUtensorMap mq,
+                                                                   const __grid_constant__ CUtensorMap mk,
+                                                                   const __grid_constant__ CUtensorMap mv,
+                                                                   const AttendParams p) {
+  constexpr int kHalves = D / 64;
+  constexpr int kSt = kStages<D>;
+  constexpr bool kBf = Elem<T>::kBf16;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint8_t* sQ = smem;                            // [2]
+  uint8_t* sK = sQ + 2 * kQBytes<D>;             // [kSt]
+  uint8_t* sV = sK + kSt * kKeyBytes<D>;         // [kSt]
+  uint64_t* bar = reinterpret_cast<uint64_t*>(sV + kSt * kKeyBytes<D>);
+  uint64_t* q_full = bar;              // [2] Q of the row tile landed
+  uint64_t* q_empty = q_full + 2;      // [2] its last S is done
+  uint64_t* k_full = q_empty + 2;      // [kSt]
+  uint64_t* k_empty = k_full + kSt;    // [kSt] both row tiles' S are done
+  uint64_t* v_full = k_empty + kSt;    // [kSt]
+  uint64_t* v_empty = v_full + kSt;    // [kSt] both row tiles' P V are done
+  uint64_t* s_full = v_empty + kSt;    // [2] scores in TMEM
+  uint64_t* p_full = s_full + 2;       // [2][2] P of the row tile, keys 0-63 and 64-127
+  uint64_t* o_full = p_full + 4;       // [2] last P V of the item done
+  uint64_t* o_empty = o_full + 2;      // [2] the item's O has been read
+  uint64_t* drain = o_empty + 2;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain + 1);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+  static_assert((2 + 2 + 4 * kSt + 2 + 4 + 2 + 2 + 1) * 8 + 8 <= 512, "barrier area");
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int total = p.n_items * (p.q_heads / p.fold);
+  const int per = kTileRows / p.fold;  // tokens of a row tile
+
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&q_full[i], 1);
+      mbar_init(&q_empty[i], 1);
+      mbar_init(&s_full[i], 1);
+      mbar_init(&p_full[2 * i], 4);
+      mbar_init(&p_full[2 * i + 1], 4);
+      mbar_init(&o_full[i], 1);
+      mbar_init(&o_empty[i], 4);
+    }
+    for (int s = 0; s < kSt; ++s) {
+      mbar_init(&k_full[s], 1);
+      mbar_init(&k_empty[s], 1);
+      mbar_init(&v_full[s], 1);
+      mbar_init(&v_empty[s], 1);
+    }
+    mbar_init(drain, 1);
+    *abort_flag = 0;
+    fence_mbar_init();
+    tma_prefetch_desc(&mq);
+    tma_prefetch_desc(&mk);
+    tma_prefetch_desc(&mv);
+  }
+  if (warp == 10) {
+    tmem_alloc(tmem_slot, kTmemCols);
+    tmem_relinquish();
+    tc_fence_before();
+  }
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+
+  if (warp >= 8) {
+  asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kOtherRegs));
+  if (warp == 8 || warp == 9) {
+    // ---------------------------------------------------------------- TMA producers
+    const bool keys = warp == 8;
+    uint8_t* ring = keys ? sK : sV;
+    uint64_t* full = keys ? k_full : v_full;
+    uint64_t* empty = keys ? k_empty : v_empty;
+    Walk wk;
+    wk.init(p, total);
+    int s = 0, loaded = 0, q_loads[2] = {0, 0};
+    uint32_t ph = 0;
+    bool ok = true;
+    int page = 0;
+    KeyTile t{};
+    if (wk.w < total) {
+      t = key_tile<kTileKeys>(wk.it, 0);
+      page = TileCopy<kTileKeys, kHalves>::page_of(p, t, lane);
+    }
+    while (ok && wk.w < total) {
+      if (keys) {
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          if (!ok || !wk.count[i]) continue;
+          ok = __all_sync(0xffffffffu, mbar_wait(&q_empty[i], (q_loads[i] & 1) ^ 1u, abort_flag));
+          if (!ok) continue;
+          if (lane == 0) {
+            mbar_arrive_expect_tx(&q_full[i], per * p.fold * D * 2);
+            for (int h = 0; h < kHalves; ++h)
+              tma_load_3d(sQ + i * kQBytes<D> + h * (kTileRows * 128), &mq, &q_full[i], 64 * h, wk.hg * p.fold,
+                          wk.it.tok0 + i * per);
+          }
+          ++q_loads[i];
+        }
+      }
+      for (int j = 0; ok && j < wk.tiles; ++j) {
+        const int hg = wk.hg;
+        const bool last = j + 1 == wk.tiles;
+        const int n = TileCopy<kTileKeys, kHalves>::copies(t, p.box);
+        ok = __all_sync(0xffffffffu, mbar_wait(&empty[s], ph ^ 1u, abort_flag));
+        if (!ok) break;
+        if (lane == 0) mbar_arrive_expect_tx(&full[s], n * p.box * D * 2);
+        __syncwarp();
+        TileCopy<kTileKeys, kHalves>::issue(p, t, page, lane, ring + s * kKeyBytes<D>, keys ? &mk : &mv, &full[s],
+                                            hg / p.per_kv);
+        ++loaded;
+        if (++s == kSt) {
+          s = 0;
+          ph ^= 1u;
+        }
+        // The next tile's page numbers are on their way before the wait for its slot.
+        if (last) break;
+        t = key_tile<kTileKeys>(wk.it, j + 1);
+        page = TileCopy<kTileKeys, kHalves>::page_of(p, t, lane);
+      }
+      wk.next(p, total);
+      if (wk.w < total) {
+        t = key_tile<kTileKeys>(wk.it, 0);
+        page = TileCopy<kTileKeys, kHalves>::page_of(p, t, lane);
+      }
+    }
+    if (!ok && lane == 0) {
+      *abort_flag = 1;
+      atomicOr_system(p.err, kErrWaitTimeout);
+    }
+    // Every copy lands before the CTA leaves, also when another role gave up before using it.
+    for (int j = max(0, loaded - kSt); j < loaded; ++j) wait_done(&full[j % kSt], (j / kSt) & 1);
+    if (keys)
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+        if (q_loads[i]) wait_done(&q_full[i], (q_loads[i] - 1) & 1);
+  } else if (warp == 10) {
+    // ---------------------------------------------------------------- MMA issuer
+    Walk ws, wp;  // ws: the step (item, key tile) whose S is issued next, one ahead of P V's
+    ws.init(p, total);
+    wp.init(p, total);
+    int js = 0, jp = 0;              // key tile within the item
+    int ks = 0, vs = 0;              // ring slots
+    uint32_t kph = 0, vph = 0;
+    uint32_t q_ph = 0, p_ph = 0, oe_ph = 0;  // parity bits by row tile
+    bool ok = true;
+    const uint64_t dq = smem_desc_sw128(smem_u32(sQ)), dk = smem_desc_sw128(smem_u32(sK));
+    const uint64_t dv = desc_mn(smem_u32(sV), kTileKeys * 128);
+    // S_i of the step at ws.
+    auto issue_s = [&](int i, const KeyTile& t) {
+      if (js == 0) {
+        if (!__all_sync(0xffffffffu, mbar_wait(&q_full[i], (q_ph >> i) & 1, abort_flag))) return false;
+        q_ph ^= 1u << i;
+      }
+      tc_fence_after();
+      if (lane == 0) {
+        const uint32_t id = idesc_f16(kTileRows, (ws.seen(p, t, i) + 15) & ~15, kBf);
+        const uint64_t a = dq + static_cast<uint64_t>(i * (kQBytes<D> >> 4));
+        const uint64_t b = dk + static_cast<uint64_t>(ks * (kKeyBytes<D> >> 4));
+#pragma unroll
+        for (int k = 0; k < D / 16; ++k) {
+          const uint64_t off = (k / 4) * (kTileRows * 128 >> 4) + 2 * (k % 4);
+          tc_mma_f16(tmem + i * 128, a + off, b + off, id, k > 0);
+        }
+        tc_commit(&s_full[i]);
+        if (js == ws.count[i] - 1) tc_commit(&q_empty[i]);
+      }
+      __syncwarp();
+      return true;
+    };
+    // Both row tiles' part in K of the step is issued: release the slot, move on.
+    auto end_s = [&]() {
+      if (lane == 0) tc_commit(&k_empty[ks]);
+      __syncwarp();
+      if (++ks == kSt) {
+        ks = 0;
+        kph ^= 1u;
+      }
+      if (++js == ws.tiles) {
+        js = 0;
+        ws.next(p, total);
+      }
+    };
+    auto wait_k = [&]() { return __all_sync(0xffffffffu, mbar_wait(&k_full[ks], kph, abort_flag)); };
+    if (ws.w < total) {
+      const KeyTile t = key_tile<kTileKeys>(ws.it, 0);
+      ok = wait_k();
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+        if (ok && js < ws.count[i]) ok = issue_s(i, t);
+      if (ok) end_s();
+    }
+    while (ok && wp.w < total) {
+      const KeyTile t = key_tile<kTileKeys>(wp.it, jp);
+      const bool more = ws.w < total;
+      KeyTile ts{};
+      if (more) ts = key_tile<kTileKeys>(ws.it, js);
+      bool have_k = false, have_v = false;
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        if (jp < wp.count[i]) {
+          if (jp == 0) {
+            // The previous item's O has been read out of the accumulator.
+            ok = __all_sync(0xffffffffu, mbar_wait(&o_empty[i], ((oe_ph >> i) & 1) ^ 1u, abort_flag));
+            if (!ok) break;
+            oe_ph ^= 1u << i;
+          }
+          if (!have_v) {
+            ok = __all_sync(0xffffffffu, mbar_wait(&v_full[vs], vph, abort_flag));
+            if (!ok) break;
+            have_v = true;
+            const int upto = (t.valid + 15) & ~15;
+            if (t.valid < upto) {
+              // What lies past the last key may be anything, NaN included, and meets weights of 0: clear it.
+              for (int c = lane; c < (upto - t.valid) * kHalves * 8; c += 32) {
+                const int row = t.valid + c / (kHalves * 8), h = c / 8 % kHalves;
+                *reinterpret_cast<uint4*>(sV + vs * kKeyBytes<D> + h * (kTileKeys * 128) + row * 128 + c % 8 * 16) =
+                    make_uint4(0, 0, 0, 0);
+              }
+              fence_async_shared();
+              __syncwarp();
+            }
+          }
+          const int n16 = (wp.seen(p, t, i) + 15) >> 4;
+          const uint64_t b = dv + static_cast<uint64_t>(vs * (kKeyBytes<D> >> 4));
+          constexpr uint32_t id = idesc_f16(kTileRows, D, kBf) | (1u << 16);
+#pragma unroll
+          for (int half = 0; half < 2; ++half) {
+            ok = __all_sync(0xffffffffu, mbar_wait_spin(&p_full[2 * i + half], (p_ph >> i) & 1, abort_flag));
+            if (!ok) break;
+            tc_fence_after();
+            if (lane == 0) {
+#pragma unroll
+              for (int k = 4 * half; k < 4 * half + 4; ++k)
+                if (k < n16)
+                  tc_mma_f16_ts(tmem + 256 + i * 128, tmem + i * 128 + 8 * k, b + 128 * k, id, jp > 0 || k > 0);
+            }
+            __syncwarp();
+          }
+          if (!ok) break;
+          p_ph ^= 1u << i;
+          if (jp == wp.count[i] - 1 && lane == 0) tc_commit(&o_full[i]);
+          __syncwarp();
+        }
+        if (more && js < ws.count[i]) {
+          if (!have_k) {
+            ok = wait_k();
+            if (!ok) break;
+            have_k = true;
+          }
+          ok = issue_s(i, ts);
+          if (!ok) break;
+        }
+      }
+      if (!ok) break;
+      if (lane == 0) tc_commit(&v_empty[vs]);
+      __syncwarp();
+      if (++vs == kSt) {
+        vs = 0;
+        vph ^= 1u;
+      }
+      if (more) end_s();
+      if (++jp == wp.tiles) {
+        jp = 0;
+        wp.next(p, total);
+      }
+    }
+    if (lane == 0) {
+      if (!ok) {
+        *abort_flag = 1;
+        atomicOr_system(p.err, kErrWaitTimeout);
+      }
+      tc_commit(drain);  // every MMA is done before TMEM is released
+    }
+    __syncwarp();
+    if (!wait_done(drain, 0) && lane == 0) atomicOr_system(p.err, kErrWaitTimeout);
+  }
+  } else {
+    // ---------------------------------------------------------------- softmax
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSoftmaxRegs));
+    const int i = warp >> 2;                       // row tile
+    const int r = (warp & 3) * 32 + lane;          // row = TMEM lane
+    const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
+    const uint32_t ts = tmem + lanes + i * 128, to = tmem + lanes + 256 + i * 128;
+    const int my_tok = i * per + r / p.fold, my_head = r % p.fold;
+    constexpr float kRescale = 8.f;  // P stays below 2^8
+    constexpr float kNone = -1e30f;  // no key seen yet
+    const uint64_t sl2 = f2_pack(p.scale_log2, p.scale_log2);
+    Walk wk;
+    wk.init(p, total);
+    uint32_t s_ph = 0, o_ph = 0;
+    bool fail = false, fin = false, fin_live = false;
+    float fin_l = 0.f, fin_m = 0.f;
+    int fin_tok = 0, fin_head = 0, fin_part = 0;
+    // Writes the finished item's row: O / l from TMEM.
+    auto read_out = [&]() {
+      const bool none = fin_l == 0.f;  // the row saw no key
+      const float inv = 1.f / fin_l;
+      StepParts pt{0, 1};
+      int64_t at = 0;
+      T* dst = nullptr;
+      float* part = nullptr;
+      if (fin_live) {
+        pt = p.parts[fin_tok];
+        const float ls = none ? -INFINITY : fin_m + log2f(fin_l);
+        if (pt.count == 1) {
+          dst = static_cast<T*>(p.out) + fin_tok * p.out_token + fin_head * p.out_head;
+          if (p.lse) p.lse[int64_t(fin_tok) * p.q_heads + fin_head] = ls * 0.6931471805599453f;
+        } else {
+          at = int64_t(pt.first + fin_part) * p.q_heads + fin_head;
+          part = p.part_o + at * D;
+          p.part_l[at] = ls;
+        }
+      }
+#pragma unroll
+      for (int c = 0; c < D / 32; ++c) {
+        float t[32];
+        tmem_ld32(to + 32 * c, t);
+        tc_wait_ld();
+#pragma unroll
+        for (int e = 0; e < 32; ++e) t[e] = none ? 0.f : t[e] * inv;
+        if (dst) {
+#pragma unroll
+          for (int e = 0; e < 4; ++e) reinterpret_cast<uint4*>(dst + 32 * c)[e] = pack8<T>(t + 8 * e);
+        } else if (part) {
+#pragma unroll
+          for (int e = 0; e < 8; ++e)
+            reinterpret_cast<float4*>(part + 32 * c)[e] = make_float4(t[4 * e], t[4 * e + 1], t[4 * e + 2], t[4 * e + 3]);
+        }
+      }
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&o_empty[i]);
+      fin = false;
+    };
+    while (!fail && wk.w < total) {
+      const int n = i ? wk.count[1] : wk.count[0];
+      float m = kNone, l = 0.f;
+      const int own = wk.it.diag + my_tok + 1;  // own keys that the row sees
+      for (int j = 0; j < n; ++j) {
+        const KeyTile t = key_tile<kTileKeys>(wk.it, j);
+        const int lim = min(t.valid, t.own ? own - t.base : t.valid);  // the row's visible keys: those below
+        const int n16 = (wk.seen(p, t, i) + 15) & ~15;               // columns that S has
+        fail = !__all_sync(0xffffffffu, mbar_wait(&s_full[i], s_ph, abort_flag));
+        if (fail) break;
+        s_ph ^= 1u;
+        tc_fence_after();
+        float s[4][32];
+#pragma unroll
+        for (int c = 0; c < 4; ++c)
+          if (32 * c < n16) tmem_ld32(ts + 32 * c, s[c]);
+        tc_wait_ld();
+        float mt = -INFINITY;
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          if (32 * c >= n16) continue;
+          const int k = lim - 32 * c;
+          if (!__all_sync(0xffffffffu, k >= 32)) {
+            const uint32_t vis = k <= 0 ? 0u : k >= 32 ? 0xffffffffu : (1u << k) - 1u;
+#pragma unroll
+            for (int e = 0; e < 32; ++e)
+              if (!((vis >> e) & 1u)) s[c][e] = -INFINITY;
+          }
+          float mx[4] = {fmax3(s[c][0], s[c][1], s[c][2]), fmax3(s[c][3], s[c][4], s[c][5]),
+                         fmax3(s[c][6], s[c][7], s[c][8]), fmax3(s[c][9], s[c][10], s[c][11])};
+#pragma unroll
+          for (int e = 12; e < 32; e += 2) mx[(e >> 1) & 3] = fmax3(mx[(e >> 1) & 3], s[c][e], s[c][e + 1]);
+          mt = fmaxf(mt, fmax3(mx[0], mx[1], fmaxf(mx[2], mx[3])));
+        }
+        mt *= p.scale_log2;
+        const bool need = m != kNone && mt > m + kRescale;
+        if (m == kNone) m = fmaxf(m, mt);
+        if (__any_sync(0xffffffffu, need)) {
+          // P V of the tile before is done (see above) and this tile's has not been issued.
+          const float alpha = need ? ex2_approx(m - mt) : 1.f;
+#pragma unroll
+          for (int c = 0; c < D / 16; ++c) {
+            float o[16];
+            tmem_ld16(to + 16 * c, o);
+            tc_wait_ld();
+            uint32_t w[16];
+#pragma unroll
+            for (int e = 0; e < 16; ++e) w[e] = __float_as_uint(o[e] * alpha);
+            tmem_st16(to + 16 * c, w);
+          }
+          tc_wait_st();
+          if (need) {
+            l *= alpha;
+            m = mt;
+          }
+        }
+        const uint64_t nm2 = f2_pack(-m, -m);
+        uint64_t ps[2] = {0ull, 0ull};
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          if (32 * c < n16) {
+            uint32_t w[16];
+#pragma unroll
+            for (int e = 0; e < 16; ++e) {
+              float x0, x1;
+              f2_unpack(f2_fma(f2_pack(s[c][2 * e], s[c][2 * e + 1]), sl2, nm2), x0, x1);
+              const float p0 = ex2_approx(x0), p1 = ex2_approx(x1);
+              ps[e & 1] = f2_add(ps[e & 1], f2_pack(p0, p1));
+              auto v = Elem<T>::pack(p0, p1);
+              w[e] = *reinterpret_cast<uint32_t*>(&v);
+            }
+            tmem_st16(ts + 16 * c, w);
+          }
+          if (c & 1) {
+            tc_wait_st();
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&p_full[2 * i + (c >> 1)]);
+          }
+        }
+        float p0, p1, p2, p3;
+        f2_unpack(ps[0], p0, p1);
+        f2_unpack(ps[1], p2, p3);
+        l += (p0 + p1) + (p2 + p3);
+        if (fin) read_out();  // S of this item means that the last item's P V are done
+      }
+      if (fail) break;
+      if (n) {
+        fin = true;
+        fin_live = my_tok < wk.it.n && r < per * p.fold;
+        fin_l = l;
+        fin_m = m;
+        fin_tok = wk.it.tok0 + my_tok;
+        fin_head = wk.hg * p.fold + my_head;
+        fin_part = wk.it.part;
+        o_ph ^= 1u;
+      }
+      wk.next(p, total);
+    }
+    if (!fail && fin) {
+      fail = !__all_sync(0xffffffffu, mbar_wait(&o_full[i], o_ph ^ 1u, abort_flag));
+      if (!fail) {
+        tc_fence_after();
+        read_out();
+      }
+    }
+    if (fail && lane == 0) {
+      *abort_flag = 1;
+      atomicOr_system(p.err, kErrWaitTimeout);
+    }
+  }
+  __syncthreads();
+  if (warp == 10) {
+    tc_fence_after();
+    tmem_dealloc(tmem, kTmemCols);
+  }
+}
+
+template <typename T, int D>
+cudaError_t launch(const CUtensorMap& mq, const CUtensorMap& mk, const CUtensorMap& mv, const AttendParams& p,
+                   cudaStream_t st) {
+  static PerDeviceOnce once;
+  const cudaError_t e = once.run([] {
+    cudaFuncAttributes attr;
+    const cudaError_t g = cudaFuncGetAttributes(&attr, attend_tiles_kernel<T, D>);
+    if (g != cudaSuccess) return g;
+    if (attr.numRegs != kLaunchRegs) return cudaErrorInvalidConfiguration;  // the split would wait forever
+    return cudaFuncSetAttribute(attend_tiles_kernel<T, D>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemBytes<D>);
+  });
+  if (e != cudaSuccess) return e;
+  const int total = p.n_items * (p.q_heads / p.fold);
+  attend_tiles_kernel<T, D><<<std::min(total, device_sm_count()), kThreads, kSmemBytes<D>, st>>>(mq, mk, mv, p);
+  return cudaGetLastError();
+}
+
+}  // namespace
+
+cudaError_t attend_tiles(Act act, int head_dim, const CUtensorMap& mq, const CUtensorMap& mk, const CUtensorMap& mv,
+                         const AttendParams& p, cudaStream_t st) {
+  if (act == Act::kBf16)
+    return head_dim == 64 ? launch<__nv_bfloat16, 64>(mq, mk, mv, p, st) : launch<__nv_bfloat16, 128>(mq, mk, mv, p, st);
+  return head_dim == 64 ? launch<__half, 64>(mq, mk, mv, p, st) : launch<__half, 128>(mq, mk, mv, p, st);
+}
+
+}  // namespace rv

@@ -3,6 +3,7 @@
 // every layer.
 #include "decode.h"
 
+#include <algorithm>
 #include <climits>
 #include <cmath>
 #include <cstring>
@@ -10,6 +11,7 @@
 #include <mutex>
 #include <new>
 #include <string>
+#include <utility>
 #include <vector>
 
 #include "../../include/ripvec_b200.h"
@@ -42,6 +44,20 @@ constexpr int64_t kMaxKeys = int64_t(1) << 30;    // of one sequence or prefix
 
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 
+// What one sequence's queries see: its tokens tok0 .. tok0 + n - 1, prefix keys [0, len_a) in the pages from
+// pg[pg_a] and own keys [0, len_b) in those from pg[pg_b], of which token i sees those below diag + i + 1.
+struct StepSeq {
+  int tok0, n, pg_a, len_a, pg_b, len_b, diag;
+};
+
+// The attention work of a plan.
+struct Schedule {
+  std::vector<rv::StepItem> row_items, tile_items;
+  std::vector<rv::StepParts> parts;  // by token
+  std::vector<int> joined;
+  int64_t n_parts = 0;
+};
+
 }  // namespace
 
 struct rv_step {
@@ -56,13 +72,25 @@ struct rv_step {
   int last_pos = -1;  // largest position of a new token
   char* meta = nullptr;
   size_t meta_cap = 0;
+  int fold = 1;  // query heads of a key/value head that share a row tile: the largest divisor up to kRowTile
   const rv::StepToken* tokens = nullptr;
-  const rv::StepSeq* seqs = nullptr;
-  const int* pages = nullptr;
+  const rv::StepParts* parts = nullptr;
+  const rv::StepItem *row_items = nullptr, *tile_items = nullptr;
+  const int *joined = nullptr, *pages = nullptr;
+  int n_row_items = 0, n_tile_items = 0, n_joined = 0;
+  float* work = nullptr;  // partial results
+  size_t work_cap = 0;    // floats
+  int64_t n_parts = 0;
+  unsigned int* err_host = nullptr;  // error word in mapped host memory: kernels write it, calls look at it
+  unsigned int* err_dev = nullptr;
   Staging staging[2];
   int turn = 0;
-  std::vector<char> host;
+  // host side of the plan, kept for its memory
+  std::vector<rv::StepToken> tok;
+  std::vector<StepSeq> seq;
+  std::vector<int> group_first, pg;
   std::vector<int> writer;  // by page: 1 + the sequence that writes to it
+  Schedule sched;
   // Calls on different streams wait for one another: plan, append and attend share the plan's device
   // records and the workspace.
   cudaEvent_t last = nullptr;
@@ -79,6 +107,15 @@ int fail(rv_step* s, int code, const std::string& why) {
 
 int cuda_fail(rv_step* s, const char* what, cudaError_t e) {
   return fail(s, e == cudaErrorMemoryAllocation ? RV_E_NOMEM : RV_E_CUDA, std::string(what) + ": " + cudaGetErrorString(e));
+}
+
+// An error that an earlier call's kernels reported (without waiting for those still queued).
+bool device_error(rv_step* s) {
+  volatile unsigned int* w = s->err_host;
+  if (!*w) return false;
+  *w = 0;
+  s->err = "a kernel of an earlier call gave up waiting: its outputs are not valid";
+  return true;
 }
 
 bool capturing(cudaStream_t st) {
@@ -126,10 +163,191 @@ std::string take_pool(const rv_step* s, const rv_kv_cache* c, rv::KvPool* out, r
 
 bool rows_aligned(const void* p, int64_t ts, int64_t hs) { return aligned16(p) && ts % 8 == 0 && hs % 8 == 0; }
 
+// ---------------------------------------------------------------- attention schedule
+// Attention work before its keys are split.
+struct Job {
+  rv::StepItem it;
+  bool packed;  // rows of several sequences against their prefix
+};
+
+int tiles_of(const rv::StepItem& it, int keys) {
+  return (it.a1 - it.a0 + keys - 1) / keys + (it.b1 - it.b0 + keys - 1) / keys;
+}
+
+// Cuts an item's key tiles into parts of at most `most` tiles of about equal length.
+template <class F>
+void cut(const rv::StepItem& it, int keys, int most, F&& emit) {
+  const int na = (it.a1 - it.a0 + keys - 1) / keys, n = tiles_of(it, keys);
+  const int parts = std::max(1, (n + most - 1) / most);
+  for (int k = 0; k < parts; ++k) {
+    const int lo = int(int64_t(n) * k / parts), hi = int(int64_t(n) * (k + 1) / parts);
+    rv::StepItem x = it;
+    x.a0 = std::min(it.a1, it.a0 + std::min(lo, na) * keys);
+    x.a1 = std::min(it.a1, it.a0 + std::min(hi, na) * keys);
+    x.b0 = std::min(it.b1, it.b0 + std::max(0, lo - na) * keys);
+    x.b1 = std::min(it.b1, it.b0 + std::max(0, hi - na) * keys);
+    x.part = k;
+    emit(x, parts);
+  }
+}
+
+// Time of a part of `tiles` key tiles in the tensor-core kernel, in key tiles of two row tiles: a lone row
+// tile leaves the tensor cores waiting for its softmax; starting and writing a part takes about two tiles.
+double tile_cost(const rv::StepItem& it, int tiles, int per) { return (it.n > per ? 1.0 : 0.7) * tiles + 2.0; }
+
+// The longest time of any SM when parts of at most `most` tiles are dealt out, longest first, forwards and
+// backwards in turn, as the kernel walks them.
+double makespan(const std::vector<Job>& jobs, int most, int per, int groups, int sms) {
+  std::vector<std::pair<double, int>> cost;  // by part, `groups` times each
+  for (const Job& j : jobs)
+    cut(j.it, rv::kTileKeys, most, [&](const rv::StepItem& x, int parts) {
+      cost.push_back({tile_cost(x, tiles_of(x, rv::kTileKeys), per) + (parts > 1 ? 1.0 : 0.0), groups});
+    });
+  std::sort(cost.begin(), cost.end(), [](const auto& a, const auto& b) { return a.first > b.first; });
+  std::vector<double> load(size_t(sms), 0.0);
+  int64_t w = 0;
+  for (const auto& c : cost)
+    for (int k = 0; k < c.second; ++k, ++w) {
+      const int64_t round = w / sms, at = w % sms;
+      load[size_t(round & 1 ? sms - 1 - at : at)] += c.first;
+    }
+  return *std::max_element(load.begin(), load.end());
+}
+
+// Longest part, in key tiles, for the tensor-core kernel's jobs.  Cutting keys costs a partial result and its
+// join, so it is done only where it shortens the kernel: with few jobs that each walk many keys.
+int choose_tile_cut(const std::vector<Job>& jobs, int per, int groups, int sms) {
+  int64_t total = 0;
+  int longest = 1;
+  for (const Job& j : jobs) {
+    const int n = tiles_of(j.it, rv::kTileKeys);
+    total += n;
+    longest = std::max(longest, n);
+  }
+  total *= groups;
+  // Enough work for every SM many times over, none of it long against an SM's share: leave it whole.
+  if (int64_t(longest) * sms * 4 <= total) return longest;
+  double best = makespan(jobs, longest, per, groups, sms);
+  int most = longest;
+  for (int k = 2; k <= 64; k += k < 12 ? 1 : k / 4) {
+    const int u = std::max(1, int((int64_t(longest) + k - 1) / k));
+    int64_t parts = 0;
+    for (const Job& j : jobs) parts += (tiles_of(j.it, rv::kTileKeys) + u - 1) / u;
+    if (parts * groups > int64_t(sms) * 16) break;
+    const double t = makespan(jobs, u, per, groups, sms);
+    if (t < 0.95 * best) {
+      best = t;
+      most = u;
+    }
+    if (u == 1) break;
+  }
+  return most;
+}
+
+// Longest part, in 64-key tiles, for the few-row kernel's jobs: about three parts for each of two CTAs an SM
+// where there is that much work, and at least 4 tiles, below which starting a CTA costs more than its keys.
+int choose_row_cut(const std::vector<Job>& jobs, int groups, int sms) {
+  int64_t total = 0;
+  for (const Job& j : jobs) total += tiles_of(j.it, rv::kRowKeys);
+  total *= groups;
+  return int(std::max<int64_t>(4, (total + 6 * sms - 1) / (6 * sms)));
+}
+
+// Divides a step's attention into items.  A sequence whose rows fill a row tile by themselves walks the prefix
+// and its own keys in one item, without partial results.  Sequences of few rows share the prefix: the rows of
+// all of them are packed into row tiles that read each prefix key once, and their own keys are separate items.
+void schedule(const std::vector<StepSeq>& seqs, const std::vector<int>& group_first, int n_tokens, int fold,
+              int groups, int sms, Schedule* out) {
+  const int per = rv::kTileRows / fold;
+  std::vector<Job> rows, tiles;
+  auto add = [&](bool to_rows, int tok0, int n, const StepSeq& s, bool prefix, bool own, int diag, bool packed) {
+    rv::StepItem it{};
+    it.tok0 = tok0;
+    it.n = n;
+    it.pg_a = s.pg_a;
+    it.a1 = prefix ? s.len_a : 0;
+    it.pg_b = s.pg_b;
+    it.b1 = own ? std::max(0, std::min<int>(s.len_b, int(std::min<int64_t>(INT_MAX / 2, int64_t(diag) + n)))) : 0;
+    it.diag = diag;
+    if (it.a1 == 0 && it.b1 == 0) return;
+    (to_rows ? rows : tiles).push_back({it, packed});
+  };
+  for (size_t g = 0; g + 1 < group_first.size(); ++g) {
+    int b = group_first[g];
+    const int end = group_first[g + 1];
+    while (b < end) {
+      // A run of sequences of few rows.
+      int e = b, live = 0, n = 0;
+      while (e < end && seqs[e].n * fold < rv::kTileRows / 2) {
+        live += seqs[e].n > 0;
+        n += seqs[e].n;
+        ++e;
+      }
+      if (live > 1 && seqs[b].len_a > 0) {
+        const int t0 = seqs[b].tok0;
+        // One kernel for all of a run, so that all its tokens get as many partials of the prefix.
+        if (n * fold <= rv::kRowTile) add(true, t0, n, seqs[b], true, false, 0, true);
+        else
+          for (int t = 0; t < n; t += 2 * per) add(false, t0 + t, std::min(2 * per, n - t), seqs[b], true, false, 0, true);
+        for (; b < e; ++b)
+          if (seqs[b].n > 0)
+            add(seqs[b].n * fold <= rv::kRowTile, seqs[b].tok0, seqs[b].n, seqs[b], false, true, seqs[b].diag, false);
+        continue;
+      }
+      const StepSeq& s = seqs[b];
+      if (s.n * fold <= rv::kRowTile) {
+        if (s.n > 0) add(true, s.tok0, s.n, s, true, true, s.diag, false);
+      } else {
+        for (int t = 0; t < s.n; t += 2 * per)
+          add(false, s.tok0 + t, std::min(2 * per, s.n - t), s, true, true,
+              s.diag > INT_MAX / 4 ? s.diag : s.diag + t, false);
+      }
+      ++b;
+    }
+  }
+  // Parts: a token's partials are numbered through its items in order.
+  out->parts.assign(size_t(n_tokens), {0, 0});
+  const int row_cut = rows.empty() ? 1 : choose_row_cut(rows, groups, sms);
+  const int tile_cut = tiles.empty() ? 1 : choose_tile_cut(tiles, per, groups, sms);
+  auto emit = [&](const std::vector<Job>& jobs, bool packed, int keys, int most, std::vector<rv::StepItem>* items) {
+    for (const Job& j : jobs) {
+      if (j.packed != packed) continue;
+      const int base = out->parts[size_t(j.it.tok0)].count;
+      int count = 0;
+      cut(j.it, keys, most, [&](rv::StepItem x, int parts) {
+        count = parts;
+        x.part += base;
+        items->push_back(x);
+      });
+      for (int t = j.it.tok0; t < j.it.tok0 + j.it.n; ++t) out->parts[size_t(t)].count += count;
+    }
+  };
+  // Prefixes first: their items cut through sequences, and a sequence's tokens must agree in what came before
+  // the item of its own keys.
+  for (const bool packed : {true, false}) {
+    emit(tiles, packed, rv::kTileKeys, tile_cut, &out->tile_items);
+    emit(rows, packed, rv::kRowKeys, row_cut, &out->row_items);
+  }
+  std::stable_sort(out->tile_items.begin(), out->tile_items.end(), [&](const rv::StepItem& a, const rv::StepItem& b) {
+    return tile_cost(a, tiles_of(a, rv::kTileKeys), per) > tile_cost(b, tiles_of(b, rv::kTileKeys), per);
+  });
+  std::stable_sort(out->row_items.begin(), out->row_items.end(), [](const rv::StepItem& a, const rv::StepItem& b) {
+    return tiles_of(a, rv::kRowKeys) > tiles_of(b, rv::kRowKeys);
+  });
+  for (int t = 0; t < n_tokens; ++t) {
+    rv::StepParts& pt = out->parts[size_t(t)];
+    pt.first = int(out->n_parts);
+    if (pt.count == 1) continue;
+    out->joined.push_back(t);
+    out->n_parts += pt.count;
+  }
+}
+
 int plan(rv_step* s, int32_t n_seqs, const int32_t* q_lens, const int32_t* own_lens, const int32_t* own_pages,
          int32_t n_groups, const int32_t* group_sizes, const int32_t* prefix_lens, const int32_t* prefix_pages,
          int64_t num_pages, int32_t causal, cudaStream_t st) {
   s->planned = false;
+  if (device_error(s)) return RV_E_DEVICE;
   if (n_seqs < 0 || n_groups < 0 || num_pages < 0 || num_pages > INT_MAX || (n_seqs > 0 && (!q_lens || !own_lens)) ||
       (n_groups > 0 && (!group_sizes || !prefix_lens)))
     return fail(s, RV_E_INVALID, "null or negative argument");
@@ -161,25 +379,24 @@ int plan(rv_step* s, int32_t n_seqs, const int32_t* q_lens, const int32_t* own_l
   for (int64_t i = 0; i < n_own_pages; ++i)
     if (own_pages[i] < 0 || own_pages[i] >= num_pages) return fail(s, RV_E_INVALID, "page out of range");
 
-  const size_t o_tokens = 0, o_seqs = o_tokens + size_t(tokens) * sizeof(rv::StepToken);
-  const size_t o_pages = o_seqs + size_t(n_seqs) * sizeof(rv::StepSeq);
-  const size_t bytes = o_pages + size_t(n_prefix_pages + n_own_pages) * sizeof(int);
-  s->host.resize(bytes ? bytes : 1);
-  auto* tk = reinterpret_cast<rv::StepToken*>(s->host.data() + o_tokens);
-  auto* sq = reinterpret_cast<rv::StepSeq*>(s->host.data() + o_seqs);
-  int* pg = reinterpret_cast<int*>(s->host.data() + o_pages);
-  if (n_prefix_pages) std::memcpy(pg, prefix_pages, size_t(n_prefix_pages) * 4);
-  if (n_own_pages) std::memcpy(pg + n_prefix_pages, own_pages, size_t(n_own_pages) * 4);
+  s->tok.resize(size_t(tokens));
+  s->seq.resize(size_t(n_seqs));
+  s->group_first.assign(1, 0);
+  auto* tk = s->tok.data();
+  auto* sq = s->seq.data();
+  std::vector<int>& pg = s->pg;
+  pg.assign(prefix_pages, prefix_pages + n_prefix_pages);
+  pg.insert(pg.end(), own_pages, own_pages + n_own_pages);
   s->writer.assign(size_t(num_pages), 0);
   int t = 0, b = 0, last_pos = -1;
   int64_t pa = 0, pb = n_prefix_pages;
   for (int g = 0; g < n_groups; ++g) {
     for (int k = 0; k < group_sizes[g]; ++k, ++b) {
       const int n = q_lens[b], own = own_lens[b];
-      sq[b] = {t, n, int(pa), prefix_lens[g], int(pb), own, causal ? own - n : INT_MAX / 2, 0};
+      sq[b] = {t, n, int(pa), prefix_lens[g], int(pb), own, causal ? own - n : INT_MAX / 2};
       for (int i = 0; i < n; ++i) {
         const int place = own - n + i;  // negative only when nothing can be appended
-        const int page = place >= 0 ? pg[pb + place / ps] : 0;
+        const int page = place >= 0 ? pg[size_t(pb + place / ps)] : 0;
         tk[t++] = {page, place >= 0 ? place % ps : 0, prefix_lens[g] + place, b};
         if (place < 0) continue;
         int& w = s->writer[size_t(page)];
@@ -190,10 +407,36 @@ int plan(rv_step* s, int32_t n_seqs, const int32_t* q_lens, const int32_t* own_l
       pb += count(own);
     }
     pa += count(prefix_lens[g]);
+    s->group_first.push_back(b);
   }
   // A page that new tokens go to belongs to no prefix.
   for (int64_t i = 0; i < n_prefix_pages; ++i)
     if (s->writer[size_t(prefix_pages[i])]) can_append = false;
+
+  Schedule& sc = s->sched;
+  sc.row_items.clear();
+  sc.tile_items.clear();
+  sc.joined.clear();
+  sc.n_parts = 0;
+  schedule(s->seq, s->group_first, int(tokens), s->fold, s->q_heads / s->fold, rv::device_sm_count(), &sc);
+  if (sc.n_parts > INT_MAX ||
+      (int64_t(sc.row_items.size()) + int64_t(sc.tile_items.size())) * (s->q_heads / s->fold) > INT_MAX)
+    return fail(s, RV_E_INVALID, "the step is too large");
+
+  // The records, one after the other, each on 16 bytes.
+  size_t bytes = 0;
+  auto place_of = [&bytes](size_t n) {
+    const size_t at = bytes;
+    bytes += (n + 15) / 16 * 16;
+    return at;
+  };
+  const size_t o_tokens = place_of(s->tok.size() * sizeof(rv::StepToken));
+  const size_t o_parts = place_of(sc.parts.size() * sizeof(rv::StepParts));
+  const size_t o_rows = place_of(sc.row_items.size() * sizeof(rv::StepItem));
+  const size_t o_tiles = place_of(sc.tile_items.size() * sizeof(rv::StepItem));
+  const size_t o_joined = place_of(sc.joined.size() * sizeof(int));
+  const size_t o_pages = place_of(pg.size() * sizeof(int));
+  const size_t floats = size_t(sc.n_parts) * size_t(s->q_heads) * size_t(s->head_dim + 1);
 
   Staging& sg = s->staging[s->turn];
   s->turn ^= 1;
@@ -217,15 +460,39 @@ int plan(rv_step* s, int32_t n_seqs, const int32_t* q_lens, const int32_t* own_l
       return cuda_fail(s, "plan records", e);
     s->meta_cap = want;
   }
-  if (bytes) std::memcpy(sg.p, s->host.data(), bytes);
+  auto put = [&sg](size_t at, const void* p, size_t n) {
+    if (n) std::memcpy(sg.p + at, p, n);
+  };
+  put(o_tokens, s->tok.data(), s->tok.size() * sizeof(rv::StepToken));
+  put(o_parts, sc.parts.data(), sc.parts.size() * sizeof(rv::StepParts));
+  put(o_rows, sc.row_items.data(), sc.row_items.size() * sizeof(rv::StepItem));
+  put(o_tiles, sc.tile_items.data(), sc.tile_items.size() * sizeof(rv::StepItem));
+  put(o_joined, sc.joined.data(), sc.joined.size() * sizeof(int));
+  put(o_pages, pg.data(), pg.size() * sizeof(int));
+  if (s->work_cap < floats) {
+    if (s->work) cudaFree(s->work);
+    s->work = nullptr;
+    s->work_cap = 0;
+    const size_t want = floats + floats / 4;
+    if ((e = cudaMalloc(reinterpret_cast<void**>(&s->work), want * sizeof(float))) != cudaSuccess)
+      return cuda_fail(s, "partial results", e);
+    s->work_cap = want;
+  }
   if ((e = enter(s, st)) != cudaSuccess) return cuda_fail(s, "ordering streams", e);
   if (bytes && (e = cudaMemcpyAsync(s->meta, sg.p, bytes, cudaMemcpyHostToDevice, st)) != cudaSuccess)
     return cuda_fail(s, "plan upload", e);
   if ((e = cudaEventRecord(sg.done, st)) != cudaSuccess) return cuda_fail(s, "plan upload", e);
   if ((e = leave(s, st)) != cudaSuccess) return cuda_fail(s, "ordering streams", e);
   s->tokens = reinterpret_cast<rv::StepToken*>(s->meta + o_tokens);
-  s->seqs = reinterpret_cast<rv::StepSeq*>(s->meta + o_seqs);
+  s->parts = reinterpret_cast<rv::StepParts*>(s->meta + o_parts);
+  s->row_items = reinterpret_cast<rv::StepItem*>(s->meta + o_rows);
+  s->tile_items = reinterpret_cast<rv::StepItem*>(s->meta + o_tiles);
+  s->joined = reinterpret_cast<int*>(s->meta + o_joined);
   s->pages = reinterpret_cast<int*>(s->meta + o_pages);
+  s->n_row_items = int(sc.row_items.size());
+  s->n_tile_items = int(sc.tile_items.size());
+  s->n_joined = int(sc.joined.size());
+  s->n_parts = sc.n_parts;
   s->n_tokens = int(tokens);
   s->num_pages = num_pages;
   s->last_pos = last_pos;
@@ -251,9 +518,14 @@ int rv_step_create(int device, int32_t q_heads, int32_t kv_heads, int32_t head_d
   s->kv_heads = kv_heads;
   s->head_dim = head_dim;
   s->page_size = page_size;
+  for (int f = 1; f <= rv::kRowTile; ++f)
+    if (q_heads / kv_heads % f == 0) s->fold = f;
   DeviceGuard g(device);
   bool ok = g.ok && cudaEventCreateWithFlags(&s->last, cudaEventDisableTiming) == cudaSuccess;
   for (auto& sg : s->staging) ok = ok && cudaEventCreateWithFlags(&sg.done, cudaEventDisableTiming) == cudaSuccess;
+  ok = ok && cudaHostAlloc(reinterpret_cast<void**>(&s->err_host), sizeof(unsigned int), cudaHostAllocMapped) == cudaSuccess;
+  if (ok) *s->err_host = 0;
+  ok = ok && cudaHostGetDevicePointer(reinterpret_cast<void**>(&s->err_dev), s->err_host, 0) == cudaSuccess;
   if (!ok) {
     cudaGetLastError();
     rv_step_destroy(s);
@@ -276,6 +548,8 @@ void rv_step_destroy(rv_step* s) {
       if (sg.p) cudaFreeHost(sg.p);
     }
     if (s->meta) cudaFree(s->meta);
+    if (s->work) cudaFree(s->work);
+    if (s->err_host) cudaFreeHost(s->err_host);
     if (s->last) cudaEventDestroy(s->last);
   }
   delete s;
@@ -308,6 +582,7 @@ int rv_step_append(rv_step* s, const rv_kv_cache* cache, const void* q, int64_t 
   if (!s) return RV_E_INVALID;
   std::lock_guard<std::mutex> lk(s->mu);
   try {
+    if (device_error(s)) return RV_E_DEVICE;
     if (!s->planned) return fail(s, RV_E_NOT_READY, "no plan");
     if (!s->can_append)
       return fail(s, RV_E_INVALID, "the plan cannot append: own_lens below q_lens, or a page that new tokens go to is "
@@ -355,6 +630,7 @@ int rv_step_attend(rv_step* s, const rv_kv_cache* cache, const void* q, int64_t 
   if (!s) return RV_E_INVALID;
   std::lock_guard<std::mutex> lk(s->mu);
   try {
+    if (device_error(s)) return RV_E_DEVICE;
     if (!s->planned) return fail(s, RV_E_NOT_READY, "no plan");
     rv::AttendArgs a{};
     rv::Act act;
@@ -372,10 +648,20 @@ int rv_step_attend(rv_step* s, const rv_kv_cache* cache, const void* q, int64_t 
       return fail(s, RV_E_INVALID, "queries and output must start on 16 bytes and have strides of 16 bytes");
     if (q_token <= 0 || q_head <= 0 || out_token <= 0 || out_head <= 0)
       return fail(s, RV_E_INVALID, "the strides of queries and output must be positive");
-    a.tokens = s->tokens;
-    a.seqs = s->seqs;
+    a.row_items = s->row_items;
+    a.tile_items = s->tile_items;
+    a.parts = s->parts;
+    a.joined = s->joined;
     a.pages = s->pages;
+    a.n_row_items = s->n_row_items;
+    a.n_tile_items = s->n_tile_items;
+    a.n_joined = s->n_joined;
     a.n_tokens = s->n_tokens;
+    a.fold = s->fold;
+    a.part_o = s->work;
+    a.part_l = s->work + s->n_parts * s->q_heads * s->head_dim;
+    a.num_pages = cache->num_pages;
+    a.err = s->err_dev;
     a.q_heads = s->q_heads;
     a.kv_heads = s->kv_heads;
     a.head_dim = s->head_dim;
@@ -428,6 +714,10 @@ int rv_rms_norm(int32_t act_dtype, const void* x, int64_t x_stride, const void* 
   a.scales = scales;
   a.group = group ? group : hidden;
   a.eps = eps;
+  auto on16 = [](const void* p, int64_t stride) { return aligned16(p) && stride % 8 == 0; };
+  a.vec = hidden % 8 == 0 && on16(x, x_stride) && on16(residual, residual_stride) &&
+          on16(residual_out, residual_out_stride) &&
+          (out8 ? reinterpret_cast<uintptr_t>(out) % 8 == 0 && out_stride % 8 == 0 : on16(out, out_stride));
   const cudaError_t e =
       rv::rms_norm(act_dtype == RV_DTYPE_BF16 ? rv::Act::kBf16 : rv::Act::kF16, a, static_cast<cudaStream_t>(stream));
   return e == cudaSuccess ? RV_OK : RV_E_CUDA;

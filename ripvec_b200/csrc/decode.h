@@ -16,11 +16,18 @@ struct alignas(16) StepToken {
   int page, slot, pos, seq;
 };
 
-// What one sequence's queries see: keys [0, len_a) of the prefix whose pages start at pages[pg_a],
-// then keys of its own, pages from pages[pg_b]: token i of the sequence (tokens tok0 .. tok0 + n - 1)
-// sees own keys j < min(len_b, diag + i + 1).
-struct alignas(16) StepSeq {
-  int tok0, n, pg_a, len_a, pg_b, len_b, diag, pad;
+// A piece of attention work for each group of query heads: tokens tok0 .. tok0 + n - 1 against prefix keys
+// [a0, a1) (pages from pages[pg_a]) and own keys [b0, b1) (pages from pages[pg_b]), of which token i sees
+// those below diag + i + 1.  a0 and b0 are multiples of the key tile.  The result is partial number `part`
+// of each of its tokens (StepParts).
+struct alignas(16) StepItem {
+  int tok0, n, pg_a, a0, a1, pg_b, b0, b1, diag, part, pad0, pad1;
+};
+
+// Partial results of a token: partials first .. first + count - 1 of the workspace; with count 1 its item
+// writes the output itself.
+struct alignas(8) StepParts {
+  int first, count;
 };
 
 // Key and value pools of one layer: element (page, head, slot, d) of either at
@@ -51,17 +58,30 @@ struct AppendArgs {
 };
 cudaError_t kv_append(Act act, const AppendArgs& a, cudaStream_t st);
 
+// Query heads that share key/value loads: a row tile holds `fold` heads of every token.
+constexpr int kRowTile = 16;         // rows of an item of the few-row kernel
+constexpr int kRowKeys = 64;         // keys of its tile
+constexpr int kTileRows = 128;       // rows of one of the two row tiles of a tensor-core item
+constexpr int kTileKeys = 128;       // keys of its tile
+
 struct AttendArgs {
-  const StepToken* tokens;
-  const StepSeq* seqs;
+  const StepItem* row_items;   // for attend_rows: n * fold <= kRowTile
+  const StepItem* tile_items;  // for attend_tiles: n <= 2 * (kTileRows / fold), most work first
+  const StepParts* parts;      // by token
+  const int* joined;           // tokens with a partial count other than 1
   const int* pages;
-  int n_tokens, q_heads, kv_heads, head_dim;
+  int n_row_items, n_tile_items, n_joined;
+  int n_tokens, q_heads, kv_heads, head_dim, fold;
   Rows q;
   void* out;
   int64_t out_token, out_head;
-  float* lse;  // [tokens, q_heads] or null
+  float* lse;     // [tokens, q_heads] or null
+  float* part_o;  // [partials, q_heads, head_dim] results of items, divided by their own sums
+  float* part_l;  // [partials, q_heads] log2 of the sums (-inf: no key)
   KvPool pool;
+  int64_t num_pages;
   float scale;
+  unsigned int* err;  // error word that the host reads
 };
 cudaError_t step_attend(Act act, const AttendArgs& a, cudaStream_t st);
 
@@ -76,6 +96,7 @@ struct NormArgs {
   float* scales;       // [rows, hidden / group]
   int group;           // values a scale stands for (hidden: one scale a row)
   float eps;
+  bool vec;  // hidden a multiple of 8, every row of x, residual and the outputs on 16 bytes (codes: 8)
 };
 cudaError_t rms_norm(Act act, const NormArgs& a, cudaStream_t st);
 

@@ -1,77 +1,105 @@
-// Attention of a decoding step over the paged cache: every query of a sequence sees its group's shared
-// prefix and, of its sequence's own keys, those up to its own place.
-#include "common.cuh"
-#include "decode.h"
+// Attention of a decoding step: the two kernels that compute partial or final rows, and the join of tokens
+// whose keys were split over several items.
+#include "step_attend.cuh"
 
 namespace rv {
 
 namespace {
 
-// One warp per (token, query head), the head's values spread over the lanes; one pass over the keys
-// with a running maximum m and sum l.
+// One warp per (token, query head): out = sum_i 2^(l_i - max) o_i / sum_i 2^(l_i - max).  A token without any
+// item sees no key: zeros and -inf.
 template <typename T, int D>
-__global__ void __launch_bounds__(128) attend_rows_kernel(AttendArgs a) {
+__global__ void __launch_bounds__(128) join_kernel(const int* __restrict__ tokens, int n, const AttendParams p) {
   constexpr int kPer = D / 32;
   const int lane = threadIdx.x & 31;
   const int64_t w = int64_t(blockIdx.x) * 4 + (threadIdx.x >> 5);
-  if (w >= int64_t(a.n_tokens) * a.q_heads) return;
-  const int t = static_cast<int>(w / a.q_heads), h = static_cast<int>(w % a.q_heads);
-  const int kvh = h / (a.q_heads / a.kv_heads);
-  const StepSeq s = a.seqs[a.tokens[t].seq];
-  const int own = min(s.len_b, s.diag + (t - s.tok0) + 1);
-  const T* q = static_cast<const T*>(a.q.p) + t * a.q.token_stride + h * a.q.head_stride;
-  const float sl = a.scale * 1.4426950408889634f;
-  float qr[kPer], o[kPer];
+  if (w >= int64_t(n) * p.q_heads) return;
+  const int tok = tokens[w / p.q_heads], head = static_cast<int>(w % p.q_heads);
+  const StepParts pt = p.parts[tok];
+  const int64_t at = int64_t(pt.first) * p.q_heads + head;
+  float top = -INFINITY;
+  for (int i = lane; i < pt.count; i += 32) top = fmaxf(top, p.part_l[at + int64_t(i) * p.q_heads]);
 #pragma unroll
-  for (int i = 0; i < kPer; ++i) {
-    qr[i] = Elem<T>::to_f(q[lane * kPer + i]) * sl;
-    o[i] = 0.f;
-  }
-  float m = -INFINITY, l = 0.f;
-  for (int part = 0; part < 2; ++part) {
-    const int n = part ? own : s.len_a;
-    const int* pg = a.pages + (part ? s.pg_b : s.pg_a);
-    for (int j = 0; j < n; ++j) {
-      const int64_t off = pg[j / a.pool.page_size] * a.pool.page_stride + kvh * a.pool.head_stride +
-                          (j % a.pool.page_size) * a.pool.slot_stride + lane * kPer;
-      const T* kp = static_cast<const T*>(a.pool.k) + off;
-      const T* vp = static_cast<const T*>(a.pool.v) + off;
-      float x = 0.f;
+  for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+  float v[kPer] = {}, sum = 0.f;
+  if (top != -INFINITY) {
+    for (int i = 0; i < pt.count; ++i) {
+      const int64_t k = at + int64_t(i) * p.q_heads;
+      const float f = ex2_approx(p.part_l[k] - top);
+      sum += f;
 #pragma unroll
-      for (int i = 0; i < kPer; ++i) x += qr[i] * Elem<T>::to_f(kp[i]);
-#pragma unroll
-      for (int e = 16; e > 0; e >>= 1) x += __shfl_xor_sync(0xffffffffu, x, e);
-      const float mn = fmaxf(m, x);
-      const float f = m == mn ? 1.f : exp2f(m - mn);
-      const float p = exp2f(x - mn);
-      l = l * f + p;
-#pragma unroll
-      for (int i = 0; i < kPer; ++i) o[i] = o[i] * f + p * Elem<T>::to_f(vp[i]);
-      m = mn;
+      for (int e = 0; e < kPer; ++e) v[e] += f * p.part_o[k * D + lane * kPer + e];
     }
   }
-  T* out = static_cast<T*>(a.out) + t * a.out_token + h * a.out_head;
-  const float inv = l == 0.f ? 0.f : 1.f / l;
+  const float inv = sum > 0.f ? 1.f / sum : sum == 0.f ? 0.f : sum;
+  T* dst = static_cast<T*>(p.out) + tok * p.out_token + head * p.out_head + lane * kPer;
 #pragma unroll
-  for (int i = 0; i < kPer; ++i) out[lane * kPer + i] = Elem<T>::from_f(o[i] * inv);
-  if (a.lse && lane == 0)
-    a.lse[int64_t(t) * a.q_heads + h] = l == 0.f ? -INFINITY : (m + log2f(l)) * 0.6931471805599453f;
+  for (int e = 0; e < kPer; ++e) dst[e] = Elem<T>::from_f(v[e] * inv);
+  if (p.lse && lane == 0)
+    p.lse[int64_t(tok) * p.q_heads + head] = sum == 0.f ? -INFINITY : (top + log2f(sum)) * 0.6931471805599453f;
 }
 
 template <typename T>
-cudaError_t launch(const AttendArgs& a, cudaStream_t st) {
-  const int64_t warps = int64_t(a.n_tokens) * a.q_heads;
-  const int blocks = static_cast<int>((warps + 3) / 4);
-  if (a.head_dim == 64) attend_rows_kernel<T, 64><<<blocks, 128, 0, st>>>(a);
-  else attend_rows_kernel<T, 128><<<blocks, 128, 0, st>>>(a);
+cudaError_t join(const AttendArgs& a, const AttendParams& p, cudaStream_t st) {
+  const int blocks = static_cast<int>((int64_t(a.n_joined) * a.q_heads + 3) / 4);
+  if (a.head_dim == 64) join_kernel<T, 64><<<blocks, 128, 0, st>>>(a.joined, a.n_joined, p);
+  else join_kernel<T, 128><<<blocks, 128, 0, st>>>(a.joined, a.n_joined, p);
   return cudaGetLastError();
+}
+
+bool pool_map(CUtensorMap* m, const void* base, bool bf, const AttendArgs& a, int box) {
+  const uint64_t dims[4] = {uint64_t(a.head_dim), uint64_t(a.pool.page_size), uint64_t(a.kv_heads), uint64_t(a.num_pages)};
+  const uint64_t strides[3] = {uint64_t(a.pool.slot_stride) * 2, uint64_t(a.pool.head_stride) * 2,
+                               uint64_t(a.pool.page_stride) * 2};
+  const uint32_t b[4] = {64, uint32_t(box), 1, 1};
+  return make_tmap_16bit(m, base, bf, 4, dims, strides, b);
 }
 
 }  // namespace
 
 cudaError_t step_attend(Act act, const AttendArgs& a, cudaStream_t st) {
   if (a.n_tokens <= 0) return cudaSuccess;
-  return act == Act::kBf16 ? launch<__nv_bfloat16>(a, st) : launch<__half>(a, st);
+  const bool bf = act == Act::kBf16;
+  AttendParams p{};
+  p.parts = a.parts;
+  p.pages = a.pages;
+  p.q_heads = a.q_heads;
+  p.fold = a.fold;
+  p.per_kv = a.q_heads / a.kv_heads / a.fold;
+  p.page_size = a.pool.page_size;
+  p.out = a.out;
+  p.out_token = a.out_token;
+  p.out_head = a.out_head;
+  p.lse = a.lse;
+  p.part_o = a.part_o;
+  p.part_l = a.part_l;
+  p.scale_log2 = a.scale * 1.4426950408889634f;
+  p.err = a.err;
+  CUtensorMap mk, mv, mq;
+  cudaError_t e = cudaSuccess;
+  if (a.n_tile_items > 0) {
+    p.items = a.tile_items;
+    p.n_items = a.n_tile_items;
+    p.box = a.pool.page_size < kTileKeys ? a.pool.page_size : kTileKeys;
+    const uint64_t dims[3] = {uint64_t(a.head_dim), uint64_t(a.q_heads), uint64_t(a.n_tokens)};
+    const uint64_t strides[2] = {uint64_t(a.q.head_stride) * 2, uint64_t(a.q.token_stride) * 2};
+    const uint32_t box[3] = {64, uint32_t(a.fold), uint32_t(kTileRows / a.fold)};
+    if (!pool_map(&mk, a.pool.k, bf, a, p.box) || !pool_map(&mv, a.pool.v, bf, a, p.box) ||
+        !make_tmap_16bit(&mq, a.q.p, bf, 3, dims, strides, box))
+      return cudaErrorInvalidValue;
+    e = attend_tiles(act, a.head_dim, mq, mk, mv, p, st);
+    if (e != cudaSuccess) return e;
+  }
+  if (a.n_row_items > 0) {
+    p.items = a.row_items;
+    p.n_items = a.n_row_items;
+    p.box = a.pool.page_size < kRowKeys ? a.pool.page_size : kRowKeys;
+    if (!pool_map(&mk, a.pool.k, bf, a, p.box) || !pool_map(&mv, a.pool.v, bf, a, p.box)) return cudaErrorInvalidValue;
+    e = attend_rows(act, a.head_dim, mk, mv, a.q, p, st);
+    if (e != cudaSuccess) return e;
+  }
+  if (a.n_joined > 0) e = bf ? join<__nv_bfloat16>(a, p, st) : join<__half>(a, p, st);
+  return e;
 }
 
 }  // namespace rv

@@ -1,0 +1,90 @@
+// Shared by the attention kernels of a decoding step.
+#pragma once
+
+#include "common.cuh"
+#include "decode.h"
+#include "tmap.h"
+
+namespace rv {
+
+// What a launch of either kernel needs beside its tensor maps.
+struct AttendParams {
+  const StepItem* items;
+  const StepParts* parts;
+  const int* pages;
+  int n_items, q_heads, fold, per_kv;  // per_kv: head groups of `fold` query heads to a key/value head
+  int page_size, box;                  // box: keys of one page copy
+  void* out;
+  int64_t out_token, out_head;
+  float *lse, *part_o, *part_l;
+  float scale_log2;
+  unsigned int* err;
+};
+
+__device__ __forceinline__ float ex2_approx(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+__device__ __forceinline__ void tma_load_3d(void* dst, const CUtensorMap* map, uint64_t* bar, int x, int y, int z) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes"
+      " [%0], [%1, {%3, %4, %5}], [%2];" ::"r"(smem_u32(dst)),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(smem_u32(bar)), "r"(x), "r"(y), "r"(z)
+      : "memory");
+}
+__device__ __forceinline__ void tma_load_4d(void* dst, const CUtensorMap* map, uint64_t* bar, int x, int y, int z,
+                                            int w) {
+  asm volatile(
+      "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes"
+      " [%0], [%1, {%3, %4, %5, %6}], [%2];" ::"r"(smem_u32(dst)),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(smem_u32(bar)), "r"(x), "r"(y), "r"(z), "r"(w)
+      : "memory");
+}
+
+// Key tile j of an item: first key, how many there are, and the page list it is read through.
+struct KeyTile {
+  int base, valid, pg;
+  bool own;
+};
+template <int kKeys>
+__device__ __forceinline__ KeyTile key_tile(const StepItem& it, int j) {
+  const int na = (it.a1 - it.a0 + kKeys - 1) / kKeys;
+  KeyTile t;
+  t.own = j >= na;
+  t.base = t.own ? it.b0 + (j - na) * kKeys : it.a0 + j * kKeys;
+  t.valid = min(kKeys, (t.own ? it.b1 : it.a1) - t.base);
+  t.pg = t.own ? it.pg_b : it.pg_a;
+  return t;
+}
+template <int kKeys>
+__device__ __forceinline__ int key_tiles(const StepItem& it) {
+  return (it.a1 - it.a0 + kKeys - 1) / kKeys + (it.b1 - it.b0 + kKeys - 1) / kKeys;
+}
+
+// One lane's share of a key tile's copies: lane (copy * kHalves + half) brings 64 values of the head from the
+// box of keys `copy`.  The page number is read ahead of the copy by page_of.
+template <int kKeys, int kHalves>
+struct TileCopy {
+  static __device__ __forceinline__ int copies(const KeyTile& t, int box) { return (t.valid + box - 1) / box; }
+  static __device__ __forceinline__ int page_of(const AttendParams& p, const KeyTile& t, int lane) {
+    const int c = lane / kHalves;
+    if (c >= copies(t, p.box)) return 0;
+    return __ldg(&p.pages[t.pg + (t.base + c * p.box) / p.page_size]);
+  }
+  static __device__ __forceinline__ void issue(const AttendParams& p, const KeyTile& t, int page, int lane,
+                                               uint8_t* dst, const CUtensorMap* map, uint64_t* bar, int kv_head) {
+    const int c = lane / kHalves, half = lane % kHalves;
+    if (c >= copies(t, p.box)) return;
+    tma_load_4d(dst + half * (kKeys * 128) + c * p.box * 128, map, bar, half * 64, (t.base + c * p.box) % p.page_size,
+                kv_head, page);
+  }
+};
+
+cudaError_t attend_rows(Act act, int head_dim, const CUtensorMap& mk, const CUtensorMap& mv, const Rows& q,
+                        const AttendParams& p, cudaStream_t st);
+cudaError_t attend_tiles(Act act, int head_dim, const CUtensorMap& mq, const CUtensorMap& mk, const CUtensorMap& mv,
+                         const AttendParams& p, cudaStream_t st);
+
+}  // namespace rv

@@ -50,6 +50,22 @@ bool make_tmap_2d_16bit(CUtensorMap* out, const void* base, bool is_bf16, uint64
   return true;
 }
 
+bool make_tmap_16bit(CUtensorMap* out, const void* base, bool is_bf16, int rank, const uint64_t* dims,
+                     const uint64_t* strides, const uint32_t* box) {
+  auto fn = encode_fn();
+  if (!fn || rank < 2 || rank > 5) return false;
+  cuuint64_t d[5], st[4];
+  cuuint32_t b[5], one[5] = {1, 1, 1, 1, 1};
+  for (int i = 0; i < rank; ++i) {
+    d[i] = dims[i];
+    b[i] = box[i];
+    if (i + 1 < rank) st[i] = strides[i];
+  }
+  return fn(out, is_bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, rank,
+            const_cast<void*>(base), d, st, b, one, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+            CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
 int device_sm_count() {
   static std::atomic<int> cache[64] = {};
   int dev = 0;

@@ -45,6 +45,11 @@ bool make_tmap_2d_16bit(CUtensorMap* out, const void* base, bool is_bf16, uint64
                         uint64_t outer, uint64_t row_stride_bytes, uint32_t box_inner,
                         uint32_t box_outer, std::string* why, int swizzle_bytes = 128);
 
+// Encodes a tensor of 16-bit elements of `rank` axes (innermost first, unit stride along it; strides in
+// bytes of the other axes) for tiled TMA copies of `box` with 128-byte swizzling.  False as above.
+bool make_tmap_16bit(CUtensorMap* out, const void* base, bool is_bf16, int rank, const uint64_t* dims,
+                     const uint64_t* strides, const uint32_t* box);
+
 // Number of SMs of the current device (cached per device).
 int device_sm_count();
 

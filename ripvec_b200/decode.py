@@ -23,14 +23,17 @@ from . import _lib as L
 _DTYPES = {torch.bfloat16: L.RV_DTYPE_BF16, torch.float16: L.RV_DTYPE_F16}
 
 
-def _stream(stream, device) -> int | None:
-    return (torch.cuda.current_stream(device).cuda_stream if stream is None else stream) or None
+# torch's current stream of a device as a handle, without the stream object around it.
+_current_stream = torch._C._cuda_getCurrentRawStream
 
 
-def _rows(name: str, t, tokens: int, heads: int, dim: int, dtype, device) -> None:
-    if t.shape != (tokens, heads, dim) or t.dtype != dtype or t.device != device or t.stride(2) != 1:
-        raise ValueError(f"{name} must be [{tokens}, {heads}, {dim}] {dtype} on {device} with unit stride along the "
-                         f"last axis, got {tuple(t.shape)} {t.dtype} on {t.device} with strides {t.stride()}")
+def _rows(name: str, t, shape: tuple, cache: "PagedCache") -> tuple:
+    """Address, token stride and head stride of ``t``, which must be ``shape`` rows like the cache's."""
+    st, sh, sd = t.stride() if t.ndim == 3 else (0, 0, 0)
+    if sd != 1 or t.shape != shape or t.dtype is not cache.dtype or t.get_device() != cache.device_index:
+        raise ValueError(f"{name} must be {shape} {cache.dtype} on {cache.device} with unit stride along the last "
+                         f"axis, got {tuple(t.shape)} {t.dtype} on {t.device} with strides {t.stride()}")
+    return t.data_ptr(), st, sh
 
 
 def _i32(values) -> np.ndarray:
@@ -53,7 +56,7 @@ class PagedCache:
             raise ValueError("k and v must have the same strides, and unit stride along the last axis")
         self.k, self.v = k, v
         self.num_pages, self.kv_heads, self.page_size, self.head_dim = k.shape
-        self.dtype, self.device = k.dtype, k.device
+        self.dtype, self.device, self.device_index = k.dtype, k.device, k.get_device()
         sp, sh, ss, _ = k.stride()
         self.desc = L.KvCache(k.data_ptr(), v.data_ptr(), self.num_pages, sp, sh, ss, _DTYPES[k.dtype], self.kv_heads,
                               self.head_dim, self.page_size)
@@ -126,7 +129,7 @@ class DecodeStep:
         op, pp = flat(own_pages, ol), flat(prefix_pages, pl)
         self._check(self._lib.rv_step_plan(self._h, len(ql), ql.ctypes.data, ol.ctypes.data, op.ctypes.data, len(gs),
                                            gs.ctypes.data, pl.ctypes.data, pp.ctypes.data, num_pages, bool(causal),
-                                           _stream(stream, self.device)))
+                                           _current_stream(self.device.index) if stream is None else stream))
         self.tokens = int(ql.sum())
 
     def append(self, cache: PagedCache, q, k, v, cos, sin, *, q_out=None, interleaved: bool = False,
@@ -137,25 +140,23 @@ class DecodeStep:
         keys and values only."""
         t, d = self._tokens(), self.head_dim
         if q is not None:
-            _rows("q", q, t, self.q_heads, d, cache.dtype, cache.device)
+            qa = _rows("q", q, (t, self.q_heads, d), cache)
             if q_out is None:
                 q_out = torch.empty((t, self.q_heads, d), dtype=q.dtype, device=q.device)
-            _rows("q_out", q_out, t, self.q_heads, d, cache.dtype, cache.device)
-            qa = (q.data_ptr(), q.stride(0), q.stride(1))
-            qo = (q_out.data_ptr(), q_out.stride(0), q_out.stride(1))
+            qo = _rows("q_out", q_out, (t, self.q_heads, d), cache)
         elif q_out is not None:
             raise ValueError("q_out without q")
         else:
             qa = qo = (None, 0, 0)
-        _rows("k", k, t, self.kv_heads, d, cache.dtype, cache.device)
-        _rows("v", v, t, self.kv_heads, d, cache.dtype, cache.device)
-        if cos.shape != sin.shape or cos.ndim != 2 or cos.dtype != torch.float32 or sin.dtype != torch.float32 \
-                or cos.device != cache.device or sin.device != cache.device or not cos.is_contiguous() \
-                or not sin.is_contiguous():
+        ka, va = _rows("k", k, (t, self.kv_heads, d), cache), _rows("v", v, (t, self.kv_heads, d), cache)
+        if cos.ndim != 2 or cos.shape != sin.shape or cos.dtype is not torch.float32 or sin.dtype is not torch.float32 \
+                or cos.get_device() != cache.device_index or sin.get_device() != cache.device_index \
+                or not cos.is_contiguous() or not sin.is_contiguous():
             raise ValueError("cos and sin must be contiguous [positions, rot / 2] f32 tensors on the cache's device")
-        rc = self._lib.rv_step_append(self._h, cache._ref, *qa, k.data_ptr(), k.stride(0), k.stride(1), v.data_ptr(),
-                                      v.stride(0), v.stride(1), *qo, cos.data_ptr(), sin.data_ptr(), cos.shape[0],
-                                      2 * cos.shape[1], interleaved, _stream(stream, cache.device))
+        positions, half = cos.shape
+        rc = self._lib.rv_step_append(self._h, cache._ref, *qa, *ka, *va, *qo, cos.data_ptr(), sin.data_ptr(), positions,
+                                      2 * half, interleaved,
+                                      _current_stream(cache.device_index) if stream is None else stream)
         if rc:
             self._check(rc)
         return q_out
@@ -166,17 +167,17 @@ class DecodeStep:
         (``scale`` 1 / sqrt(head_dim) by default).  ``lse [tokens, q_heads]`` f32, where given, receives the
         log of the softmax's denominator.  Returns ``out [tokens, q_heads, head_dim]``."""
         t, d = self._tokens(), self.head_dim
-        _rows("q", q, t, self.q_heads, d, cache.dtype, cache.device)
+        shape = (t, self.q_heads, d)
+        qa = _rows("q", q, shape, cache)
         if out is None:
-            out = torch.empty((t, self.q_heads, d), dtype=q.dtype, device=q.device)
-        else:
-            _rows("out", out, t, self.q_heads, d, cache.dtype, cache.device)
-        if lse is not None and (lse.shape != (t, self.q_heads) or lse.dtype != torch.float32
-                                or lse.device != cache.device or not lse.is_contiguous()):
+            out = torch.empty(shape, dtype=q.dtype, device=q.device)
+        oa = _rows("out", out, shape, cache)
+        if lse is not None and (lse.shape != shape[:2] or lse.dtype is not torch.float32
+                                or lse.get_device() != cache.device_index or not lse.is_contiguous()):
             raise ValueError(f"lse must be a contiguous [{t}, {self.q_heads}] f32 tensor on the cache's device")
-        rc = self._lib.rv_step_attend(self._h, cache._ref, q.data_ptr(), q.stride(0), q.stride(1), out.data_ptr(),
-                                      out.stride(0), out.stride(1), None if lse is None else lse.data_ptr(),
-                                      d ** -0.5 if scale is None else scale, _stream(stream, cache.device))
+        rc = self._lib.rv_step_attend(self._h, cache._ref, *qa, *oa, None if lse is None else lse.data_ptr(),
+                                      d ** -0.5 if scale is None else scale,
+                                      _current_stream(cache.device_index) if stream is None else stream)
         if rc:
             self._check(rc)
         return out
@@ -188,41 +189,47 @@ def rms_norm(x, weight, *, residual=None, residual_out=None, out=None, eps: floa
     ``out = h / sqrt(mean(h^2) + eps) * weight``; ``h`` in 16 bits goes to ``residual_out`` where given (it may
     be ``residual`` or ``x``).  Returns ``(out, scales)``: 16-bit rows and ``None``, or with ``out_8bit`` e4m3
     codes and their f32 scales ``[rows, hidden / group]`` (``group = 0``: one scale a row)."""
-    if x.ndim != 2 or x.dtype not in _DTYPES or not x.is_cuda or (x.shape[1] > 1 and x.stride(1) != 1):
+    code, dev = _DTYPES.get(x.dtype), x.get_device()
+    if code is None or x.ndim != 2 or dev < 0 or (x.shape[1] > 1 and x.stride(1) != 1):
         raise ValueError("x must be a 2-D bf16 or f16 CUDA tensor with unit stride along the last axis")
-    rows, hidden = x.shape
-    if weight.shape != (hidden,) or weight.dtype != torch.float32 or weight.device != x.device \
+    shape = rows, hidden = x.shape
+    if weight.shape != shape[1:] or weight.dtype is not torch.float32 or weight.get_device() != dev \
             or not weight.is_contiguous():
         raise ValueError("weight must be a contiguous f32 [hidden] tensor on x's device")
-    for name, t in (("residual", residual), ("residual_out", residual_out)):
-        if t is not None and (t.shape != x.shape or t.dtype != x.dtype or t.device != x.device
-                              or (hidden > 1 and t.stride(1) != 1)):
-            raise ValueError(f"{name} must be like x, with unit stride along the last axis")
+
+    def like(name, t, dtype):
+        if t.shape != shape or t.dtype is not dtype or t.get_device() != dev or (hidden > 1 and t.stride(1) != 1):
+            raise ValueError(f"{name} must be {tuple(shape)} {dtype} on x's device, with unit stride along the last axis")
+        return t.data_ptr(), t.stride(0)
+
+    ra = (None, 0) if residual is None else like("residual", residual, x.dtype)
+    roa = (None, 0) if residual_out is None else like("residual_out", residual_out, x.dtype)
     if group and (not out_8bit or group not in (32, 64, 128, 256) or hidden % group):
         raise ValueError("group must be 32, 64, 128 or 256, divide hidden, and comes with out_8bit")
     dt = torch.float8_e4m3fn if out_8bit else x.dtype
     if out is None:
-        out = torch.empty((rows, hidden), dtype=dt, device=x.device)
-    elif out.shape != x.shape or out.dtype != dt or out.device != x.device or (hidden > 1 and out.stride(1) != 1):
-        raise ValueError(f"out must be [{rows}, {hidden}] {dt} on x's device, with unit stride along the last axis")
-    shape = (rows, hidden // group if group else 1)
+        out = torch.empty(shape, dtype=dt, device=x.device)
+    oa = like("out", out, dt)
     if not out_8bit:
         if scales is not None:
             raise ValueError("scales come with out_8bit")
-    elif scales is None:
-        scales = torch.empty(shape, dtype=torch.float32, device=x.device)
-    elif scales.shape != shape or scales.dtype != torch.float32 or scales.device != x.device \
-            or not scales.is_contiguous():
-        raise ValueError(f"scales must be a contiguous {shape} f32 tensor on x's device")
+    else:
+        per_row = hidden // group if group else 1
+        if scales is None:
+            scales = torch.empty((rows, per_row), dtype=torch.float32, device=x.device)
+        elif scales.shape != (rows, per_row) or scales.dtype is not torch.float32 or scales.get_device() != dev \
+                or not scales.is_contiguous():
+            raise ValueError(f"scales must be a contiguous {(rows, per_row)} f32 tensor on x's device")
     if rows == 0:
         return out, scales
-    code = _DTYPES[x.dtype]
-    with torch.cuda.device(x.device):
-        rc = L.lib().rv_rms_norm(code, x.data_ptr(), x.stride(0), L.ptr(residual),
-                                 0 if residual is None else residual.stride(0), weight.data_ptr(), L.ptr(residual_out),
-                                 0 if residual_out is None else residual_out.stride(0), out.data_ptr(), out.stride(0),
-                                 L.RV_DTYPE_E4M3 if out_8bit else code, L.ptr(scales), group, rows, hidden, eps,
-                                 _stream(stream, x.device))
-    if rc != L.RV_OK:
+    args = (code, x.data_ptr(), x.stride(0), *ra, weight.data_ptr(), *roa, *oa, L.RV_DTYPE_E4M3 if out_8bit else code,
+            scales.data_ptr() if out_8bit else None, group, rows, hidden, eps,
+            _current_stream(dev) if stream is None else stream)
+    if torch.cuda.current_device() == dev:
+        rc = L.lib().rv_rms_norm(*args)
+    else:
+        with torch.cuda.device(dev):
+            rc = L.lib().rv_rms_norm(*args)
+    if rc:
         raise L.RvError(rc, "rv_rms_norm failed (hidden from 1 to 65536, row strides of at least hidden, eps >= 0)")
     return out, scales
