@@ -71,9 +71,8 @@ __global__ void __launch_bounds__(kThreads) attend_rows_kernel(const __grid_cons
   uint64_t* empty = full + kStages<D>;
   volatile int* abort_flag = reinterpret_cast<volatile int*>(empty + kStages<D>);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int groups = p.q_heads / p.fold;
-  const StepItem it = p.items[blockIdx.x / groups];
-  const int hg = blockIdx.x % groups;
+  const StepItem it = p.items[blockIdx.x / p.groups];
+  const int hg = blockIdx.x % p.groups;
   const int tiles = key_tiles<kRowKeys>(it);
 
   if (threadIdx.x == 0) {
@@ -315,7 +314,7 @@ cudaError_t launch(const CUtensorMap& mk, const CUtensorMap& mv, const Rows& q, 
     return cudaFuncSetAttribute(attend_rows_kernel<T, D>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemBytes<D>);
   });
   if (e != cudaSuccess) return e;
-  attend_rows_kernel<T, D><<<p.n_items * (p.q_heads / p.fold), kThreads, kSmemBytes<D>, st>>>(mk, mv, q, p);
+  attend_rows_kernel<T, D><<<p.n_items * p.groups, kThreads, kSmemBytes<D>, st>>>(mk, mv, q, p);
   return cudaGetLastError();
 }
 

@@ -6,7 +6,8 @@
 // kernel is persistent, one CTA per SM; both row tiles share every K and V tile that a CTA loads.  Warp roles:
 //   warps 0..3, 4..7  softmax of row tile 0, 1: one row per thread,
 //   warp 8            TMA of Q and K, warp 9 TMA of V: page by page into rings of 128-key slots,
-//   warp 10           TMEM owner and issuer of the tcgen05.mma.
+//   warp 10           TMEM owner and issuer of the tcgen05.mma,
+//   warp 11           clears V tiles past their last key.
 // Per key tile and row tile i:
 //   S_i = Q_i K^T     tcgen05.mma M=128 N<=128 into TMEM columns of its own,
 //   softmax           scores by tcgen05.ld, masks, P = exp2(s - m) in 16 bits over S_i (tcgen05.st),
@@ -25,8 +26,7 @@ namespace rv {
 
 namespace {
 
-constexpr int kSoftmaxWarps = 8;
-constexpr int kThreads = 384;   // three warpgroups; warp 11 only takes part in the register split
+constexpr int kThreads = 384;   // three warpgroups
 // Registers a thread: the softmax warpgroups hold a row of 128 scores each and take some of the third's.  The
 // launch must bring what the split adds up to (checked before the first launch): 2 * 208 + 88 = 3 * 168.
 constexpr int kLaunchRegs = 168, kSoftmaxRegs = 208, kOtherRegs = 88;
@@ -68,34 +68,31 @@ struct Walk {
   int w, round;
   int hg;
   StepItem it;
+  int na;        // prefix key tiles; own ones follow
   int tiles;     // key tiles
   int count[2];  // of which row tile 0, 1 takes this many (0: no tokens)
+  int own[2];    // own keys from b0 on that the row tile's last token sees
 
   __device__ __forceinline__ static int index(int round) {
     return round * gridDim.x + ((round & 1) ? gridDim.x - 1 - blockIdx.x : blockIdx.x);
   }
   __device__ __forceinline__ void load(const AttendParams& p, int total) {
     if (w >= total) return;
-    const int groups = p.q_heads / p.fold;
-    hg = w % groups;
-    it = p.items[w / groups];
+    hg = w % p.groups;
+    it = p.items[w / p.groups];
     const int nw = index(round + 1);
     if (nw < total) {
-      const char* nx = reinterpret_cast<const char*>(&p.items[nw / groups]);
+      const char* nx = reinterpret_cast<const char*>(&p.items[nw / p.groups]);
       asm volatile("prefetch.global.L1 [%0];" ::"l"(nx));
       asm volatile("prefetch.global.L1 [%0];" ::"l"(nx + 32));
     }
-    const int na = (it.a1 - it.a0 + kTileKeys - 1) / kTileKeys;
-    const int per = kTileRows / p.fold;  // tokens of a row tile
+    na = (it.a1 - it.a0 + kTileKeys - 1) / kTileKeys;
     tiles = 0;
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
-      count[i] = 0;
-      if (i * per >= it.n) continue;
-      // Own keys that the row tile's last token sees; a row tile that sees none still takes one tile, all
-      // masked, which gives its rows their empty result.
-      const int lim = min(it.b1, it.diag + min(it.n, (i + 1) * per));
-      count[i] = max(1, na + (max(0, lim - it.b0) + kTileKeys - 1) / kTileKeys);
+      own[i] = max(0, min(it.b1, it.diag + min(it.n, (i + 1) * p.per)) - it.b0);
+      // A row tile that sees no key still takes one tile, all masked, which gives its rows their empty result.
+      count[i] = i * p.per < it.n ? max(1, na + (own[i] + kTileKeys - 1) / kTileKeys) : 0;
       tiles = max(tiles, count[i]);
     }
   }
@@ -109,11 +106,14 @@ struct Walk {
     w = index(round);
     load(p, total);
   }
-  // Keys of tile t that row tile i can see, at least 1 (masked then).
-  __device__ __forceinline__ int seen(const AttendParams& p, const KeyTile& t, int i) const {
-    if (!t.own) return t.valid;
-    const int last = min(it.n, (i + 1) * (kTileRows / p.fold));
-    return max(1, min(t.valid, it.diag + last - t.base));
+  // Keys of tile j that were copied.
+  __device__ __forceinline__ int valid(int j) const {
+    return min(kTileKeys, j < na ? it.a1 - it.a0 - j * kTileKeys : it.b1 - it.b0 - (j - na) * kTileKeys);
+  }
+  // Keys of tile j that some row of row tile i sees, at least 1 (masked then), in whole blocks of 16.
+  __device__ __forceinline__ int seen16(int j, int i) const {
+    const int k = j < na ? it.a1 - it.a0 - j * kTileKeys : own[i] - (j - na) * kTileKeys;
+    return (max(1, min(kTileKeys, k)) + 15) & ~15;
   }
 };
 
@@ -137,18 +137,19 @@ __global__ void __launch_bounds__(kThreads, 1) attend_tiles_kernel(const __grid_
   uint64_t* k_empty = k_full + kSt;    // [kSt] both row tiles' S are done
   uint64_t* v_full = k_empty + kSt;    // [kSt]
   uint64_t* v_empty = v_full + kSt;    // [kSt] both row tiles' P V are done
-  uint64_t* s_full = v_empty + kSt;    // [2] scores in TMEM
+  uint64_t* v_land = v_empty + kSt;    // [kSt] a ragged V tile landed, to be cleared past its keys
+  uint64_t* s_full = v_land + kSt;    // [2] scores in TMEM
   uint64_t* p_full = s_full + 2;       // [2][2] P of the row tile, keys 0-63 and 64-127
   uint64_t* o_full = p_full + 4;       // [2] last P V of the item done
   uint64_t* o_empty = o_full + 2;      // [2] the item's O has been read
   uint64_t* drain = o_empty + 2;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain + 1);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
-  static_assert((2 + 2 + 4 * kSt + 2 + 4 + 2 + 2 + 1) * 8 + 8 <= 512, "barrier area");
+  static_assert((2 + 2 + 5 * kSt + 2 + 4 + 2 + 2 + 1) * 8 + 8 <= 512, "barrier area");
 
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int total = p.n_items * (p.q_heads / p.fold);
-  const int per = kTileRows / p.fold;  // tokens of a row tile
+  const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
+  const int total = p.n_items * p.groups;
+  const int per = p.per;
 
   if (threadIdx.x == 0) {
     for (int i = 0; i < 2; ++i) {
@@ -165,6 +166,7 @@ __global__ void __launch_bounds__(kThreads, 1) attend_tiles_kernel(const __grid_
       mbar_init(&k_empty[s], 1);
       mbar_init(&v_full[s], 1);
       mbar_init(&v_empty[s], 1);
+      mbar_init(&v_land[s], 1);
     }
     mbar_init(drain, 1);
     *abort_flag = 0;
@@ -194,6 +196,7 @@ __global__ void __launch_bounds__(kThreads, 1) attend_tiles_kernel(const __grid_
     wk.init(p, total);
     int s = 0, loaded = 0, q_loads[2] = {0, 0};
     uint32_t ph = 0;
+    uint32_t on_land = 0, land_ph = 0;  // by slot: the last copy was a ragged V tile's; parity of v_land
     bool ok = true;
     int page = 0;
     KeyTile t{};
@@ -223,11 +226,16 @@ __global__ void __launch_bounds__(kThreads, 1) attend_tiles_kernel(const __grid_
         const int n = TileCopy<kTileKeys, kHalves>::copies(t, p.box);
         ok = __all_sync(0xffffffffu, mbar_wait(&empty[s], ph ^ 1u, abort_flag));
         if (!ok) break;
-        if (lane == 0) mbar_arrive_expect_tx(&full[s], n * p.box * D * 2);
+        // A V tile with keys past the last in its last block of 16 goes by way of warp 11.
+        uint64_t* land = !keys && (t.valid & 15) ? &v_land[s] : &full[s];
+        if (lane == 0) mbar_arrive_expect_tx(land, n * p.box * D * 2);
         __syncwarp();
-        TileCopy<kTileKeys, kHalves>::issue(p, t, page, lane, ring + s * kKeyBytes<D>, keys ? &mk : &mv, &full[s],
+        TileCopy<kTileKeys, kHalves>::issue(p, t, page, lane, ring + s * kKeyBytes<D>, keys ? &mk : &mv, land,
                                             hg / p.per_kv);
         ++loaded;
+        const uint32_t bit = 1u << s;
+        on_land = land == &full[s] ? on_land & ~bit : on_land | bit;
+        if (on_land & bit) land_ph ^= bit;
         if (++s == kSt) {
           s = 0;
           ph ^= 1u;
@@ -248,32 +256,74 @@ __global__ void __launch_bounds__(kThreads, 1) attend_tiles_kernel(const __grid_
       atomicOr_system(p.err, kErrWaitTimeout);
     }
     // Every copy lands before the CTA leaves, also when another role gave up before using it.
-    for (int j = max(0, loaded - kSt); j < loaded; ++j) wait_done(&full[j % kSt], (j / kSt) & 1);
+    // (A ragged V tile's copy lands on v_land; its slot's v_full then depends on warp 11, which may have left.)
+    for (int q = 0; q < kSt; ++q)
+      if ((on_land >> q) & 1) wait_done(&v_land[q], ((land_ph >> q) & 1) ^ 1u);
+      else if (q < loaded) wait_done(&full[q], ((loaded - 1 - q) / kSt) & 1);
     if (keys)
 #pragma unroll
       for (int i = 0; i < 2; ++i)
         if (q_loads[i]) wait_done(&q_full[i], (q_loads[i] - 1) & 1);
-  } else if (warp == 10) {
+  } else if (warp == 11) {
+    // ---------------------------------------------------------------- ragged V tiles
+    // What lies past the last key of a page may be anything, NaN included, and P V would meet it with weights
+    // of 0: it is cleared up to the next block of 16 keys, where P V stops.
+    Walk wk;
+    wk.init(p, total);
+    int s = 0, done = 0;
+    uint32_t land_ph = 0;  // parity by slot
+    bool ok = true;
+    while (ok && wk.w < total) {
+      for (int j = 0; j < wk.tiles; ++j) {
+        const int valid = wk.valid(j), upto = (valid + 15) & ~15;
+        if (valid < upto) {
+          ok = __all_sync(0xffffffffu, mbar_wait(&v_land[s], (land_ph >> s) & 1, abort_flag));
+          if (!ok) break;
+          land_ph ^= 1u << s;
+          for (int c = lane; c < (upto - valid) * kHalves * 8; c += 32) {
+            const int row = valid + c / (kHalves * 8), h = c / 8 % kHalves;
+            *reinterpret_cast<uint4*>(sV + s * kKeyBytes<D> + h * (kTileKeys * 128) + row * 128 + c % 8 * 16) =
+                make_uint4(0, 0, 0, 0);
+          }
+          fence_async_shared();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&v_full[s]);
+        }
+        if (++s == kSt) s = 0;
+      }
+      wk.next(p, total);
+    }
+    if (!ok && lane == 0) {
+      *abort_flag = 1;
+      atomicOr_system(p.err, kErrWaitTimeout);
+    }
+  } else {
     // ---------------------------------------------------------------- MMA issuer
-    Walk ws, wp;  // ws: the step (item, key tile) whose S is issued next, one ahead of P V's
+    // The whole warp walks the steps (item, key tile); one elected lane issues.  S runs one step ahead of P V:
+    // ws, js are the step whose S is issued next.
+    Walk ws, wp;
     ws.init(p, total);
     wp.init(p, total);
-    int js = 0, jp = 0;              // key tile within the item
-    int ks = 0, vs = 0;              // ring slots
+    int js = 0, jp = 0;
+    int ks = 0, vs = 0;  // ring slots
     uint32_t kph = 0, vph = 0;
     uint32_t q_ph = 0, p_ph = 0, oe_ph = 0;  // parity bits by row tile
     bool ok = true;
     const uint64_t dq = smem_desc_sw128(smem_u32(sQ)), dk = smem_desc_sw128(smem_u32(sK));
     const uint64_t dv = desc_mn(smem_u32(sV), kTileKeys * 128);
-    // S_i of the step at ws.
-    auto issue_s = [&](int i, const KeyTile& t) {
+    auto wait = [&](uint64_t* b, uint32_t parity) {
+      return __all_sync(0xffffffffu, mbar_wait_spin(b, parity, abort_flag));
+    };
+    // S_i of the step at ws, whose K is in slot ks.
+    auto issue_s = [&](int i) {
       if (js == 0) {
-        if (!__all_sync(0xffffffffu, mbar_wait(&q_full[i], (q_ph >> i) & 1, abort_flag))) return false;
+        if (!wait(&q_full[i], (q_ph >> i) & 1)) return false;
         q_ph ^= 1u << i;
       }
       tc_fence_after();
-      if (lane == 0) {
-        const uint32_t id = idesc_f16(kTileRows, (ws.seen(p, t, i) + 15) & ~15, kBf);
+      const uint32_t id = idesc_f16(kTileRows, ws.seen16(js, i), kBf);
+      const bool last = js == ws.count[i] - 1;
+      if (elect_one()) {
         const uint64_t a = dq + static_cast<uint64_t>(i * (kQBytes<D> >> 4));
         const uint64_t b = dk + static_cast<uint64_t>(ks * (kKeyBytes<D> >> 4));
 #pragma unroll
@@ -282,14 +332,14 @@ __global__ void __launch_bounds__(kThreads, 1) attend_tiles_kernel(const __grid_
           tc_mma_f16(tmem + i * 128, a + off, b + off, id, k > 0);
         }
         tc_commit(&s_full[i]);
-        if (js == ws.count[i] - 1) tc_commit(&q_empty[i]);
+        if (last) tc_commit(&q_empty[i]);
       }
       __syncwarp();
       return true;
     };
-    // Both row tiles' part in K of the step is issued: release the slot, move on.
+    // Both row tiles' S of the step is issued: release K's slot, move on.
     auto end_s = [&]() {
-      if (lane == 0) tc_commit(&k_empty[ks]);
+      if (elect_one()) tc_commit(&k_empty[ks]);
       __syncwarp();
       if (++ks == kSt) {
         ks = 0;
@@ -300,79 +350,59 @@ __global__ void __launch_bounds__(kThreads, 1) attend_tiles_kernel(const __grid_
         ws.next(p, total);
       }
     };
-    auto wait_k = [&]() { return __all_sync(0xffffffffu, mbar_wait(&k_full[ks], kph, abort_flag)); };
     if (ws.w < total) {
-      const KeyTile t = key_tile<kTileKeys>(ws.it, 0);
-      ok = wait_k();
+      ok = wait(&k_full[ks], kph);
 #pragma unroll
       for (int i = 0; i < 2; ++i)
-        if (ok && js < ws.count[i]) ok = issue_s(i, t);
+        if (ok && js < ws.count[i]) ok = issue_s(i);
       if (ok) end_s();
     }
     while (ok && wp.w < total) {
-      const KeyTile t = key_tile<kTileKeys>(wp.it, jp);
       const bool more = ws.w < total;
-      KeyTile ts{};
-      if (more) ts = key_tile<kTileKeys>(ws.it, js);
-      bool have_k = false, have_v = false;
+      bool have_v = false, have_k = false;
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
+        if (!ok) continue;
         if (jp < wp.count[i]) {
           if (jp == 0) {
             // The previous item's O has been read out of the accumulator.
-            ok = __all_sync(0xffffffffu, mbar_wait(&o_empty[i], ((oe_ph >> i) & 1) ^ 1u, abort_flag));
-            if (!ok) break;
+            ok = wait(&o_empty[i], ((oe_ph >> i) & 1) ^ 1u);
             oe_ph ^= 1u << i;
           }
-          if (!have_v) {
-            ok = __all_sync(0xffffffffu, mbar_wait(&v_full[vs], vph, abort_flag));
-            if (!ok) break;
-            have_v = true;
-            const int upto = (t.valid + 15) & ~15;
-            if (t.valid < upto) {
-              // What lies past the last key may be anything, NaN included, and meets weights of 0: clear it.
-              for (int c = lane; c < (upto - t.valid) * kHalves * 8; c += 32) {
-                const int row = t.valid + c / (kHalves * 8), h = c / 8 % kHalves;
-                *reinterpret_cast<uint4*>(sV + vs * kKeyBytes<D> + h * (kTileKeys * 128) + row * 128 + c % 8 * 16) =
-                    make_uint4(0, 0, 0, 0);
-              }
-              fence_async_shared();
-              __syncwarp();
-            }
-          }
-          const int n16 = (wp.seen(p, t, i) + 15) >> 4;
+          if (ok && !have_v) ok = have_v = wait(&v_full[vs], vph);
+          const int n16 = wp.seen16(jp, i) >> 4;
           const uint64_t b = dv + static_cast<uint64_t>(vs * (kKeyBytes<D> >> 4));
+          const uint32_t acc = jp > 0;
+          const bool last = jp == wp.count[i] - 1;
           constexpr uint32_t id = idesc_f16(kTileRows, D, kBf) | (1u << 16);
+          ok = ok && wait(&p_full[2 * i], (p_ph >> i) & 1);
+          if (!ok) continue;
+          tc_fence_after();
+          if (elect_one()) {
 #pragma unroll
-          for (int half = 0; half < 2; ++half) {
-            ok = __all_sync(0xffffffffu, mbar_wait_spin(&p_full[2 * i + half], (p_ph >> i) & 1, abort_flag));
-            if (!ok) break;
-            tc_fence_after();
-            if (lane == 0) {
-#pragma unroll
-              for (int k = 4 * half; k < 4 * half + 4; ++k)
-                if (k < n16)
-                  tc_mma_f16_ts(tmem + 256 + i * 128, tmem + i * 128 + 8 * k, b + 128 * k, id, jp > 0 || k > 0);
-            }
-            __syncwarp();
+            for (int k = 0; k < 4; ++k)
+              if (k < n16) tc_mma_f16_ts(tmem + 256 + i * 128, tmem + i * 128 + 8 * k, b + 128 * k, id, k > 0 ? 1u : acc);
           }
-          if (!ok) break;
-          p_ph ^= 1u << i;
-          if (jp == wp.count[i] - 1 && lane == 0) tc_commit(&o_full[i]);
           __syncwarp();
+          ok = wait(&p_full[2 * i + 1], (p_ph >> i) & 1);
+          if (!ok) continue;
+          tc_fence_after();
+          if (elect_one()) {
+#pragma unroll
+            for (int k = 4; k < 8; ++k)
+              if (k < n16) tc_mma_f16_ts(tmem + 256 + i * 128, tmem + i * 128 + 8 * k, b + 128 * k, id, 1u);
+            if (last) tc_commit(&o_full[i]);
+          }
+          __syncwarp();
+          p_ph ^= 1u << i;
         }
         if (more && js < ws.count[i]) {
-          if (!have_k) {
-            ok = wait_k();
-            if (!ok) break;
-            have_k = true;
-          }
-          ok = issue_s(i, ts);
-          if (!ok) break;
+          if (!have_k) ok = have_k = wait(&k_full[ks], kph);
+          ok = ok && issue_s(i);
         }
       }
       if (!ok) break;
-      if (lane == 0) tc_commit(&v_empty[vs]);
+      if (elect_one()) tc_commit(&v_empty[vs]);
       __syncwarp();
       if (++vs == kSt) {
         vs = 0;
@@ -384,7 +414,7 @@ __global__ void __launch_bounds__(kThreads, 1) attend_tiles_kernel(const __grid_
         wp.next(p, total);
       }
     }
-    if (lane == 0) {
+    if (elect_one()) {
       if (!ok) {
         *abort_flag = 1;
         atomicOr_system(p.err, kErrWaitTimeout);
@@ -459,7 +489,7 @@ __global__ void __launch_bounds__(kThreads, 1) attend_tiles_kernel(const __grid_
       for (int j = 0; j < n; ++j) {
         const KeyTile t = key_tile<kTileKeys>(wk.it, j);
         const int lim = min(t.valid, t.own ? own - t.base : t.valid);  // the row's visible keys: those below
-        const int n16 = (wk.seen(p, t, i) + 15) & ~15;               // columns that S has
+        const int n16 = wk.seen16(j, i);                             // columns that S has
         fail = !__all_sync(0xffffffffu, mbar_wait(&s_full[i], s_ph, abort_flag));
         if (fail) break;
         s_ph ^= 1u;
@@ -582,7 +612,7 @@ cudaError_t launch(const CUtensorMap& mq, const CUtensorMap& mk, const CUtensorM
     return cudaFuncSetAttribute(attend_tiles_kernel<T, D>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemBytes<D>);
   });
   if (e != cudaSuccess) return e;
-  const int total = p.n_items * (p.q_heads / p.fold);
+  const int total = p.n_items * p.groups;
   attend_tiles_kernel<T, D><<<std::min(total, device_sm_count()), kThreads, kSmemBytes<D>, st>>>(mq, mk, mv, p);
   return cudaGetLastError();
 }

@@ -65,7 +65,9 @@ cudaError_t step_attend(Act act, const AttendArgs& a, cudaStream_t st) {
   p.pages = a.pages;
   p.q_heads = a.q_heads;
   p.fold = a.fold;
+  p.groups = a.q_heads / a.fold;
   p.per_kv = a.q_heads / a.kv_heads / a.fold;
+  p.per = kTileRows / a.fold;
   p.page_size = a.pool.page_size;
   p.out = a.out;
   p.out_token = a.out_token;

@@ -12,7 +12,9 @@ struct AttendParams {
   const StepItem* items;
   const StepParts* parts;
   const int* pages;
-  int n_items, q_heads, fold, per_kv;  // per_kv: head groups of `fold` query heads to a key/value head
+  int n_items, q_heads, fold;
+  int groups, per_kv;  // head groups of `fold` query heads: all, and to a key/value head
+  int per;             // tokens of a row tile of the tensor-core kernel
   int page_size, box;                  // box: keys of one page copy
   void* out;
   int64_t out_token, out_head;
@@ -25,6 +27,19 @@ __device__ __forceinline__ float ex2_approx(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
+}
+
+// True in one lane of the (converged) warp.  tcgen05 instructions take their operands from uniform registers;
+// behind this election the compiler knows that one lane runs them, and issues them back to back, which behind
+// `lane == 0` it does not.
+__device__ __forceinline__ bool elect_one() {
+  uint32_t p;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t.reg .b32 r;\n\t"
+      "elect.sync r|p, 0xffffffff;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}\n"
+      : "=r"(p));
+  return p != 0;
 }
 
 __device__ __forceinline__ void tma_load_3d(void* dst, const CUtensorMap* map, uint64_t* bar, int x, int y, int z) {
