@@ -6,8 +6,9 @@
 // kernel is persistent, one CTA per SM; both row tiles share every K and V tile that a CTA loads.  Warp roles:
 //   warps 0..3, 4..7  softmax of row tile 0, 1: one row per thread,
 //   warp 8            TMA of Q and K, warp 9 TMA of V: page by page into rings of 128-key slots,
-//   warp 10           TMEM owner and issuer of the tcgen05.mma,
-//   warp 11           clears V tiles past their last key.
+//   warps 10, 11      issuers of the tcgen05.mma of row tile 0, 1 (one issuer for both spent more time between
+//                     its instructions than the tensor cores on them: 4600 cycles a step against 3500); warp
+//                     10 owns TMEM.
 // Per key tile and row tile i:
 //   S_i = Q_i K^T     tcgen05.mma M=128 N<=128 into TMEM columns of its own,
 //   softmax           scores by tcgen05.ld, masks, P = exp2(s - m) in 16 bits over S_i (tcgen05.st),
@@ -106,13 +107,39 @@ struct Walk {
     w = index(round);
     load(p, total);
   }
-  // Keys of tile j that were copied.
-  __device__ __forceinline__ int valid(int j) const {
-    return min(kTileKeys, j < na ? it.a1 - it.a0 - j * kTileKeys : it.b1 - it.b0 - (j - na) * kTileKeys);
-  }
   // Keys of tile j that some row of row tile i sees, at least 1 (masked then), in whole blocks of 16.
   __device__ __forceinline__ int seen16(int j, int i) const {
     const int k = j < na ? it.a1 - it.a0 - j * kTileKeys : own[i] - (j - na) * kTileKeys;
+    return (max(1, min(kTileKeys, k)) + 15) & ~15;
+  }
+};
+
+// The same walk by steps (item, key tile), as far as the issuer of row tile i needs it.
+struct Steps {
+  int w, round, j;
+  int na, prefix, own, count, tiles;
+
+  __device__ __forceinline__ void load(const AttendParams& p, int total, int i) {
+    j = 0;
+    w = Walk::index(round);
+    if (w >= total) return;
+    Walk wk;
+    wk.w = w;
+    wk.round = round;
+    wk.load(p, total);
+    na = wk.na;
+    prefix = wk.it.a1 - wk.it.a0;
+    own = i ? wk.own[1] : wk.own[0];
+    count = i ? wk.count[1] : wk.count[0];
+    tiles = wk.tiles;
+  }
+  __device__ __forceinline__ void next(const AttendParams& p, int total, int i) {
+    if (++j < tiles) return;
+    ++round;
+    load(p, total, i);
+  }
+  __device__ __forceinline__ int seen16() const {
+    const int k = j < na ? prefix - j * kTileKeys : own - (j - na) * kTileKeys;
     return (max(1, min(kTileKeys, k)) + 15) & ~15;
   }
 };
@@ -142,10 +169,11 @@ __global__ void __launch_bounds__(kThreads, 1) attend_tiles_kernel(const __grid_
   uint64_t* p_full = s_full + 2;       // [2][2] P of the row tile, keys 0-63 and 64-127
   uint64_t* o_full = p_full + 4;       // [2] last P V of the item done
   uint64_t* o_empty = o_full + 2;      // [2] the item's O has been read
-  uint64_t* drain = o_empty + 2;
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain + 1);
+  uint64_t* turn = o_empty + 2;        // [2] issuer 0, 1 may issue: the other has issued its step
+  uint64_t* drain = turn + 2;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain + 2);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
-  static_assert((2 + 2 + 5 * kSt + 2 + 4 + 2 + 2 + 1) * 8 + 8 <= 512, "barrier area");
+  static_assert((2 + 2 + 5 * kSt + 2 + 4 + 2 + 2 + 2 + 2) * 8 + 8 <= 512, "barrier area");
 
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   const int total = p.n_items * p.groups;
@@ -160,15 +188,17 @@ __global__ void __launch_bounds__(kThreads, 1) attend_tiles_kernel(const __grid_
       mbar_init(&p_full[2 * i + 1], 4);
       mbar_init(&o_full[i], 1);
       mbar_init(&o_empty[i], 4);
+      mbar_init(&turn[i], 1);
     }
     for (int s = 0; s < kSt; ++s) {
       mbar_init(&k_full[s], 1);
-      mbar_init(&k_empty[s], 1);
+      mbar_init(&k_empty[s], 2);
       mbar_init(&v_full[s], 1);
-      mbar_init(&v_empty[s], 1);
+      mbar_init(&v_empty[s], 2);
       mbar_init(&v_land[s], 1);
     }
-    mbar_init(drain, 1);
+    mbar_init(&drain[0], 1);
+    mbar_init(&drain[1], 1);
     *abort_flag = 0;
     fence_mbar_init();
     tma_prefetch_desc(&mq);
@@ -197,6 +227,21 @@ __global__ void __launch_bounds__(kThreads, 1) attend_tiles_kernel(const __grid_
     int s = 0, loaded = 0, q_loads[2] = {0, 0};
     uint32_t ph = 0;
     uint32_t on_land = 0, land_ph = 0;  // by slot: the last copy was a ragged V tile's; parity of v_land
+    int ragged = 0, ragged_slot = 0;    // keys of the ragged tile that is still to be cleared
+    auto clear = [&](int slot, int valid) {
+      if (!__all_sync(0xffffffffu, mbar_wait(&v_land[slot], (land_ph >> slot) & 1, abort_flag))) return false;
+      land_ph ^= 1u << slot;
+      const int upto = (valid + 15) & ~15;
+      for (int c = lane; c < (upto - valid) * kHalves * 8; c += 32) {
+        const int row = valid + c / (kHalves * 8), h = c / 8 % kHalves;
+        *reinterpret_cast<uint4*>(sV + slot * kKeyBytes<D> + h * (kTileKeys * 128) + row * 128 + c % 8 * 16) =
+            make_uint4(0, 0, 0, 0);
+      }
+      fence_async_shared();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&v_full[slot]);
+      return true;
+    };
     bool ok = true;
     int page = 0;
     KeyTile t{};
@@ -224,9 +269,17 @@ __global__ void __launch_bounds__(kThreads, 1) attend_tiles_kernel(const __grid_
         const int hg = wk.hg;
         const bool last = j + 1 == wk.tiles;
         const int n = TileCopy<kTileKeys, kHalves>::copies(t, p.box);
+        if (ragged) {
+          // The tile before: its copy has had the time that this slot takes to fall free.
+          ok = clear(ragged_slot, ragged);
+          ragged = 0;
+          if (!ok) break;
+        }
         ok = __all_sync(0xffffffffu, mbar_wait(&empty[s], ph ^ 1u, abort_flag));
         if (!ok) break;
-        // A V tile with keys past the last in its last block of 16 goes by way of warp 11.
+        // What lies past the last key of a page may be anything, NaN included, and P V would meet it with weights
+        // of 0: a V tile that ends inside a block of 16 keys lands on a barrier of its own, and this warp clears
+        // the rest of the block before it is announced.
         uint64_t* land = !keys && (t.valid & 15) ? &v_land[s] : &full[s];
         if (lane == 0) mbar_arrive_expect_tx(land, n * p.box * D * 2);
         __syncwarp();
@@ -235,7 +288,10 @@ __global__ void __launch_bounds__(kThreads, 1) attend_tiles_kernel(const __grid_
         ++loaded;
         const uint32_t bit = 1u << s;
         on_land = land == &full[s] ? on_land & ~bit : on_land | bit;
-        if (on_land & bit) land_ph ^= bit;
+        if (on_land & bit) {
+          ragged = t.valid;
+          ragged_slot = s;
+        }
         if (++s == kSt) {
           s = 0;
           ph ^= 1u;
@@ -251,178 +307,140 @@ __global__ void __launch_bounds__(kThreads, 1) attend_tiles_kernel(const __grid_
         page = TileCopy<kTileKeys, kHalves>::page_of(p, t, lane);
       }
     }
+    if (ok && ragged) {
+      ok = clear(ragged_slot, ragged);
+      ragged = 0;
+    }
     if (!ok && lane == 0) {
       *abort_flag = 1;
       atomicOr_system(p.err, kErrWaitTimeout);
     }
     // Every copy lands before the CTA leaves, also when another role gave up before using it.
-    // (A ragged V tile's copy lands on v_land; its slot's v_full then depends on warp 11, which may have left.)
-    for (int q = 0; q < kSt; ++q)
-      if ((on_land >> q) & 1) wait_done(&v_land[q], ((land_ph >> q) & 1) ^ 1u);
-      else if (q < loaded) wait_done(&full[q], ((loaded - 1 - q) / kSt) & 1);
+    for (int q = 0; q < kSt && q < loaded; ++q) {
+      if (!((on_land >> q) & 1)) wait_done(&full[q], ((loaded - 1 - q) / kSt) & 1);
+      else if (ragged && ragged_slot == q) wait_done(&v_land[q], (land_ph >> q) & 1);  // not cleared: gave up
+    }
     if (keys)
 #pragma unroll
       for (int i = 0; i < 2; ++i)
         if (q_loads[i]) wait_done(&q_full[i], (q_loads[i] - 1) & 1);
-  } else if (warp == 11) {
-    // ---------------------------------------------------------------- ragged V tiles
-    // What lies past the last key of a page may be anything, NaN included, and P V would meet it with weights
-    // of 0: it is cleared up to the next block of 16 keys, where P V stops.
-    Walk wk;
-    wk.init(p, total);
-    int s = 0, done = 0;
-    uint32_t land_ph = 0;  // parity by slot
-    bool ok = true;
-    while (ok && wk.w < total) {
-      for (int j = 0; j < wk.tiles; ++j) {
-        const int valid = wk.valid(j), upto = (valid + 15) & ~15;
-        if (valid < upto) {
-          ok = __all_sync(0xffffffffu, mbar_wait(&v_land[s], (land_ph >> s) & 1, abort_flag));
-          if (!ok) break;
-          land_ph ^= 1u << s;
-          for (int c = lane; c < (upto - valid) * kHalves * 8; c += 32) {
-            const int row = valid + c / (kHalves * 8), h = c / 8 % kHalves;
-            *reinterpret_cast<uint4*>(sV + s * kKeyBytes<D> + h * (kTileKeys * 128) + row * 128 + c % 8 * 16) =
-                make_uint4(0, 0, 0, 0);
-          }
-          fence_async_shared();
-          __syncwarp();
-          if (lane == 0) mbar_arrive(&v_full[s]);
-        }
-        if (++s == kSt) s = 0;
-      }
-      wk.next(p, total);
-    }
-    if (!ok && lane == 0) {
-      *abort_flag = 1;
-      atomicOr_system(p.err, kErrWaitTimeout);
-    }
   } else {
-    // ---------------------------------------------------------------- MMA issuer
-    // The whole warp walks the steps (item, key tile); one elected lane issues.  S runs one step ahead of P V:
-    // ws, js are the step whose S is issued next.
-    Walk ws, wp;
-    ws.init(p, total);
-    wp.init(p, total);
-    int js = 0, jp = 0;
+    // ---------------------------------------------------------------- MMA issuers
+    // Warp 10 + i walks the steps for row tile i; one elected lane issues.  S runs one step ahead of P V.
+    const int i = warp - 10;
+    Steps ws, wp;  // of the next S, of the next P V
+    ws.round = wp.round = 0;
+    ws.load(p, total, i);
+    wp.load(p, total, i);
     int ks = 0, vs = 0;  // ring slots
     uint32_t kph = 0, vph = 0;
-    uint32_t q_ph = 0, p_ph = 0, oe_ph = 0;  // parity bits by row tile
+    uint32_t q_ph = 0, p_ph = 0, oe_ph = 1, t_ph = i ^ 1;
     bool ok = true;
-    const uint64_t dq = smem_desc_sw128(smem_u32(sQ)), dk = smem_desc_sw128(smem_u32(sK));
+    const uint64_t dq = smem_desc_sw128(smem_u32(sQ + i * kQBytes<D>)), dk = smem_desc_sw128(smem_u32(sK));
     const uint64_t dv = desc_mn(smem_u32(sV), kTileKeys * 128);
+    const uint32_t ts = tmem + i * 128, to = tmem + 256 + i * 128;
     auto wait = [&](uint64_t* b, uint32_t parity) {
       return __all_sync(0xffffffffu, mbar_wait_spin(b, parity, abort_flag));
     };
-    // S_i of the step at ws, whose K is in slot ks.
-    auto issue_s = [&](int i) {
-      if (js == 0) {
-        if (!wait(&q_full[i], (q_ph >> i) & 1)) return false;
-        q_ph ^= 1u << i;
-      }
-      tc_fence_after();
-      const uint32_t id = idesc_f16(kTileRows, ws.seen16(js, i), kBf);
-      const bool last = js == ws.count[i] - 1;
-      if (elect_one()) {
-        const uint64_t a = dq + static_cast<uint64_t>(i * (kQBytes<D> >> 4));
-        const uint64_t b = dk + static_cast<uint64_t>(ks * (kKeyBytes<D> >> 4));
-#pragma unroll
-        for (int k = 0; k < D / 16; ++k) {
-          const uint64_t off = (k / 4) * (kTileRows * 128 >> 4) + 2 * (k % 4);
-          tc_mma_f16(tmem + i * 128, a + off, b + off, id, k > 0);
+    // S of the step at ws, then release of its K.
+    // (Both issuers wait for every K and V, also where their row tile has no part in it: a slot is released
+    // once by each, in the fill that it holds.)
+    auto step_s = [&]() {
+      if (!wait(&k_full[ks], kph)) return false;
+      if (ws.j < ws.count) {
+        if (ws.j == 0) {
+          if (!wait(&q_full[i], q_ph)) return false;
+          q_ph ^= 1u;
         }
-        tc_commit(&s_full[i]);
-        if (last) tc_commit(&q_empty[i]);
+        tc_fence_after();
+        const uint32_t id = idesc_f16(kTileRows, ws.seen16(), kBf);
+        const bool last = ws.j == ws.count - 1;
+        if (elect_one()) {
+          const uint64_t b = dk + static_cast<uint64_t>(ks * (kKeyBytes<D> >> 4));
+#pragma unroll
+          for (int k = 0; k < D / 16; ++k) {
+            const uint64_t off = (k / 4) * (kTileRows * 128 >> 4) + 2 * (k % 4);
+            tc_mma_f16(ts, dq + off, b + off, id, k > 0);
+          }
+          tc_commit(&s_full[i]);
+          if (last) tc_commit(&q_empty[i]);
+          tc_commit(&k_empty[ks]);
+        }
+      } else if (elect_one()) {
+        tc_commit(&k_empty[ks]);
       }
-      __syncwarp();
-      return true;
-    };
-    // Both row tiles' S of the step is issued: release K's slot, move on.
-    auto end_s = [&]() {
-      if (elect_one()) tc_commit(&k_empty[ks]);
       __syncwarp();
       if (++ks == kSt) {
         ks = 0;
         kph ^= 1u;
       }
-      if (++js == ws.tiles) {
-        js = 0;
-        ws.next(p, total);
-      }
+      ws.next(p, total, i);
+      return true;
     };
-    if (ws.w < total) {
-      ok = wait(&k_full[ks], kph);
-#pragma unroll
-      for (int i = 0; i < 2; ++i)
-        if (ok && js < ws.count[i]) ok = issue_s(i);
-      if (ok) end_s();
-    }
+    if (ws.w < total) ok = step_s();
     while (ok && wp.w < total) {
-      const bool more = ws.w < total;
-      bool have_v = false, have_k = false;
-#pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        if (!ok) continue;
-        if (jp < wp.count[i]) {
-          if (jp == 0) {
-            // The previous item's O has been read out of the accumulator.
-            ok = wait(&o_empty[i], ((oe_ph >> i) & 1) ^ 1u);
-            oe_ph ^= 1u << i;
-          }
-          if (ok && !have_v) ok = have_v = wait(&v_full[vs], vph);
-          const int n16 = wp.seen16(jp, i) >> 4;
-          const uint64_t b = dv + static_cast<uint64_t>(vs * (kKeyBytes<D> >> 4));
-          const uint32_t acc = jp > 0;
-          const bool last = jp == wp.count[i] - 1;
-          constexpr uint32_t id = idesc_f16(kTileRows, D, kBf) | (1u << 16);
-          ok = ok && wait(&p_full[2 * i], (p_ph >> i) & 1);
-          if (!ok) continue;
-          tc_fence_after();
-          if (elect_one()) {
-#pragma unroll
-            for (int k = 0; k < 4; ++k)
-              if (k < n16) tc_mma_f16_ts(tmem + 256 + i * 128, tmem + i * 128 + 8 * k, b + 128 * k, id, k > 0 ? 1u : acc);
-          }
-          __syncwarp();
-          ok = wait(&p_full[2 * i + 1], (p_ph >> i) & 1);
-          if (!ok) continue;
-          tc_fence_after();
-          if (elect_one()) {
-#pragma unroll
-            for (int k = 4; k < 8; ++k)
-              if (k < n16) tc_mma_f16_ts(tmem + 256 + i * 128, tmem + i * 128 + 8 * k, b + 128 * k, id, 1u);
-            if (last) tc_commit(&o_full[i]);
-          }
-          __syncwarp();
-          p_ph ^= 1u << i;
-        }
-        if (more && js < ws.count[i]) {
-          if (!have_k) ok = have_k = wait(&k_full[ks], kph);
-          ok = ok && issue_s(i);
-        }
-      }
+      ok = wait(&v_full[vs], vph);
       if (!ok) break;
-      if (elect_one()) tc_commit(&v_empty[vs]);
+      if (wp.j < wp.count) {
+        if (wp.j == 0) {
+          // The previous item's O has been read out of the accumulator.
+          ok = wait(&o_empty[i], oe_ph);
+          oe_ph ^= 1u;
+        }
+        ok = ok && wait(&p_full[2 * i], p_ph);
+        if (!ok) break;
+      }
+      // The issuers take turns, so that one row tile's MMAs run in one piece: interleaved, both row tiles' scores
+      // would come at the same time, and both softmaxes would run, and the tensor cores rest, at the same time.
+      ok = wait(&turn[i], t_ph);
+      if (!ok) break;
+      t_ph ^= 1u;
+      if (wp.j < wp.count) {
+        const int n16 = wp.seen16() >> 4;
+        const uint64_t b = dv + static_cast<uint64_t>(vs * (kKeyBytes<D> >> 4));
+        const uint32_t acc = wp.j > 0;
+        const bool last = wp.j == wp.count - 1;
+        constexpr uint32_t id = idesc_f16(kTileRows, D, kBf) | (1u << 16);
+        tc_fence_after();
+        if (elect_one()) {
+#pragma unroll
+          for (int k = 0; k < 4; ++k)
+            if (k < n16) tc_mma_f16_ts(to, ts + 8 * k, b + 128 * k, id, k > 0 ? 1u : acc);
+        }
+        __syncwarp();
+        ok = wait(&p_full[2 * i + 1], p_ph);
+        if (!ok) break;
+        p_ph ^= 1u;
+        tc_fence_after();
+        if (elect_one()) {
+#pragma unroll
+          for (int k = 4; k < 8; ++k)
+            if (k < n16) tc_mma_f16_ts(to, ts + 8 * k, b + 128 * k, id, 1u);
+          if (last) tc_commit(&o_full[i]);
+          tc_commit(&v_empty[vs]);
+        }
+      } else if (elect_one()) {
+        tc_commit(&v_empty[vs]);
+      }
       __syncwarp();
       if (++vs == kSt) {
         vs = 0;
         vph ^= 1u;
       }
-      if (more) end_s();
-      if (++jp == wp.tiles) {
-        jp = 0;
-        wp.next(p, total);
-      }
+      wp.next(p, total, i);
+      if (ws.w < total) ok = step_s();
+      if (lane == 0) mbar_arrive(&turn[i ^ 1]);
+      __syncwarp();
     }
     if (elect_one()) {
       if (!ok) {
         *abort_flag = 1;
         atomicOr_system(p.err, kErrWaitTimeout);
       }
-      tc_commit(drain);  // every MMA is done before TMEM is released
+      tc_commit(&drain[i]);  // every MMA is done before TMEM is released
     }
     __syncwarp();
-    if (!wait_done(drain, 0) && lane == 0) atomicOr_system(p.err, kErrWaitTimeout);
+    if (!wait_done(&drain[i], 0) && lane == 0) atomicOr_system(p.err, kErrWaitTimeout);
   }
   } else {
     // ---------------------------------------------------------------- softmax
@@ -495,26 +513,44 @@ __global__ void __launch_bounds__(kThreads, 1) attend_tiles_kernel(const __grid_
         s_ph ^= 1u;
         tc_fence_after();
         float s[4][32];
+        float mt;
+        if (__all_sync(0xffffffffu, lim >= kTileKeys)) {
+          // Every key is visible to every row of the warp.  Six chains of maxima; the second half's scores
+          // arrive while the first half's are compared.
+          tmem_ld32(ts, s[0]);
+          tmem_ld32(ts + 32, s[1]);
+          tc_wait_ld();
+          tmem_ld32(ts + 64, s[2]);
+          tmem_ld32(ts + 96, s[3]);
+          float mx[6];
 #pragma unroll
-        for (int c = 0; c < 4; ++c)
-          if (32 * c < n16) tmem_ld32(ts + 32 * c, s[c]);
-        tc_wait_ld();
-        float mt = -INFINITY;
+          for (int e = 0; e < 6; ++e) mx[e] = fmaxf(s[0][2 * e], s[0][2 * e + 1]);
 #pragma unroll
-        for (int c = 0; c < 4; ++c) {
-          if (32 * c >= n16) continue;
-          const int k = lim - 32 * c;
-          if (!__all_sync(0xffffffffu, k >= 32)) {
+          for (int e = 12; e < 64; e += 2) mx[e / 2 % 6] = fmax3(mx[e / 2 % 6], s[e >> 5][e & 31], s[e >> 5][(e & 31) + 1]);
+          tc_wait_ld();
+#pragma unroll
+          for (int e = 64; e < 128; e += 2) mx[e / 2 % 6] = fmax3(mx[e / 2 % 6], s[e >> 5][e & 31], s[e >> 5][(e & 31) + 1]);
+          mt = fmaxf(fmax3(mx[0], mx[1], mx[2]), fmax3(mx[3], mx[4], mx[5]));
+        } else {
+#pragma unroll
+          for (int c = 0; c < 4; ++c)
+            if (32 * c < n16) tmem_ld32(ts + 32 * c, s[c]);
+          tc_wait_ld();
+          mt = -INFINITY;
+#pragma unroll
+          for (int c = 0; c < 4; ++c) {
+            if (32 * c >= n16) continue;
+            const int k = lim - 32 * c;
             const uint32_t vis = k <= 0 ? 0u : k >= 32 ? 0xffffffffu : (1u << k) - 1u;
 #pragma unroll
             for (int e = 0; e < 32; ++e)
               if (!((vis >> e) & 1u)) s[c][e] = -INFINITY;
-          }
-          float mx[4] = {fmax3(s[c][0], s[c][1], s[c][2]), fmax3(s[c][3], s[c][4], s[c][5]),
-                         fmax3(s[c][6], s[c][7], s[c][8]), fmax3(s[c][9], s[c][10], s[c][11])};
+            float mx[4] = {fmax3(s[c][0], s[c][1], s[c][2]), fmax3(s[c][3], s[c][4], s[c][5]),
+                           fmax3(s[c][6], s[c][7], s[c][8]), fmax3(s[c][9], s[c][10], s[c][11])};
 #pragma unroll
-          for (int e = 12; e < 32; e += 2) mx[(e >> 1) & 3] = fmax3(mx[(e >> 1) & 3], s[c][e], s[c][e + 1]);
-          mt = fmaxf(mt, fmax3(mx[0], mx[1], fmaxf(mx[2], mx[3])));
+            for (int e = 12; e < 32; e += 2) mx[(e >> 1) & 3] = fmax3(mx[(e >> 1) & 3], s[c][e], s[c][e + 1]);
+            mt = fmaxf(mt, fmax3(mx[0], mx[1], fmaxf(mx[2], mx[3])));
+          }
         }
         mt *= p.scale_log2;
         const bool need = m != kNone && mt > m + kRescale;
