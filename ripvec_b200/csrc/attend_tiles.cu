@@ -6,19 +6,19 @@
 // kernel is persistent, one CTA per SM; both row tiles share every K and V tile that a CTA loads.  Warp roles:
 //   warps 0..3, 4..7  softmax of row tile 0, 1: one row per thread,
 //   warp 8            TMA of Q and K, warp 9 TMA of V: page by page into rings of 128-key slots,
-//   warps 10, 11      issuers of the tcgen05.mma of row tile 0, 1 (one issuer for both spent more time between
-//                     its instructions than the tensor cores on them: 4600 cycles a step against 3500); warp
-//                     10 owns TMEM.
-// Per key tile and row tile i:
-//   S_i = Q_i K^T     tcgen05.mma M=128 N<=128 into TMEM columns of its own,
-//   softmax           scores by tcgen05.ld, masks, P = exp2(s - m) in 16 bits over S_i (tcgen05.st),
-//   O_i += P V        P from TMEM, V as an MN-major operand, in two halves of 64 keys, so that the first half
-//                     multiplies while the second half's exponentials are computed.
-// While one row tile's softmax runs, the tensor cores work on the other.  The reference maximum m moves only
-// when a row's maximum grows by more than 2^8; then the row's O is rescaled in TMEM.  S of a tile is issued
-// after P V of the tile before it by the same thread, so the barrier that announces S also means that the
-// earlier P V is done: rescaling needs no wait of its own.  An item's O is read out after the next item's
-// first P is written, before that item's first P V.
+//   warps 10, 11      issuers of row tile 0's, 1's S; warp 10 owns TMEM,
+//   warps 12, 13      issuers of row tile 0's, 1's P V.
+// Work goes by half tiles of 64 keys.  Per half tile and row tile i:
+//   S_i = Q_i K^T     tcgen05.mma M=128 N<=64 into one of the row tile's two score buffers in TMEM,
+//   softmax           scores by tcgen05.ld, masks, P = exp2(s - m) in 16 bits over the scores (tcgen05.st),
+//   O_i += P V        P from TMEM, V as an MN-major operand.
+// S of a buffer is issued as soon as the P V that read the buffer's last P is done (MMAs of different shapes and
+// accumulators are not ordered among themselves), so a softmax warp finds its next scores ready when it has
+// written a P.  An issuing warp spends some 100 cycles on each wait and 30 on each MMA, one after the other: with
+// S and P V of a row tile from one warp that was 2300 cycles a half tile, and the softmax waited for it.  The
+// reference maximum m moves only when a row's maximum grows by more than 2^8; then the row's O is rescaled in
+// TMEM, once the P V before is done.  An item's O is read out after the next item's first P is written, before
+// that item's first P V.
 #include <algorithm>
 
 #include "step_attend.cuh"
@@ -27,12 +27,13 @@ namespace rv {
 
 namespace {
 
-constexpr int kThreads = 384;   // three warpgroups
-// Registers a thread: the softmax warpgroups hold a row of 128 scores each and take some of the third's.  The
-// launch must bring what the split adds up to (checked before the first launch): 2 * 208 + 88 = 3 * 168.
-constexpr int kLaunchRegs = 168, kSoftmaxRegs = 208, kOtherRegs = 88;
-static_assert(2 * kSoftmaxRegs + kOtherRegs <= 3 * kLaunchRegs, "register split");
-constexpr int kTmemCols = 512;  // S0, S1 at 0, 128; O0, O1 at 256, 384
+constexpr int kThreads = 512;   // four warpgroups
+// Registers a thread: the softmax warpgroups hold 64 scores of a row each and take some of the others'.  The
+// launch must bring what the split adds up to (checked before the first launch): 2 * 160 + 2 * 96 = 4 * 128.
+constexpr int kLaunchRegs = 128, kSoftmaxRegs = 160, kOtherRegs = 96;
+static_assert(2 * kSoftmaxRegs + 2 * kOtherRegs <= 4 * kLaunchRegs, "register split");
+constexpr int kTmemCols = 512;  // scores of row tile i at 128 i and 128 i + 64, O at 256 + 128 i
+constexpr int kHalfKeys = 64;
 
 template <int D>
 constexpr int kStages = D == 128 ? 2 : 4;  // of K and of V
@@ -114,7 +115,7 @@ struct Walk {
   }
 };
 
-// The same walk by steps (item, key tile), as far as the issuer of row tile i needs it.
+// The same walk by key tiles, as far as an issuer of one row tile needs it.
 struct Steps {
   int w, round, j;
   int na, prefix, own, count, tiles;
@@ -133,12 +134,18 @@ struct Steps {
     count = i ? wk.count[1] : wk.count[0];
     tiles = wk.tiles;
   }
+  __device__ __forceinline__ void init(const AttendParams& p, int total, int i) {
+    round = 0;
+    load(p, total, i);
+  }
   __device__ __forceinline__ void next(const AttendParams& p, int total, int i) {
     if (++j < tiles) return;
     ++round;
     load(p, total, i);
   }
+  // As Walk::seen16, 0 where the row tile has no part in the key tile.
   __device__ __forceinline__ int seen16() const {
+    if (j >= count) return 0;
     const int k = j < na ? prefix - j * kTileKeys : own - (j - na) * kTileKeys;
     return (max(1, min(kTileKeys, k)) + 15) & ~15;
   }
@@ -165,15 +172,15 @@ __global__ void __launch_bounds__(kThreads, 1) attend_tiles_kernel(const __grid_
   uint64_t* v_full = k_empty + kSt;    // [kSt]
   uint64_t* v_empty = v_full + kSt;    // [kSt] both row tiles' P V are done
   uint64_t* v_land = v_empty + kSt;    // [kSt] a ragged V tile landed, to be cleared past its keys
-  uint64_t* s_full = v_land + kSt;    // [2] scores in TMEM
-  uint64_t* p_full = s_full + 2;       // [2][2] P of the row tile, keys 0-63 and 64-127
-  uint64_t* o_full = p_full + 4;       // [2] last P V of the item done
+  uint64_t* s_full = v_land + kSt;     // [2][2] scores of the row tile's buffer in TMEM
+  uint64_t* p_full = s_full + 4;       // [2][2] P of the buffer
+  uint64_t* pv_done = p_full + 4;      // [2][2] P V of the buffer's P
+  uint64_t* o_full = pv_done + 4;      // [2] the item's last P V
   uint64_t* o_empty = o_full + 2;      // [2] the item's O has been read
-  uint64_t* turn = o_empty + 2;        // [2] issuer 0, 1 may issue: the other has issued its step
-  uint64_t* drain = turn + 2;
+  uint64_t* drain = o_empty + 2;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain + 2);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
-  static_assert((2 + 2 + 5 * kSt + 2 + 4 + 2 + 2 + 2 + 2) * 8 + 8 <= 512, "barrier area");
+  static_assert((2 + 2 + 5 * kSt + 4 + 4 + 4 + 2 + 2 + 2) * 8 + 8 <= 512, "barrier area");
 
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   const int total = p.n_items * p.groups;
@@ -183,12 +190,13 @@ __global__ void __launch_bounds__(kThreads, 1) attend_tiles_kernel(const __grid_
     for (int i = 0; i < 2; ++i) {
       mbar_init(&q_full[i], 1);
       mbar_init(&q_empty[i], 1);
-      mbar_init(&s_full[i], 1);
-      mbar_init(&p_full[2 * i], 4);
-      mbar_init(&p_full[2 * i + 1], 4);
+      for (int k = 0; k < 2; ++k) {
+        mbar_init(&s_full[2 * i + k], 1);
+        mbar_init(&p_full[2 * i + k], 4);
+        mbar_init(&pv_done[2 * i + k], 1);
+      }
       mbar_init(&o_full[i], 1);
       mbar_init(&o_empty[i], 4);
-      mbar_init(&turn[i], 1);
     }
     for (int s = 0; s < kSt; ++s) {
       mbar_init(&k_full[s], 1);
@@ -197,8 +205,8 @@ __global__ void __launch_bounds__(kThreads, 1) attend_tiles_kernel(const __grid_
       mbar_init(&v_empty[s], 2);
       mbar_init(&v_land[s], 1);
     }
-    mbar_init(&drain[0], 1);
-    mbar_init(&drain[1], 1);
+    mbar_init(&drain[0], 2);
+    mbar_init(&drain[1], 2);
     *abort_flag = 0;
     fence_mbar_init();
     tma_prefetch_desc(&mq);
@@ -324,113 +332,113 @@ __global__ void __launch_bounds__(kThreads, 1) attend_tiles_kernel(const __grid_
 #pragma unroll
       for (int i = 0; i < 2; ++i)
         if (q_loads[i]) wait_done(&q_full[i], (q_loads[i] - 1) & 1);
-  } else {
+  } else if (warp < 14) {
     // ---------------------------------------------------------------- MMA issuers
-    // Warp 10 + i walks the steps for row tile i; one elected lane issues.  S runs one step ahead of P V.
-    const int i = warp - 10;
-    Steps ws, wp;  // of the next S, of the next P V
-    ws.round = wp.round = 0;
-    ws.load(p, total, i);
-    wp.load(p, total, i);
-    int ks = 0, vs = 0;  // ring slots
-    uint32_t kph = 0, vph = 0;
-    uint32_t q_ph = 0, p_ph = 0, oe_ph = 1, t_ph = i ^ 1;
+    // The whole warp walks the key tiles; one elected lane issues.  Every issuer waits for every K (V), also where
+    // its row tile has no part in it: a slot is released once by each row tile, in the fill that it holds.
+    const int i = warp & 1;
+    Steps st;
+    st.init(p, total, i);
+    int slot = 0;
+    uint32_t ph = 0, t_ph = 0;  // parity of the ring, of this row tile's key tiles
+    uint32_t q_ph = 0, oe_ph = 1;
     bool ok = true;
-    const uint64_t dq = smem_desc_sw128(smem_u32(sQ + i * kQBytes<D>)), dk = smem_desc_sw128(smem_u32(sK));
-    const uint64_t dv = desc_mn(smem_u32(sV), kTileKeys * 128);
     const uint32_t ts = tmem + i * 128, to = tmem + 256 + i * 128;
-    auto wait = [&](uint64_t* b, uint32_t parity) {
+    auto wait = [&](uint64_t* b, uint32_t parity) -> bool {
       return __all_sync(0xffffffffu, mbar_wait_spin(b, parity, abort_flag));
     };
-    // S of the step at ws, then release of its K.
-    // (Both issuers wait for every K and V, also where their row tile has no part in it: a slot is released
-    // once by each, in the fill that it holds.)
-    auto step_s = [&]() {
-      if (!wait(&k_full[ks], kph)) return false;
-      if (ws.j < ws.count) {
-        if (ws.j == 0) {
-          if (!wait(&q_full[i], q_ph)) return false;
+    if (warp < 12) {
+      const uint64_t dq = smem_desc_sw128(smem_u32(sQ + i * kQBytes<D>)), dk = smem_desc_sw128(smem_u32(sK));
+      while (st.w < total) {
+        const int seen = st.seen16();
+        const bool last = st.j == st.count - 1;
+        ok = wait(&k_full[slot], ph);
+        if (ok && seen && st.j == 0) {
+          ok = wait(&q_full[i], q_ph);
           q_ph ^= 1u;
         }
-        tc_fence_after();
-        const uint32_t id = idesc_f16(kTileRows, ws.seen16(), kBf);
-        const bool last = ws.j == ws.count - 1;
-        if (elect_one()) {
-          const uint64_t b = dk + static_cast<uint64_t>(ks * (kKeyBytes<D> >> 4));
+        if (seen) {
 #pragma unroll
-          for (int k = 0; k < D / 16; ++k) {
-            const uint64_t off = (k / 4) * (kTileRows * 128 >> 4) + 2 * (k % 4);
-            tc_mma_f16(ts, dq + off, b + off, id, k > 0);
+          for (int h = 0; h < 2; ++h) {
+            // The last P of the buffer has been used.
+            ok = ok && wait(&pv_done[2 * i + h], t_ph ^ 1u);
+            if (!ok) break;
+            tc_fence_after();
+            const int n = min(kHalfKeys, seen - h * kHalfKeys);
+            const uint32_t id = idesc_f16(kTileRows, n, kBf);
+            const uint64_t b = dk + static_cast<uint64_t>(slot * (kKeyBytes<D> >> 4) + h * (kHalfKeys * 128 >> 4));
+            if (elect_one()) {
+              if (n > 0) {
+#pragma unroll
+                for (int k = 0; k < D / 16; ++k) {
+                  const uint64_t off = (k / 4) * (kTileRows * 128 >> 4) + 2 * (k % 4);
+                  tc_mma_f16(ts + h * kHalfKeys, dq + off, b + off, id, k > 0);
+                }
+              }
+              tc_commit(&s_full[2 * i + h]);
+              if (h == 1) {
+                tc_commit(&k_empty[slot]);
+                if (last) tc_commit(&q_empty[i]);
+              }
+            }
+            __syncwarp();
           }
-          tc_commit(&s_full[i]);
-          if (last) tc_commit(&q_empty[i]);
-          tc_commit(&k_empty[ks]);
+          t_ph ^= 1u;
+        } else if (ok && lane == 0) {
+          mbar_arrive(&k_empty[slot]);
         }
-      } else if (elect_one()) {
-        tc_commit(&k_empty[ks]);
+        if (!ok) break;
+        if (++slot == kSt) {
+          slot = 0;
+          ph ^= 1u;
+        }
+        st.next(p, total, i);
       }
-      __syncwarp();
-      if (++ks == kSt) {
-        ks = 0;
-        kph ^= 1u;
-      }
-      ws.next(p, total, i);
-      return true;
-    };
-    if (ws.w < total) ok = step_s();
-    while (ok && wp.w < total) {
-      ok = wait(&v_full[vs], vph);
-      if (!ok) break;
-      if (wp.j < wp.count) {
-        if (wp.j == 0) {
+    } else {
+      const uint64_t dv = desc_mn(smem_u32(sV), kTileKeys * 128);
+      while (st.w < total) {
+        const int seen = st.seen16();
+        const bool last = st.j == st.count - 1;
+        ok = wait(&v_full[slot], ph);
+        if (ok && seen && st.j == 0) {
           // The previous item's O has been read out of the accumulator.
           ok = wait(&o_empty[i], oe_ph);
           oe_ph ^= 1u;
         }
-        ok = ok && wait(&p_full[2 * i], p_ph);
-        if (!ok) break;
-      }
-      // The issuers take turns, so that one row tile's MMAs run in one piece: interleaved, both row tiles' scores
-      // would come at the same time, and both softmaxes would run, and the tensor cores rest, at the same time.
-      ok = wait(&turn[i], t_ph);
-      if (!ok) break;
-      t_ph ^= 1u;
-      if (wp.j < wp.count) {
-        const int n16 = wp.seen16() >> 4;
-        const uint64_t b = dv + static_cast<uint64_t>(vs * (kKeyBytes<D> >> 4));
-        const uint32_t acc = wp.j > 0;
-        const bool last = wp.j == wp.count - 1;
-        constexpr uint32_t id = idesc_f16(kTileRows, D, kBf) | (1u << 16);
-        tc_fence_after();
-        if (elect_one()) {
+        if (seen) {
+          const uint32_t acc = st.j > 0;
+          constexpr uint32_t id = idesc_f16(kTileRows, D, kBf) | (1u << 16);
 #pragma unroll
-          for (int k = 0; k < 4; ++k)
-            if (k < n16) tc_mma_f16_ts(to, ts + 8 * k, b + 128 * k, id, k > 0 ? 1u : acc);
-        }
-        __syncwarp();
-        ok = wait(&p_full[2 * i + 1], p_ph);
-        if (!ok) break;
-        p_ph ^= 1u;
-        tc_fence_after();
-        if (elect_one()) {
+          for (int h = 0; h < 2; ++h) {
+            ok = ok && wait(&p_full[2 * i + h], t_ph);
+            if (!ok) break;
+            tc_fence_after();
+            const int n16 = (seen - h * kHalfKeys) >> 4;
+            const uint64_t b = dv + static_cast<uint64_t>(slot * (kKeyBytes<D> >> 4) + h * (kHalfKeys * 128 >> 4));
+            if (elect_one()) {
 #pragma unroll
-          for (int k = 4; k < 8; ++k)
-            if (k < n16) tc_mma_f16_ts(to, ts + 8 * k, b + 128 * k, id, 1u);
-          if (last) tc_commit(&o_full[i]);
-          tc_commit(&v_empty[vs]);
+              for (int k = 0; k < 4; ++k)
+                if (k < n16)
+                  tc_mma_f16_ts(to, ts + h * kHalfKeys + 8 * k, b + 128 * k, id, h > 0 || k > 0 ? 1u : acc);
+              tc_commit(&pv_done[2 * i + h]);
+              if (h == 1) {
+                tc_commit(&v_empty[slot]);
+                if (last) tc_commit(&o_full[i]);
+              }
+            }
+            __syncwarp();
+          }
+          t_ph ^= 1u;
+        } else if (ok && lane == 0) {
+          mbar_arrive(&v_empty[slot]);
         }
-      } else if (elect_one()) {
-        tc_commit(&v_empty[vs]);
+        if (!ok) break;
+        if (++slot == kSt) {
+          slot = 0;
+          ph ^= 1u;
+        }
+        st.next(p, total, i);
       }
-      __syncwarp();
-      if (++vs == kSt) {
-        vs = 0;
-        vph ^= 1u;
-      }
-      wp.next(p, total, i);
-      if (ws.w < total) ok = step_s();
-      if (lane == 0) mbar_arrive(&turn[i ^ 1]);
-      __syncwarp();
     }
     if (elect_one()) {
       if (!ok) {
@@ -448,14 +456,15 @@ __global__ void __launch_bounds__(kThreads, 1) attend_tiles_kernel(const __grid_
     const int i = warp >> 2;                       // row tile
     const int r = (warp & 3) * 32 + lane;          // row = TMEM lane
     const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
-    const uint32_t ts = tmem + lanes + i * 128, to = tmem + lanes + 256 + i * 128;
+    const uint32_t to = tmem + lanes + 256 + i * 128;
     const int my_tok = i * per + r / p.fold, my_head = r % p.fold;
     constexpr float kRescale = 8.f;  // P stays below 2^8
     constexpr float kNone = -1e30f;  // no key seen yet
     const uint64_t sl2 = f2_pack(p.scale_log2, p.scale_log2);
     Walk wk;
     wk.init(p, total);
-    uint32_t s_ph = 0, o_ph = 0;
+    uint32_t t_ph = 0;   // parity of the row tile's key tiles
+    uint32_t items = 0;  // items read out
     bool fail = false, fin = false, fin_live = false;
     float fin_l = 0.f, fin_m = 0.f;
     int fin_tok = 0, fin_head = 0, fin_part = 0;
@@ -482,8 +491,7 @@ __global__ void __launch_bounds__(kThreads, 1) attend_tiles_kernel(const __grid_
 #pragma unroll
       for (int c = 0; c < D / 32; ++c) {
         float t[32];
-        tmem_ld32(to + 32 * c, t);
-        tc_wait_ld();
+        tmem_read(to + 32 * c, t);
 #pragma unroll
         for (int e = 0; e < 32; ++e) t[e] = none ? 0.f : t[e] * inv;
         if (dst) {
@@ -503,87 +511,74 @@ __global__ void __launch_bounds__(kThreads, 1) attend_tiles_kernel(const __grid_
     while (!fail && wk.w < total) {
       const int n = i ? wk.count[1] : wk.count[0];
       float m = kNone, l = 0.f;
-      const int own = wk.it.diag + my_tok + 1;  // own keys that the row sees
-      for (int j = 0; j < n; ++j) {
-        const KeyTile t = key_tile<kTileKeys>(wk.it, j);
-        const int lim = min(t.valid, t.own ? own - t.base : t.valid);  // the row's visible keys: those below
-        const int n16 = wk.seen16(j, i);                             // columns that S has
-        fail = !__all_sync(0xffffffffu, mbar_wait(&s_full[i], s_ph, abort_flag));
-        if (fail) break;
-        s_ph ^= 1u;
-        tc_fence_after();
-        float s[4][32];
-        float mt;
-        if (__all_sync(0xffffffffu, lim >= kTileKeys)) {
-          // Every key is visible to every row of the warp.  Six chains of maxima; the second half's scores
-          // arrive while the first half's are compared.
-          tmem_ld32(ts, s[0]);
-          tmem_ld32(ts + 32, s[1]);
-          tc_wait_ld();
-          tmem_ld32(ts + 64, s[2]);
-          tmem_ld32(ts + 96, s[3]);
+      const int own = wk.it.diag + my_tok + 1 - wk.it.b0;  // own keys from b0 on that the row sees
+      for (int j = 0; !fail && j < n; ++j) {
+        const int seen = wk.seen16(j, i);
+        const int left = j < wk.na ? wk.it.a1 - wk.it.a0 - j * kTileKeys
+                                   : min(wk.it.b1 - wk.it.b0, own) - (j - wk.na) * kTileKeys;  // the row's keys
+#pragma unroll 1
+        for (int h = 0; h < 2; ++h) {
+          const int lim = left - h * kHalfKeys;  // the row sees the half's keys below
+          const uint32_t ts = tmem + lanes + i * 128 + h * kHalfKeys;
+          fail = !__all_sync(0xffffffffu, mbar_wait_spin(&s_full[2 * i + h], t_ph, abort_flag));
+          if (fail) break;
+          if (h * kHalfKeys >= seen) {  // no keys: nothing to read, nothing to multiply
+            if (lane == 0) mbar_arrive(&p_full[2 * i + h]);
+            continue;
+          }
+          tc_fence_after();
+          float s[64];
+          float mt;
+          tmem_read(ts, s);  // where S has fewer columns the rest is something else, and masked
+          if (!__all_sync(0xffffffffu, lim >= kHalfKeys)) {
+#pragma unroll
+            for (int c = 0; c < 2; ++c) {
+              const int k = lim - 32 * c;
+              const uint32_t vis = k <= 0 ? 0u : k >= 32 ? 0xffffffffu : (1u << k) - 1u;
+#pragma unroll
+              for (int e = 0; e < 32; ++e)
+                if (!((vis >> e) & 1u)) s[32 * c + e] = -INFINITY;
+            }
+          }
           float mx[6];
 #pragma unroll
-          for (int e = 0; e < 6; ++e) mx[e] = fmaxf(s[0][2 * e], s[0][2 * e + 1]);
+          for (int e = 0; e < 6; ++e) mx[e] = fmaxf(s[2 * e], s[2 * e + 1]);
 #pragma unroll
-          for (int e = 12; e < 64; e += 2) mx[e / 2 % 6] = fmax3(mx[e / 2 % 6], s[e >> 5][e & 31], s[e >> 5][(e & 31) + 1]);
-          tc_wait_ld();
-#pragma unroll
-          for (int e = 64; e < 128; e += 2) mx[e / 2 % 6] = fmax3(mx[e / 2 % 6], s[e >> 5][e & 31], s[e >> 5][(e & 31) + 1]);
+          for (int e = 12; e < 64; e += 2) mx[e / 2 % 6] = fmax3(mx[e / 2 % 6], s[e], s[e + 1]);
           mt = fmaxf(fmax3(mx[0], mx[1], mx[2]), fmax3(mx[3], mx[4], mx[5]));
-        } else {
+          mt *= p.scale_log2;
+          const bool need = m != kNone && mt > m + kRescale;
+          if (m == kNone) m = fmaxf(m, mt);
+          if (__any_sync(0xffffffffu, need)) {
+            // The P V before is done, and this half's has not been issued.
+            fail = !__all_sync(0xffffffffu, mbar_wait_spin(&pv_done[2 * i + (h ^ 1)], t_ph ^ (h ^ 1), abort_flag));
+            if (fail) break;
+            tc_fence_after();
+            const float alpha = need ? ex2_approx(m - mt) : 1.f;
 #pragma unroll
-          for (int c = 0; c < 4; ++c)
-            if (32 * c < n16) tmem_ld32(ts + 32 * c, s[c]);
-          tc_wait_ld();
-          mt = -INFINITY;
+            for (int c = 0; c < D / 16; ++c) {
+              float o[16];
+              tmem_read(to + 16 * c, o);
+              uint32_t w[16];
 #pragma unroll
-          for (int c = 0; c < 4; ++c) {
-            if (32 * c >= n16) continue;
-            const int k = lim - 32 * c;
-            const uint32_t vis = k <= 0 ? 0u : k >= 32 ? 0xffffffffu : (1u << k) - 1u;
-#pragma unroll
-            for (int e = 0; e < 32; ++e)
-              if (!((vis >> e) & 1u)) s[c][e] = -INFINITY;
-            float mx[4] = {fmax3(s[c][0], s[c][1], s[c][2]), fmax3(s[c][3], s[c][4], s[c][5]),
-                           fmax3(s[c][6], s[c][7], s[c][8]), fmax3(s[c][9], s[c][10], s[c][11])};
-#pragma unroll
-            for (int e = 12; e < 32; e += 2) mx[(e >> 1) & 3] = fmax3(mx[(e >> 1) & 3], s[c][e], s[c][e + 1]);
-            mt = fmaxf(mt, fmax3(mx[0], mx[1], fmaxf(mx[2], mx[3])));
+              for (int e = 0; e < 16; ++e) w[e] = __float_as_uint(o[e] * alpha);
+              tmem_st16(to + 16 * c, w);
+            }
+            tc_wait_st();
+            if (need) {
+              l *= alpha;
+              m = mt;
+            }
           }
-        }
-        mt *= p.scale_log2;
-        const bool need = m != kNone && mt > m + kRescale;
-        if (m == kNone) m = fmaxf(m, mt);
-        if (__any_sync(0xffffffffu, need)) {
-          // P V of the tile before is done (see above) and this tile's has not been issued.
-          const float alpha = need ? ex2_approx(m - mt) : 1.f;
+          const uint64_t nm2 = f2_pack(-m, -m);
+          uint64_t ps[2] = {0ull, 0ull};
 #pragma unroll
-          for (int c = 0; c < D / 16; ++c) {
-            float o[16];
-            tmem_ld16(to + 16 * c, o);
-            tc_wait_ld();
-            uint32_t w[16];
-#pragma unroll
-            for (int e = 0; e < 16; ++e) w[e] = __float_as_uint(o[e] * alpha);
-            tmem_st16(to + 16 * c, w);
-          }
-          tc_wait_st();
-          if (need) {
-            l *= alpha;
-            m = mt;
-          }
-        }
-        const uint64_t nm2 = f2_pack(-m, -m);
-        uint64_t ps[2] = {0ull, 0ull};
-#pragma unroll
-        for (int c = 0; c < 4; ++c) {
-          if (32 * c < n16) {
+          for (int c = 0; c < 2; ++c) {
             uint32_t w[16];
 #pragma unroll
             for (int e = 0; e < 16; ++e) {
               float x0, x1;
-              f2_unpack(f2_fma(f2_pack(s[c][2 * e], s[c][2 * e + 1]), sl2, nm2), x0, x1);
+              f2_unpack(f2_fma(f2_pack(s[32 * c + 2 * e], s[32 * c + 2 * e + 1]), sl2, nm2), x0, x1);
               const float p0 = ex2_approx(x0), p1 = ex2_approx(x1);
               ps[e & 1] = f2_add(ps[e & 1], f2_pack(p0, p1));
               auto v = Elem<T>::pack(p0, p1);
@@ -591,18 +586,23 @@ __global__ void __launch_bounds__(kThreads, 1) attend_tiles_kernel(const __grid_
             }
             tmem_st16(ts + 16 * c, w);
           }
-          if (c & 1) {
-            tc_wait_st();
-            tc_fence_before();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(&p_full[2 * i + (c >> 1)]);
+          tc_wait_st();
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&p_full[2 * i + h]);
+          float p0, p1, p2, p3;
+          f2_unpack(ps[0], p0, p1);
+          f2_unpack(ps[1], p2, p3);
+          l += (p0 + p1) + (p2 + p3);
+          if (fin) {
+            fail = !__all_sync(0xffffffffu, mbar_wait_spin(&o_full[i], items & 1, abort_flag));
+            if (fail) break;
+            ++items;
+            tc_fence_after();
+            read_out();
           }
         }
-        float p0, p1, p2, p3;
-        f2_unpack(ps[0], p0, p1);
-        f2_unpack(ps[1], p2, p3);
-        l += (p0 + p1) + (p2 + p3);
-        if (fin) read_out();  // S of this item means that the last item's P V are done
+        t_ph ^= 1u;
       }
       if (fail) break;
       if (n) {
@@ -613,12 +613,11 @@ __global__ void __launch_bounds__(kThreads, 1) attend_tiles_kernel(const __grid_
         fin_tok = wk.it.tok0 + my_tok;
         fin_head = wk.hg * p.fold + my_head;
         fin_part = wk.it.part;
-        o_ph ^= 1u;
       }
       wk.next(p, total);
     }
     if (!fail && fin) {
-      fail = !__all_sync(0xffffffffu, mbar_wait(&o_full[i], o_ph ^ 1u, abort_flag));
+      fail = !__all_sync(0xffffffffu, mbar_wait_spin(&o_full[i], items & 1, abort_flag));
       if (!fail) {
         tc_fence_after();
         read_out();
