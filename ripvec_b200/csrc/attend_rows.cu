@@ -64,6 +64,7 @@ template <typename T, int D>
 __global__ void __launch_bounds__(kThreads) attend_rows_kernel(const __grid_constant__ CUtensorMap mk,
                                                                const __grid_constant__ CUtensorMap mv,
                                                                const Rows q, const AttendParams p) {
+  launch_next();
   constexpr int kHalves = D / 64, kSteps = D / 16, kOut = D / 8;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* ring = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
@@ -269,7 +270,12 @@ __global__ void __launch_bounds__(kThreads) attend_rows_kernel(const __grid_cons
     }
   }
   __syncthreads();
-  if (warp == kWarps) return;
+  if (warp == kWarps) {
+    // This kernel may have started beside attend_tiles, of which it needs nothing; but what comes after it needs
+    // both, and waits for this one only: it does not end before the other has.
+    if (blockIdx.x == 0) wait_before();
+    return;
+  }
   const int rows = it.n * p.fold;
   for (int c = threadIdx.x; c < rows * (D / 8); c += 32 * kWarps) {
     const int r = c / (D / 8), d = c % (D / 8) * 8;
@@ -307,13 +313,15 @@ __global__ void __launch_bounds__(kThreads) attend_rows_kernel(const __grid_cons
 }
 
 template <typename T, int D>
-cudaError_t launch(const CUtensorMap& mk, const CUtensorMap& mv, const Rows& q, const AttendParams& p, cudaStream_t st) {
+cudaError_t launch(const CUtensorMap& mk, const CUtensorMap& mv, const Rows& q, const AttendParams& p, bool early,
+                   cudaStream_t st) {
   static_assert(kStages<D> * 2 * kTileBytes<D> >= (kWarps * kRowTile * (D + 4) + 2 * kWarps * kRowTile) * 4, "join area");
   static PerDeviceOnce once;
   const cudaError_t e = once.run([] {
     return cudaFuncSetAttribute(attend_rows_kernel<T, D>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemBytes<D>);
   });
   if (e != cudaSuccess) return e;
+  if (early) return launch_early(attend_rows_kernel<T, D>, p.n_items * p.groups, kThreads, kSmemBytes<D>, st, mk, mv, q, p);
   attend_rows_kernel<T, D><<<p.n_items * p.groups, kThreads, kSmemBytes<D>, st>>>(mk, mv, q, p);
   return cudaGetLastError();
 }
@@ -321,10 +329,11 @@ cudaError_t launch(const CUtensorMap& mk, const CUtensorMap& mv, const Rows& q, 
 }  // namespace
 
 cudaError_t attend_rows(Act act, int head_dim, const CUtensorMap& mk, const CUtensorMap& mv, const Rows& q,
-                        const AttendParams& p, cudaStream_t st) {
+                        const AttendParams& p, bool early, cudaStream_t st) {
   if (act == Act::kBf16)
-    return head_dim == 64 ? launch<__nv_bfloat16, 64>(mk, mv, q, p, st) : launch<__nv_bfloat16, 128>(mk, mv, q, p, st);
-  return head_dim == 64 ? launch<__half, 64>(mk, mv, q, p, st) : launch<__half, 128>(mk, mv, q, p, st);
+    return head_dim == 64 ? launch<__nv_bfloat16, 64>(mk, mv, q, p, early, st)
+                          : launch<__nv_bfloat16, 128>(mk, mv, q, p, early, st);
+  return head_dim == 64 ? launch<__half, 64>(mk, mv, q, p, early, st) : launch<__half, 128>(mk, mv, q, p, early, st);
 }
 
 }  // namespace rv

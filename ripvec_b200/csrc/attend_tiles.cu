@@ -156,6 +156,7 @@ __global__ void __launch_bounds__(kThreads, 1) attend_tiles_kernel(const __grid_
                                                                    const __grid_constant__ CUtensorMap mk,
                                                                    const __grid_constant__ CUtensorMap mv,
                                                                    const AttendParams p) {
+  launch_next();  // attend_rows may start on the SMs that this kernel leaves free
   constexpr int kHalves = D / 64;
   constexpr int kSt = kStages<D>;
   constexpr bool kBf = Elem<T>::kBf16;
@@ -637,7 +638,7 @@ __global__ void __launch_bounds__(kThreads, 1) attend_tiles_kernel(const __grid_
 
 template <typename T, int D>
 cudaError_t launch(const CUtensorMap& mq, const CUtensorMap& mk, const CUtensorMap& mv, const AttendParams& p,
-                   cudaStream_t st) {
+                   int ctas, cudaStream_t st) {
   static PerDeviceOnce once;
   const cudaError_t e = once.run([] {
     cudaFuncAttributes attr;
@@ -648,17 +649,18 @@ cudaError_t launch(const CUtensorMap& mq, const CUtensorMap& mk, const CUtensorM
   });
   if (e != cudaSuccess) return e;
   const int total = p.n_items * p.groups;
-  attend_tiles_kernel<T, D><<<std::min(total, device_sm_count()), kThreads, kSmemBytes<D>, st>>>(mq, mk, mv, p);
+  attend_tiles_kernel<T, D><<<std::min(total, ctas), kThreads, kSmemBytes<D>, st>>>(mq, mk, mv, p);
   return cudaGetLastError();
 }
 
 }  // namespace
 
 cudaError_t attend_tiles(Act act, int head_dim, const CUtensorMap& mq, const CUtensorMap& mk, const CUtensorMap& mv,
-                         const AttendParams& p, cudaStream_t st) {
+                         const AttendParams& p, int ctas, cudaStream_t st) {
   if (act == Act::kBf16)
-    return head_dim == 64 ? launch<__nv_bfloat16, 64>(mq, mk, mv, p, st) : launch<__nv_bfloat16, 128>(mq, mk, mv, p, st);
-  return head_dim == 64 ? launch<__half, 64>(mq, mk, mv, p, st) : launch<__half, 128>(mq, mk, mv, p, st);
+    return head_dim == 64 ? launch<__nv_bfloat16, 64>(mq, mk, mv, p, ctas, st)
+                          : launch<__nv_bfloat16, 128>(mq, mk, mv, p, ctas, st);
+  return head_dim == 64 ? launch<__half, 64>(mq, mk, mv, p, ctas, st) : launch<__half, 128>(mq, mk, mv, p, ctas, st);
 }
 
 }  // namespace rv

@@ -56,6 +56,7 @@ struct Schedule {
   std::vector<rv::StepParts> parts;  // by token
   std::vector<int> joined;
   int64_t n_parts = 0;
+  int tile_sms = 0;  // CTAs of the tensor-core kernel
 };
 
 }  // namespace
@@ -195,28 +196,38 @@ void cut(const rv::StepItem& it, int keys, int most, F&& emit) {
 // tile leaves the tensor cores waiting for its softmax; starting and writing a part takes about two tiles.
 double tile_cost(const rv::StepItem& it, int tiles, int per) { return (it.n > per ? 1.0 : 0.7) * tiles + 2.0; }
 
-// The longest time of any SM when parts of at most `most` tiles are dealt out, longest first, forwards and
-// backwards in turn, as the kernel walks them.
-double makespan(const std::vector<Job>& jobs, int most, int per, int groups, int sms) {
-  std::vector<std::pair<double, int>> cost;  // by part, `groups` times each
+// The longest time of any CTA, and all CTAs' together, when parts of at most `most` tiles are dealt out to `ctas`,
+// longest first, forwards and backwards in turn, as the kernel walks them.
+struct Span {
+  double longest, all;
+};
+Span makespan(const std::vector<Job>& jobs, int most, int per, int groups, int ctas) {
+  std::vector<double> cost;  // by part, for one of `groups`
   for (const Job& j : jobs)
     cut(j.it, rv::kTileKeys, most, [&](const rv::StepItem& x, int parts) {
-      cost.push_back({tile_cost(x, tiles_of(x, rv::kTileKeys), per) + (parts > 1 ? 1.0 : 0.0), groups});
+      cost.push_back(tile_cost(x, tiles_of(x, rv::kTileKeys), per) + (parts > 1 ? 1.0 : 0.0));
     });
-  std::sort(cost.begin(), cost.end(), [](const auto& a, const auto& b) { return a.first > b.first; });
-  std::vector<double> load(size_t(sms), 0.0);
+  std::sort(cost.begin(), cost.end(), [](double a, double b) { return a > b; });
+  std::vector<double> load(size_t(ctas), 0.0);
   int64_t w = 0;
-  for (const auto& c : cost)
-    for (int k = 0; k < c.second; ++k, ++w) {
-      const int64_t round = w / sms, at = w % sms;
-      load[size_t(round & 1 ? sms - 1 - at : at)] += c.first;
+  double all = 0;
+  for (const double c : cost)
+    for (int k = 0; k < groups; ++k, ++w) {
+      const int64_t round = w / ctas, at = w % ctas;
+      load[size_t(round & 1 ? ctas - 1 - at : at)] += c;
+      all += c;
     }
-  return *std::max_element(load.begin(), load.end());
+  return {*std::max_element(load.begin(), load.end()), all};
 }
 
-// Longest part, in key tiles, for the tensor-core kernel's jobs.  Cutting keys costs a partial result and its
-// join, so it is done only where it shortens the kernel: with few jobs that each walk many keys.
-int choose_tile_cut(const std::vector<Job>& jobs, int per, int groups, int sms) {
+// How the tensor-core kernel's jobs are cut (longest part, in key tiles) and how many CTAs it gets.  Cutting keys
+// costs a partial result and its join, so it is done only where it shortens the step: with few jobs that each walk
+// many keys.  `rows` is the few-row kernel's time, summed over SMs, in the same unit; it runs on the SMs that are
+// left, so the step takes as long as the longest CTA here, or as all the work spread over all SMs.
+struct TileCut {
+  int most, ctas;
+};
+TileCut choose_tile_cut(const std::vector<Job>& jobs, int per, int groups, double rows, int sms) {
   int64_t total = 0;
   int longest = 1;
   for (const Job& j : jobs) {
@@ -226,22 +237,28 @@ int choose_tile_cut(const std::vector<Job>& jobs, int per, int groups, int sms) 
   }
   total *= groups;
   // Enough work for every SM many times over, none of it long against an SM's share: leave it whole.
-  if (int64_t(longest) * sms * 4 <= total) return longest;
-  double best = makespan(jobs, longest, per, groups, sms);
-  int most = longest;
-  for (int k = 2; k <= 64; k += k < 12 ? 1 : k / 4) {
-    const int u = std::max(1, int((int64_t(longest) + k - 1) / k));
+  if (int64_t(longest) * sms * 4 <= total) return {longest, sms};
+  TileCut best{longest, sms};
+  double best_time = 1e300;
+  for (int k = 1; k <= 64; k += k < 12 ? 1 : k / 4) {
+    const int u = (longest + k - 1) / k;
     int64_t parts = 0;
     for (const Job& j : jobs) parts += (tiles_of(j.it, rv::kTileKeys) + u - 1) / u;
-    if (parts * groups > int64_t(sms) * 16) break;
-    const double t = makespan(jobs, u, per, groups, sms);
-    if (t < 0.95 * best) {
-      best = t;
-      most = u;
+    parts *= groups;
+    if (k > 1 && parts > int64_t(sms) * 16) break;
+    // As many CTAs as parts, or as a half or a third of them, which leave SMs for the other kernel.
+    for (int d = 1; d <= (rows > 0 ? 3 : 1); ++d) {
+      const int ctas = int(std::min<int64_t>(sms, (parts + d - 1) / d));
+      const Span m = makespan(jobs, u, per, groups, ctas);
+      const double t = std::max(m.longest, (m.all + rows) / sms);
+      if (t < 0.97 * best_time) {
+        best_time = t;
+        best = {u, ctas};
+      }
     }
     if (u == 1) break;
   }
-  return most;
+  return best;
 }
 
 // Longest part, in 64-key tiles, for the few-row kernel's jobs: about three parts for each of two CTAs an SM
@@ -257,7 +274,8 @@ int choose_row_cut(const std::vector<Job>& jobs, int groups, int sms) {
 // and its own keys in one item, without partial results.  Sequences of few rows share the prefix: the rows of
 // all of them are packed into row tiles that read each prefix key once, and their own keys are separate items.
 void schedule(const std::vector<StepSeq>& seqs, const std::vector<int>& group_first, int n_tokens, int fold,
-              int groups, int sms, Schedule* out) {
+              int groups, int head_dim,
+              int sms, Schedule* out) {
   const int per = rv::kTileRows / fold;
   std::vector<Job> rows, tiles;
   auto add = [&](bool to_rows, int tok0, int n, const StepSeq& s, bool prefix, bool own, int diag, bool packed) {
@@ -308,7 +326,15 @@ void schedule(const std::vector<StepSeq>& seqs, const std::vector<int>& group_fi
   // Parts: a token's partials are numbered through its items in order.
   out->parts.assign(size_t(n_tokens), {0, 0});
   const int row_cut = rows.empty() ? 1 : choose_row_cut(rows, groups, sms);
-  const int tile_cut = tiles.empty() ? 1 : choose_tile_cut(tiles, per, groups, sms);
+  TileCut tile_cut{1, 0};
+  if (!tiles.empty()) {
+    // The few-row kernel's time: its bytes at an SM's share of the memory bandwidth, 43 GB/s, against the 2.2 us (1.6
+    // at head dim 64) that 128 keys of two row tiles take.
+    double row_time = 0;
+    for (const Job& j : rows) row_time += tiles_of(j.it, rv::kRowKeys) * double(rv::kRowKeys * head_dim * 4) / 43e3;
+    tile_cut = choose_tile_cut(tiles, per, groups, row_time * groups / (head_dim == 64 ? 1.6 : 2.2), sms);
+  }
+  out->tile_sms = tile_cut.ctas;
   auto emit = [&](const std::vector<Job>& jobs, bool packed, int keys, int most, std::vector<rv::StepItem>* items) {
     for (const Job& j : jobs) {
       if (j.packed != packed) continue;
@@ -325,7 +351,7 @@ void schedule(const std::vector<StepSeq>& seqs, const std::vector<int>& group_fi
   // Prefixes first: their items cut through sequences, and a sequence's tokens must agree in what came before
   // the item of its own keys.
   for (const bool packed : {true, false}) {
-    emit(tiles, packed, rv::kTileKeys, tile_cut, &out->tile_items);
+    emit(tiles, packed, rv::kTileKeys, tile_cut.most, &out->tile_items);
     emit(rows, packed, rv::kRowKeys, row_cut, &out->row_items);
   }
   std::stable_sort(out->tile_items.begin(), out->tile_items.end(), [&](const rv::StepItem& a, const rv::StepItem& b) {
@@ -418,7 +444,7 @@ int plan(rv_step* s, int32_t n_seqs, const int32_t* q_lens, const int32_t* own_l
   sc.tile_items.clear();
   sc.joined.clear();
   sc.n_parts = 0;
-  schedule(s->seq, s->group_first, int(tokens), s->fold, s->q_heads / s->fold, rv::device_sm_count(), &sc);
+  schedule(s->seq, s->group_first, int(tokens), s->fold, s->q_heads / s->fold, s->head_dim, rv::device_sm_count(), &sc);
   if (sc.n_parts > INT_MAX ||
       (int64_t(sc.row_items.size()) + int64_t(sc.tile_items.size())) * (s->q_heads / s->fold) > INT_MAX)
     return fail(s, RV_E_INVALID, "the step is too large");
@@ -656,6 +682,7 @@ int rv_step_attend(rv_step* s, const rv_kv_cache* cache, const void* q, int64_t 
     a.n_row_items = s->n_row_items;
     a.n_tile_items = s->n_tile_items;
     a.n_joined = s->n_joined;
+    a.tile_sms = s->sched.tile_sms;
     a.n_tokens = s->n_tokens;
     a.fold = s->fold;
     a.part_o = s->work;

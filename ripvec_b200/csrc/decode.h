@@ -71,6 +71,7 @@ struct AttendArgs {
   const int* joined;           // tokens with a partial count other than 1
   const int* pages;
   int n_row_items, n_tile_items, n_joined;
+  int tile_sms;  // CTAs of attend_tiles at most
   int n_tokens, q_heads, kv_heads, head_dim, fold;
   Rows q;
   void* out;

@@ -1,5 +1,7 @@
 // Attention of a decoding step: the two kernels that compute partial or final rows, and the join of tokens
 // whose keys were split over several items.
+#include <type_traits>
+
 #include "step_attend.cuh"
 
 namespace rv {
@@ -10,31 +12,58 @@ namespace {
 // item sees no key: zeros and -inf.
 template <typename T, int D>
 __global__ void __launch_bounds__(128) join_kernel(const int* __restrict__ tokens, int n, const AttendParams p) {
-  constexpr int kPer = D / 32;
+  constexpr int kPer = D / 32;  // values a lane
+  using Vec = std::conditional_t<kPer == 4, float4, float2>;
   const int lane = threadIdx.x & 31;
   const int64_t w = int64_t(blockIdx.x) * 4 + (threadIdx.x >> 5);
   if (w >= int64_t(n) * p.q_heads) return;
   const int tok = tokens[w / p.q_heads], head = static_cast<int>(w % p.q_heads);
   const StepParts pt = p.parts[tok];
   const int64_t at = int64_t(pt.first) * p.q_heads + head;
-  float top = -INFINITY;
-  for (int i = lane; i < pt.count; i += 32) top = fmaxf(top, p.part_l[at + int64_t(i) * p.q_heads]);
+  wait_before();  // for the partials
+  // Up to 32 partials at a time: one lane weighs each, all lanes add them, four loads in flight.
+  float v[kPer] = {}, sum = 0.f, top = -INFINITY;
+  for (int i0 = 0; i0 < pt.count; i0 += 32) {
+    const float ls = i0 + lane < pt.count ? p.part_l[at + int64_t(i0 + lane) * p.q_heads] : -INFINITY;
+    float mx = ls;
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-  float v[kPer] = {}, sum = 0.f;
-  if (top != -INFINITY) {
-    for (int i = 0; i < pt.count; ++i) {
-      const int64_t k = at + int64_t(i) * p.q_heads;
-      const float f = ex2_approx(p.part_l[k] - top);
-      sum += f;
+    for (int o = 16; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+    const float now = fmaxf(top, mx);
+    if (now == -INFINITY) continue;
+    const float old = ex2_approx(top - now), f = ex2_approx(ls - now);
+    top = now;
+    sum *= old;
 #pragma unroll
-      for (int e = 0; e < kPer; ++e) v[e] += f * p.part_o[k * D + lane * kPer + e];
+    for (int e = 0; e < kPer; ++e) v[e] *= old;
+    const int m = min(32, pt.count - i0);
+    const Vec* src = reinterpret_cast<const Vec*>(p.part_o + (at + int64_t(i0) * p.q_heads) * D) + lane;
+    const int64_t step = int64_t(p.q_heads) * 32;  // in Vec
+    int i = 0;
+    auto add = [&](const Vec& x, int k) {
+      const float g = __shfl_sync(0xffffffffu, f, k);
+      sum += g;
+      const float* y = reinterpret_cast<const float*>(&x);
+#pragma unroll
+      for (int e = 0; e < kPer; ++e) v[e] += g * y[e];
+    };
+    for (; i + 4 <= m; i += 4) {
+      const Vec x0 = src[i * step], x1 = src[(i + 1) * step], x2 = src[(i + 2) * step], x3 = src[(i + 3) * step];
+      add(x0, i);
+      add(x1, i + 1);
+      add(x2, i + 2);
+      add(x3, i + 3);
     }
+    for (; i < m; ++i) add(src[i * step], i);
   }
-  const float inv = sum > 0.f ? 1.f / sum : sum == 0.f ? 0.f : sum;
+  const float inv = sum == 0.f ? 0.f : 1.f / sum;
   T* dst = static_cast<T*>(p.out) + tok * p.out_token + head * p.out_head + lane * kPer;
-#pragma unroll
-  for (int e = 0; e < kPer; ++e) dst[e] = Elem<T>::from_f(v[e] * inv);
+  if constexpr (kPer == 4) {
+    auto lo = Elem<T>::pack(v[0] * inv, v[1] * inv), hi = Elem<T>::pack(v[2] * inv, v[3] * inv);
+    *reinterpret_cast<uint2*>(dst) = make_uint2(*reinterpret_cast<uint32_t*>(&lo), *reinterpret_cast<uint32_t*>(&hi));
+  } else {
+    auto x = Elem<T>::pack(v[0] * inv, v[1] * inv);
+    *reinterpret_cast<uint32_t*>(dst) = *reinterpret_cast<uint32_t*>(&x);
+  }
   if (p.lse && lane == 0)
     p.lse[int64_t(tok) * p.q_heads + head] = sum == 0.f ? -INFINITY : (top + log2f(sum)) * 0.6931471805599453f;
 }
@@ -42,9 +71,8 @@ __global__ void __launch_bounds__(128) join_kernel(const int* __restrict__ token
 template <typename T>
 cudaError_t join(const AttendArgs& a, const AttendParams& p, cudaStream_t st) {
   const int blocks = static_cast<int>((int64_t(a.n_joined) * a.q_heads + 3) / 4);
-  if (a.head_dim == 64) join_kernel<T, 64><<<blocks, 128, 0, st>>>(a.joined, a.n_joined, p);
-  else join_kernel<T, 128><<<blocks, 128, 0, st>>>(a.joined, a.n_joined, p);
-  return cudaGetLastError();
+  return launch_early(a.head_dim == 64 ? join_kernel<T, 64> : join_kernel<T, 128>, blocks, 128, 0, st, a.joined,
+                      a.n_joined, p);
 }
 
 bool pool_map(CUtensorMap* m, const void* base, bool bf, const AttendArgs& a, int box) {
@@ -89,7 +117,7 @@ cudaError_t step_attend(Act act, const AttendArgs& a, cudaStream_t st) {
     if (!pool_map(&mk, a.pool.k, bf, a, p.box) || !pool_map(&mv, a.pool.v, bf, a, p.box) ||
         !make_tmap_16bit(&mq, a.q.p, bf, 3, dims, strides, box))
       return cudaErrorInvalidValue;
-    e = attend_tiles(act, a.head_dim, mq, mk, mv, p, st);
+    e = attend_tiles(act, a.head_dim, mq, mk, mv, p, a.tile_sms, st);
     if (e != cudaSuccess) return e;
   }
   if (a.n_row_items > 0) {
@@ -97,7 +125,7 @@ cudaError_t step_attend(Act act, const AttendArgs& a, cudaStream_t st) {
     p.n_items = a.n_row_items;
     p.box = a.pool.page_size < kRowKeys ? a.pool.page_size : kRowKeys;
     if (!pool_map(&mk, a.pool.k, bf, a, p.box) || !pool_map(&mv, a.pool.v, bf, a, p.box)) return cudaErrorInvalidValue;
-    e = attend_rows(act, a.head_dim, mk, mv, a.q, p, st);
+    e = attend_rows(act, a.head_dim, mk, mv, a.q, p, a.n_tile_items > 0, st);
     if (e != cudaSuccess) return e;
   }
   if (a.n_joined > 0) e = bf ? join<__nv_bfloat16>(a, p, st) : join<__half>(a, p, st);

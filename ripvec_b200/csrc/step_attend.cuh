@@ -1,6 +1,8 @@
 // Shared by the attention kernels of a decoding step.
 #pragma once
 
+#include <utility>
+
 #include "common.cuh"
 #include "decode.h"
 #include "tmap.h"
@@ -146,9 +148,29 @@ struct TileCopy {
   }
 };
 
+// Programmatic launch: a kernel launched so may start when every CTA of the kernel before it in the stream has
+// called launch_next() (or ended), and sees that kernel's results after wait_before().
+__device__ __forceinline__ void launch_next() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+__device__ __forceinline__ void wait_before() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+template <class... P, class... A>
+cudaError_t launch_early(void (*kernel)(P...), int grid, int block, int smem, cudaStream_t st, A&&... args) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(grid);
+  cfg.blockDim = dim3(block);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cudaLaunchAttribute at = {};
+  at.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at.val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = &at;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, kernel, std::forward<A>(args)...);
+}
+
+// early: attend_tiles was launched just before.
 cudaError_t attend_rows(Act act, int head_dim, const CUtensorMap& mk, const CUtensorMap& mv, const Rows& q,
-                        const AttendParams& p, cudaStream_t st);
+                        const AttendParams& p, bool early, cudaStream_t st);
 cudaError_t attend_tiles(Act act, int head_dim, const CUtensorMap& mq, const CUtensorMap& mk, const CUtensorMap& mv,
-                         const AttendParams& p, cudaStream_t st);
+                         const AttendParams& p, int ctas, cudaStream_t st);
 
 }  // namespace rv
