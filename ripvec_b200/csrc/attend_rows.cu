@@ -19,7 +19,7 @@ constexpr int kWarps = 4;
 constexpr int kThreads = 32 * (kWarps + 1);
 
 template <int D>
-constexpr int kStages = D == 128 ? 3 : 5;
+constexpr int kStages = D == 128 ? 2 : 3;
 template <int D>
 constexpr int kTileBytes = kRowKeys * D * 2;
 template <int D>
@@ -61,7 +61,7 @@ __device__ __forceinline__ uint32_t keep(uint32_t v, int k, int valid) {
 }
 
 template <typename T, int D>
-__global__ void __launch_bounds__(kThreads) attend_rows_kernel(const __grid_constant__ CUtensorMap mk,
+__global__ void __launch_bounds__(kThreads, D == 128 ? 3 : 4) attend_rows_kernel(const __grid_constant__ CUtensorMap mk,
                                                                const __grid_constant__ CUtensorMap mv,
                                                                const Rows q, const AttendParams p) {
   launch_next();
