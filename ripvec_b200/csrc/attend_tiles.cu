@@ -35,6 +35,7 @@ static_assert(2 * kSoftmaxRegs + 2 * kOtherRegs <= 4 * kLaunchRegs, "register sp
 constexpr int kTmemCols = 512;  // scores of row tile i at 128 i and 128 i + 64, O at 256 + 128 i
 constexpr int kHalfKeys = 64;
 
+constexpr int kStageBytes = 4096;  // of a softmax warp's output: 128 bytes of 32 rows
 template <int D>
 constexpr int kStages = D == 128 ? 2 : 4;  // of K and of V
 template <int D>
@@ -42,7 +43,7 @@ constexpr int kQBytes = kTileRows * D * 2;
 template <int D>
 constexpr int kKeyBytes = kTileKeys * D * 2;
 template <int D>
-constexpr int kSmemBytes = 1024 + 2 * kQBytes<D> + 2 * kStages<D> * kKeyBytes<D> + 512;
+constexpr int kSmemBytes = 1024 + 2 * kQBytes<D> + 2 * kStages<D> * kKeyBytes<D> + 8 * kStageBytes + 512;
 
 // MN-major operand of 64-value blocks with 128-byte swizzling: 8-row groups of 1024 bytes along K, blocks of
 // 64 values `block_bytes` apart along N.
@@ -165,7 +166,8 @@ __global__ void __launch_bounds__(kThreads, 1) attend_tiles_kernel(const __grid_
   uint8_t* sQ = smem;                            // [2]
   uint8_t* sK = sQ + 2 * kQBytes<D>;             // [kSt]
   uint8_t* sV = sK + kSt * kKeyBytes<D>;         // [kSt]
-  uint64_t* bar = reinterpret_cast<uint64_t*>(sV + kSt * kKeyBytes<D>);
+  uint8_t* sO = sV + kSt * kKeyBytes<D>;         // [8] outputs on their way out
+  uint64_t* bar = reinterpret_cast<uint64_t*>(sO + 8 * kStageBytes);
   uint64_t* q_full = bar;              // [2] Q of the row tile landed
   uint64_t* q_empty = q_full + 2;      // [2] its last S is done
   uint64_t* k_full = q_empty + 2;      // [kSt]
@@ -469,39 +471,65 @@ __global__ void __launch_bounds__(kThreads, 1) attend_tiles_kernel(const __grid_
     bool fail = false, fin = false, fin_live = false;
     float fin_l = 0.f, fin_m = 0.f;
     int fin_tok = 0, fin_head = 0, fin_part = 0;
-    // Writes the finished item's row: O / l from TMEM.
+    // Writes the finished item's rows: O / l from TMEM, by way of 4 KB of shared memory a warp, so that eight lanes
+    // write 128 consecutive bytes of a row (a lane a row, 16 bytes at a time, took 4 times as long).
+    uint8_t* stage = sO + warp * kStageBytes;
+    auto write_rows = [&](uint8_t* dst, int block) {
+      // dst: this lane's row, or null; row r of the staged 128 bytes at chunk c ^ (r & 7).
+      __syncwarp();
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        const int row = 4 * k + (lane >> 3), c = lane & 7;
+        uint8_t* d = reinterpret_cast<uint8_t*>(__shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(dst), row));
+        const uint4 x = *reinterpret_cast<const uint4*>(stage + row * 128 + ((c ^ (row & 7)) << 4));
+        if (d) *reinterpret_cast<uint4*>(d + block * 128 + c * 16) = x;
+      }
+      __syncwarp();
+    };
     auto read_out = [&]() {
       const bool none = fin_l == 0.f;  // the row saw no key
       const float inv = 1.f / fin_l;
-      StepParts pt{0, 1};
-      int64_t at = 0;
-      T* dst = nullptr;
-      float* part = nullptr;
+      uint8_t *dst = nullptr, *part = nullptr;
       if (fin_live) {
-        pt = p.parts[fin_tok];
+        const StepParts pt = p.parts[fin_tok];
         const float ls = none ? -INFINITY : fin_m + log2f(fin_l);
         if (pt.count == 1) {
-          dst = static_cast<T*>(p.out) + fin_tok * p.out_token + fin_head * p.out_head;
+          dst = reinterpret_cast<uint8_t*>(static_cast<T*>(p.out) + fin_tok * p.out_token + fin_head * p.out_head);
           if (p.lse) p.lse[int64_t(fin_tok) * p.q_heads + fin_head] = ls * 0.6931471805599453f;
         } else {
-          at = int64_t(pt.first + fin_part) * p.q_heads + fin_head;
-          part = p.part_o + at * D;
+          const int64_t at = int64_t(pt.first + fin_part) * p.q_heads + fin_head;
+          part = reinterpret_cast<uint8_t*>(p.part_o + at * D);
           p.part_l[at] = ls;
         }
       }
+      if (__any_sync(0xffffffffu, dst != nullptr)) {
 #pragma unroll
-      for (int c = 0; c < D / 32; ++c) {
-        float t[32];
-        tmem_read(to + 32 * c, t);
+        for (int b = 0; b < D / 64; ++b) {
 #pragma unroll
-        for (int e = 0; e < 32; ++e) t[e] = none ? 0.f : t[e] * inv;
-        if (dst) {
+          for (int c = 0; c < 2; ++c) {
+            float t[32];
+            tmem_read(to + 64 * b + 32 * c, t);
 #pragma unroll
-          for (int e = 0; e < 4; ++e) reinterpret_cast<uint4*>(dst + 32 * c)[e] = pack8<T>(t + 8 * e);
-        } else if (part) {
+            for (int e = 0; e < 32; ++e) t[e] = none ? 0.f : t[e] * inv;
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              *reinterpret_cast<uint4*>(stage + lane * 128 + (((4 * c + e) ^ (lane & 7)) << 4)) = pack8<T>(t + 8 * e);
+          }
+          write_rows(dst, b);
+        }
+      }
+      if (__any_sync(0xffffffffu, part != nullptr)) {
+#pragma unroll
+        for (int b = 0; b < D / 32; ++b) {
+          float t[32];
+          tmem_read(to + 32 * b, t);
+#pragma unroll
+          for (int e = 0; e < 32; ++e) t[e] = none ? 0.f : t[e] * inv;
 #pragma unroll
           for (int e = 0; e < 8; ++e)
-            reinterpret_cast<float4*>(part + 32 * c)[e] = make_float4(t[4 * e], t[4 * e + 1], t[4 * e + 2], t[4 * e + 3]);
+            *reinterpret_cast<float4*>(stage + lane * 128 + ((e ^ (lane & 7)) << 4)) =
+                make_float4(t[4 * e], t[4 * e + 1], t[4 * e + 2], t[4 * e + 3]);
+          write_rows(part, b);
         }
       }
       tc_fence_before();
