@@ -1,12 +1,13 @@
 // Attention of few query rows (decoding) over paged keys.
 //
-// One CTA per (item, group of `fold` query heads): at most 16 rows, the `fold` heads of each of the item's
-// tokens, against the item's keys.  A producer warp copies 64-key tiles of K and V by TMA, page by page, into
-// a ring of shared-memory stages; each of four warps takes 16 keys of every tile: S = Q K^T and O += P V by
-// mma.sync m16n8k16 with Q in registers, its own running maximum m and sum l, so that no warp waits for another
-// until the end, where the four are joined.  Every key is read once and used for 2 * 16 rows of products, far
-// below what the tensor cores need to be busy: the kernel is bound by HBM, and mma.sync keeps S and P in
-// registers, which a 128-row tcgen05 tile would not for 16 rows.
+// Work = (item, group of `fold` query heads): at most 16 rows, the `fold` heads of each of the item's tokens,
+// against the item's keys.  Persistent CTAs take work from a counter, so that they may come and go as another
+// kernel's CTAs leave the SMs.  A producer warp copies 64-key tiles of K and V by TMA, page by page, into a ring of
+// shared-memory stages and runs ahead into the next piece of work; each of four warps takes 16 keys of every tile:
+// S = Q K^T and O += P V by mma.sync m16n8k16 with Q in registers, its own running maximum m and sum l, so that no
+// warp waits for another until the end of the piece, where the four are joined.  Every key is read once and used
+// for 2 * 16 rows of products, far below what the tensor cores need to be busy: the kernel is bound by HBM, and
+// mma.sync keeps S and P in registers, which a 128-row tcgen05 tile would not for 16 rows.
 #include <algorithm>
 
 #include "step_attend.cuh"
@@ -21,9 +22,35 @@ constexpr int kThreads = 32 * (kWarps + 1);
 template <int D>
 constexpr int kStages = D == 128 ? 2 : 3;
 template <int D>
+constexpr int kPerSm = D == 128 ? 2 : 3;  // CTAs an SM holds
+template <int D>
 constexpr int kTileBytes = kRowKeys * D * 2;
 template <int D>
-constexpr int kSmemBytes = 1024 + kStages<D> * 2 * kTileBytes<D> + 256;
+constexpr int kJoinBytes = (kWarps * kRowTile * (D + 4) + 2 * kWarps * kRowTile) * 4;
+template <int D>
+constexpr int kQBytes = kRowTile * D * 2;
+// What the consumers need to know of a piece of work, beside its query rows.
+struct alignas(16) Piece {
+  StepItem it;
+  int w, pad[3];
+  StepParts parts[kRowTile];  // of its tokens
+};
+template <int D>
+constexpr int kSmemBytes = 1024 + kStages<D> * 2 * kTileBytes<D> + kJoinBytes<D> + 2 * kQBytes<D> + 2 * sizeof(Piece) + 256;
+
+// Barrier of the four consumer warps; true for all where one of them says so.
+__device__ __forceinline__ bool consumers_or(bool x) {
+  uint32_t r;
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\t"
+      "setp.ne.u32 p, %1, 0;\n\t"
+      "barrier.red.or.pred q, 1, 128, p;\n\t"
+      "selp.u32 %0, 1, 0, q;\n\t}\n"
+      : "=r"(r)
+      : "r"(static_cast<uint32_t>(x))
+      : "memory");
+  return r != 0;
+}
 
 __device__ __forceinline__ void ldmatrix4(uint32_t addr, uint32_t (&r)[4]) {
   asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
@@ -55,31 +82,47 @@ __device__ __forceinline__ uint32_t swizzled(uint32_t base, int row, int chunk) 
   return base + row * 128 + ((chunk ^ (row & 7)) << 4);
 }
 
+__device__ __forceinline__ void copy16_async(uint32_t dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
+// Arrives on *bar when this thread's copies so far have landed (counted among the barrier's arrivals).
+__device__ __forceinline__ void copies_arrive(uint64_t* bar) {
+  asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
+}
+
 // Keeps of a register that holds keys k and k + 1 (low and high half) those below `valid`.
 __device__ __forceinline__ uint32_t keep(uint32_t v, int k, int valid) {
   return v & ((k < valid ? 0xffffu : 0u) | (k + 1 < valid ? 0xffff0000u : 0u));
 }
 
 template <typename T, int D>
-__global__ void __launch_bounds__(kThreads, D == 128 ? 3 : 4) attend_rows_kernel(const __grid_constant__ CUtensorMap mk,
+__global__ void __launch_bounds__(kThreads, kPerSm<D>) attend_rows_kernel(const __grid_constant__ CUtensorMap mk,
                                                                const __grid_constant__ CUtensorMap mv,
                                                                const Rows q, const AttendParams p) {
   launch_next();
   constexpr int kHalves = D / 64, kSteps = D / 16, kOut = D / 8;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* ring = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  uint64_t* full = reinterpret_cast<uint64_t*>(ring + kStages<D> * 2 * kTileBytes<D>);
+  float* so = reinterpret_cast<float*>(ring + kStages<D> * 2 * kTileBytes<D>);  // [kWarps][16][D + 4]
+  float* sm = so + kWarps * kRowTile * (D + 4);                                 // [kWarps][16] m, then l
+  uint8_t* sq = reinterpret_cast<uint8_t*>(so) + kJoinBytes<D>;  // [2] query rows, 128-byte blocks swizzled like K
+  Piece* piece = reinterpret_cast<Piece*>(sq + 2 * kQBytes<D>);  // [2]
+  uint64_t* full = reinterpret_cast<uint64_t*>(piece + 2);
   uint64_t* empty = full + kStages<D>;
-  volatile int* abort_flag = reinterpret_cast<volatile int*>(empty + kStages<D>);
+  uint64_t* w_full = empty + kStages<D>;  // [2] a piece and its queries are there
+  uint64_t* w_empty = w_full + 2;         // [2] its place may be used again
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(w_empty + 2);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const StepItem it = p.items[blockIdx.x / p.groups];
-  const int hg = blockIdx.x % p.groups;
-  const int tiles = key_tiles<kRowKeys>(it);
+  const int total = p.n_items * p.groups;
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < kStages<D>; ++s) {
       mbar_init(&full[s], 1);
       mbar_init(&empty[s], kWarps);
+    }
+    for (int s = 0; s < 2; ++s) {
+      mbar_init(&w_full[s], 64);  // each producer lane's writes and copies
+      mbar_init(&w_empty[s], kWarps);
     }
     *abort_flag = 0;
     fence_mbar_init();
@@ -87,43 +130,86 @@ __global__ void __launch_bounds__(kThreads, D == 128 ? 3 : 4) attend_rows_kernel
   __syncthreads();
 
   bool failed = false;
-  float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
-  float o[kOut][4];
+  int s = 0;
+  uint32_t ph = 0;
   if (warp == kWarps) {
     if (lane == 0) {
       tma_prefetch_desc(&mk);
       tma_prefetch_desc(&mv);
     }
-    KeyTile t = key_tile<kRowKeys>(it, 0);
     // Lanes 0..15 copy K, lanes 16..31 V (a 64-key tile is at most 4 boxes of 2 halves).
     const int side = lane >> 4, l16 = lane & 15;
-    int page = TileCopy<kRowKeys, kHalves>::page_of(p, t, l16);
-    uint32_t issued = 0;
-    int s = 0;
-    uint32_t ph = 0;
-    for (int j = 0; j < tiles; ++j) {
-      KeyTile nt{};
-      int next_page = 0;
-      if (j + 1 < tiles) {
-        nt = key_tile<kRowKeys>(it, j + 1);
-        next_page = TileCopy<kRowKeys, kHalves>::page_of(p, nt, l16);
-      }
-      if (!__all_sync(0xffffffffu, mbar_wait(&empty[s], ph ^ 1u, abort_flag))) {
+    int issued = 0;
+    int w = lane == 0 ? atomicAdd(p.counter, 1) : 0;
+    w = __shfl_sync(0xffffffffu, w, 0);
+    StepItem it{};
+    if (w < total) it = p.items[w / p.groups];
+    for (int turn = 0;; ++turn) {
+      // Hand over the piece of work (or that there is none left), and ask for the next.
+      Piece& pc = piece[turn & 1];
+      if (!__all_sync(0xffffffffu, mbar_wait(&w_empty[turn & 1], ((turn >> 1) & 1) ^ 1u, abort_flag))) {
         failed = true;
         break;
       }
-      const int n = TileCopy<kRowKeys, kHalves>::copies(t, p.box);
-      if (lane == 0) mbar_arrive_expect_tx(&full[s], 2 * n * p.box * D * 2);
-      __syncwarp();
-      TileCopy<kRowKeys, kHalves>::issue(p, t, page, l16, ring + (2 * s + side) * kTileBytes<D>, side ? &mv : &mk,
-                                         &full[s], hg / p.per_kv);
-      issued = j + 1;
-      if (++s == kStages<D>) {
-        s = 0;
-        ph ^= 1u;
+      if (w >= total) {
+        if (lane == 0) pc.w = w;
+        mbar_arrive(&w_full[turn & 1]);
+        copies_arrive(&w_full[turn & 1]);
+        break;
       }
-      t = nt;
-      page = next_page;
+      const int next = lane == 0 ? atomicAdd(p.counter, 1) : 0;
+      const int hg = w % p.groups, rows = it.n * p.fold;
+      KeyTile t = key_tile<kRowKeys>(it, 0);
+      int page = TileCopy<kRowKeys, kHalves>::page_of(p, t, l16);
+      {
+        const uint32_t dst = smem_u32(sq + (turn & 1) * kQBytes<D>);
+        for (int c = lane; c < rows * (D / 8); c += 32) {
+          const int r = c / (D / 8), k = c % (D / 8);
+          const T* src = static_cast<const T*>(q.p) + (it.tok0 + r / p.fold) * q.token_stride +
+                         (hg * p.fold + r % p.fold) * q.head_stride + 8 * k;
+          copy16_async(swizzled(dst + (k >> 3) * (kRowTile * 128), r, k & 7), src);
+        }
+        if (lane < it.n) pc.parts[lane] = p.parts[it.tok0 + lane];
+        if (lane == 0) {
+          pc.it = it;
+          pc.w = w;
+        }
+        mbar_arrive(&w_full[turn & 1]);
+        copies_arrive(&w_full[turn & 1]);
+      }
+      const int tiles = key_tiles<kRowKeys>(it);
+      StepItem next_it{};
+      for (int j = 0; j < tiles; ++j) {
+        KeyTile nt{};
+        int next_page = 0;
+        if (j + 1 < tiles) {
+          nt = key_tile<kRowKeys>(it, j + 1);
+          next_page = TileCopy<kRowKeys, kHalves>::page_of(p, nt, l16);
+        }
+        if (!__all_sync(0xffffffffu, mbar_wait(&empty[s], ph ^ 1u, abort_flag))) {
+          failed = true;
+          break;
+        }
+        const int n = TileCopy<kRowKeys, kHalves>::copies(t, p.box);
+        if (lane == 0) mbar_arrive_expect_tx(&full[s], 2 * n * p.box * D * 2);
+        __syncwarp();
+        TileCopy<kRowKeys, kHalves>::issue(p, t, page, l16, ring + (2 * s + side) * kTileBytes<D>, side ? &mv : &mk,
+                                           &full[s], hg / p.per_kv);
+        ++issued;
+        if (++s == kStages<D>) {
+          s = 0;
+          ph ^= 1u;
+        }
+        if (j == 0) {
+          // The next piece's record is on its way while this one's keys are.
+          w = __shfl_sync(0xffffffffu, next, 0);
+          if (w < total) next_it = p.items[w / p.groups];
+        }
+        t = nt;
+        page = next_page;
+      }
+      if (failed) break;
+      it = next_it;
     }
     if (failed && lane == 0) {
       *abort_flag = 1;
@@ -131,34 +217,52 @@ __global__ void __launch_bounds__(kThreads, D == 128 ? 3 : 4) attend_rows_kernel
     }
     // Copies in flight land before the CTA may leave, also when it gave up.
     volatile int no_abort = 0;
-    const int from = static_cast<int>(issued) > kStages<D> ? static_cast<int>(issued) - kStages<D> : 0;
-    for (int j = from; j < static_cast<int>(issued); ++j) mbar_wait(&full[j % kStages<D>], (j / kStages<D>) & 1, &no_abort);
-  } else {
-    // Rows lane / 4 and lane / 4 + 8 of the 16: head row % fold of token row / fold.
+    for (int j = max(0, issued - kStages<D>); j < issued; ++j)
+      mbar_wait(&full[j % kStages<D>], (j / kStages<D>) & 1, &no_abort);
+    // The last CTA sets the counters back for the next launch.
+    if (lane == 0) {
+      __threadfence();
+      if (atomicAdd(p.counter + 1, 1) == static_cast<int>(gridDim.x) - 1) {
+        p.counter[0] = 0;
+        p.counter[1] = 0;
+      }
+    }
+    // This kernel may have started beside attend_tiles, of which it needs nothing; but what comes after it needs
+    // both, and waits for this one only: it does not end before the other has.
+    if (blockIdx.x == 0) wait_before();
+    return;
+  }
+  for (int turn = 0;; ++turn) {
+    failed = !__all_sync(0xffffffffu, mbar_wait_spin(&w_full[turn & 1], (turn >> 1) & 1, abort_flag));
+    const Piece& pc = piece[turn & 1];
+    const int w = failed ? total : pc.w;
+    if (consumers_or(failed) || w >= total) break;
+    const StepItem it = pc.it;
+    const int hg = w % p.groups, rows = it.n * p.fold;
+    const int tiles = key_tiles<kRowKeys>(it);
+    float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
+    float o[kOut][4];
+    // Rows lane / 4 and lane / 4 + 8 of the 16: head row % fold of token row / fold.  (Rows past the last are what
+    // an earlier piece left; nothing of theirs is written.)
     uint32_t a[kSteps][4];
     int lim[2];  // own keys that the row sees
-    const int rows = it.n * p.fold;
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      const int r = (lane >> 2) + 8 * i;
-      const int tok = min(r, rows - 1) / p.fold, head = hg * p.fold + min(r, rows - 1) % p.fold;
-      lim[i] = it.diag + tok + 1;
-      const T* qp = static_cast<const T*>(q.p) + (it.tok0 + tok) * q.token_stride + head * q.head_stride + (lane & 3) * 2;
+    for (int i = 0; i < 2; ++i) lim[i] = it.diag + ((lane >> 2) + 8 * i) / p.fold + 1;
+    {
+      const uint32_t base = smem_u32(sq + (turn & 1) * kQBytes<D>);
 #pragma unroll
       for (int k = 0; k < kSteps; ++k) {
-        a[k][i] = *reinterpret_cast<const uint32_t*>(qp + 16 * k);
-        a[k][i + 2] = *reinterpret_cast<const uint32_t*>(qp + 16 * k + 8);
+        const int chunk = 2 * k + (lane >> 4);
+        ldmatrix4(swizzled(base + (chunk >> 3) * (kRowTile * 128), lane & 15, chunk & 7), a[k]);
       }
     }
 #pragma unroll
     for (int n = 0; n < kOut; ++n)
 #pragma unroll
       for (int e = 0; e < 4; ++e) o[n][e] = 0.f;
-    int s = 0;
-    uint32_t ph = 0;
     for (int j = 0; j < tiles; ++j) {
       const KeyTile t = key_tile<kRowKeys>(it, j);
-      if (!__all_sync(0xffffffffu, mbar_wait(&full[s], ph, abort_flag))) {
+      if (!__all_sync(0xffffffffu, mbar_wait_spin(&full[s], ph, abort_flag))) {
         failed = true;
         break;
       }
@@ -249,80 +353,69 @@ __global__ void __launch_bounds__(kThreads, D == 128 ? 3 : 4) attend_rows_kernel
     for (int i = 0; i < 2; ++i) {
       l[i] += __shfl_xor_sync(0xffffffffu, l[i], 1);
       l[i] += __shfl_xor_sync(0xffffffffu, l[i], 2);
-    }
-  }
-  // Join the four warps through the ring, which every copy has landed in and every warp has read.
-  __syncthreads();
-  float* so = reinterpret_cast<float*>(ring);                       // [kWarps][16][D + 4]
-  float* sm = so + kWarps * kRowTile * (D + 4);                     // [kWarps][16] m, then l
-  if (warp < kWarps) {
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
       const int r = (lane >> 2) + 8 * i;
+      if (r < rows) {
 #pragma unroll
-      for (int n = 0; n < kOut; ++n)
-        *reinterpret_cast<float2*>(&so[(warp * kRowTile + r) * (D + 4) + 8 * n + 2 * (lane & 3)]) =
-            make_float2(o[n][2 * i], o[n][2 * i + 1]);
-      if ((lane & 3) == 0) {
-        sm[warp * kRowTile + r] = m[i];
-        sm[(kWarps + warp) * kRowTile + r] = l[i];
+        for (int n = 0; n < kOut; ++n)
+          *reinterpret_cast<float2*>(&so[(warp * kRowTile + r) * (D + 4) + 8 * n + 2 * (lane & 3)]) =
+              make_float2(o[n][2 * i], o[n][2 * i + 1]);
+        if ((lane & 3) == 0) {
+          sm[warp * kRowTile + r] = m[i];
+          sm[(kWarps + warp) * kRowTile + r] = l[i];
+        }
       }
     }
-  }
-  __syncthreads();
-  if (warp == kWarps) {
-    // This kernel may have started beside attend_tiles, of which it needs nothing; but what comes after it needs
-    // both, and waits for this one only: it does not end before the other has.
-    if (blockIdx.x == 0) wait_before();
-    return;
-  }
-  const int rows = it.n * p.fold;
-  for (int c = threadIdx.x; c < rows * (D / 8); c += 32 * kWarps) {
-    const int r = c / (D / 8), d = c % (D / 8) * 8;
-    float top = -INFINITY;
+    // Join the four warps.
+    if (consumers_or(failed)) break;
+    for (int c = threadIdx.x; c < rows * (D / 8); c += 32 * kWarps) {
+      const int r = c / (D / 8), d = c % (D / 8) * 8;
+      float top = -INFINITY;
 #pragma unroll
-    for (int w = 0; w < kWarps; ++w) top = fmaxf(top, sm[w * kRowTile + r]);
-    float sum = 0.f, v[8] = {};
-    if (top != -INFINITY) {
+      for (int w = 0; w < kWarps; ++w) top = fmaxf(top, sm[w * kRowTile + r]);
+      float sum = 0.f, v[8] = {};
+      if (top != -INFINITY) {
 #pragma unroll
-      for (int w = 0; w < kWarps; ++w) {
-        const float f = ex2_approx(sm[w * kRowTile + r] - top);
-        sum += f * sm[(kWarps + w) * kRowTile + r];
-        const float* src = &so[(w * kRowTile + r) * (D + 4) + d];
+        for (int w = 0; w < kWarps; ++w) {
+          const float f = ex2_approx(sm[w * kRowTile + r] - top);
+          sum += f * sm[(kWarps + w) * kRowTile + r];
+          const float* src = &so[(w * kRowTile + r) * (D + 4) + d];
 #pragma unroll
-        for (int e = 0; e < 8; ++e) v[e] += f * src[e];
+          for (int e = 0; e < 8; ++e) v[e] += f * src[e];
+        }
+        const float inv = 1.f / sum;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] *= inv;
       }
-      const float inv = 1.f / sum;
-#pragma unroll
-      for (int e = 0; e < 8; ++e) v[e] *= inv;
+      const float ls = top == -INFINITY ? -INFINITY : top + log2f(sum);
+      const int tok = it.tok0 + r / p.fold, head = hg * p.fold + r % p.fold;
+      const StepParts pt = pc.parts[r / p.fold];
+      if (pt.count == 1) {
+        *reinterpret_cast<uint4*>(static_cast<T*>(p.out) + tok * p.out_token + head * p.out_head + d) = pack8<T>(v);
+        if (p.lse && d == 0) p.lse[int64_t(tok) * p.q_heads + head] = ls * 0.6931471805599453f;
+      } else {
+        const int64_t at = int64_t(pt.first + it.part) * p.q_heads + head;
+        float4* dst = reinterpret_cast<float4*>(p.part_o + at * D + d);
+        dst[0] = make_float4(v[0], v[1], v[2], v[3]);
+        dst[1] = make_float4(v[4], v[5], v[6], v[7]);
+        if (d == 0) p.part_l[at] = ls;
+      }
     }
-    const float ls = top == -INFINITY ? -INFINITY : top + log2f(sum);
-    const int tok = it.tok0 + r / p.fold, head = hg * p.fold + r % p.fold;
-    const StepParts pt = p.parts[tok];
-    if (pt.count == 1) {
-      *reinterpret_cast<uint4*>(static_cast<T*>(p.out) + tok * p.out_token + head * p.out_head + d) = pack8<T>(v);
-      if (p.lse && d == 0) p.lse[int64_t(tok) * p.q_heads + head] = ls * 0.6931471805599453f;
-    } else {
-      const int64_t at = int64_t(pt.first + it.part) * p.q_heads + head;
-      float4* dst = reinterpret_cast<float4*>(p.part_o + at * D + d);
-      dst[0] = make_float4(v[0], v[1], v[2], v[3]);
-      dst[1] = make_float4(v[4], v[5], v[6], v[7]);
-      if (d == 0) p.part_l[at] = ls;
-    }
+    consumers_or(false);  // read before the next piece's results are written, and this piece's place is used again
+    if (lane == 0) mbar_arrive(&w_empty[turn & 1]);
   }
 }
 
 template <typename T, int D>
 cudaError_t launch(const CUtensorMap& mk, const CUtensorMap& mv, const Rows& q, const AttendParams& p, bool early,
                    cudaStream_t st) {
-  static_assert(kStages<D> * 2 * kTileBytes<D> >= (kWarps * kRowTile * (D + 4) + 2 * kWarps * kRowTile) * 4, "join area");
   static PerDeviceOnce once;
   const cudaError_t e = once.run([] {
     return cudaFuncSetAttribute(attend_rows_kernel<T, D>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemBytes<D>);
   });
   if (e != cudaSuccess) return e;
-  if (early) return launch_early(attend_rows_kernel<T, D>, p.n_items * p.groups, kThreads, kSmemBytes<D>, st, mk, mv, q, p);
-  attend_rows_kernel<T, D><<<p.n_items * p.groups, kThreads, kSmemBytes<D>, st>>>(mk, mv, q, p);
+  const int grid = std::min(p.n_items * p.groups, kPerSm<D> * device_sm_count());
+  if (early) return launch_early(attend_rows_kernel<T, D>, grid, kThreads, kSmemBytes<D>, st, mk, mv, q, p);
+  attend_rows_kernel<T, D><<<grid, kThreads, kSmemBytes<D>, st>>>(mk, mv, q, p);
   return cudaGetLastError();
 }
 

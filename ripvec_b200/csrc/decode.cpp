@@ -84,6 +84,7 @@ struct rv_step {
   int64_t n_parts = 0;
   unsigned int* err_host = nullptr;  // error word in mapped host memory: kernels write it, calls look at it
   unsigned int* err_dev = nullptr;
+  int* counter = nullptr;
   Staging staging[2];
   int turn = 0;
   // host side of the plan, kept for its memory
@@ -179,7 +180,8 @@ int tiles_of(const rv::StepItem& it, int keys) {
 template <class F>
 void cut(const rv::StepItem& it, int keys, int most, F&& emit) {
   const int na = (it.a1 - it.a0 + keys - 1) / keys, n = tiles_of(it, keys);
-  const int parts = std::max(1, (n + most - 1) / most);
+  // Up to 4 tiles of 64 keys are not worth a join of their own.
+  const int parts = keys == rv::kRowKeys && n <= 4 ? 1 : std::max(1, (n + most - 1) / most);
   for (int k = 0; k < parts; ++k) {
     const int lo = int(int64_t(n) * k / parts), hi = int(int64_t(n) * (k + 1) / parts);
     rv::StepItem x = it;
@@ -261,13 +263,13 @@ TileCut choose_tile_cut(const std::vector<Job>& jobs, int per, int groups, doubl
   return best;
 }
 
-// Longest part, in 64-key tiles, for the few-row kernel's jobs: about three parts for each of two CTAs an SM
-// where there is that much work, and at least 4 tiles, below which starting a CTA costs more than its keys.
+// Longest part, in 64-key tiles, for the few-row kernel's jobs: where there is much work, about three parts for each
+// of two CTAs an SM, which take them as they come; where there is little, short parts, so that all SMs have one.
 int choose_row_cut(const std::vector<Job>& jobs, int groups, int sms) {
   int64_t total = 0;
   for (const Job& j : jobs) total += tiles_of(j.it, rv::kRowKeys);
   total *= groups;
-  return int(std::max<int64_t>(4, (total + 6 * sms - 1) / (6 * sms)));
+  return int(std::max<int64_t>(2, (total + 6 * sms - 1) / (6 * sms)));
 }
 
 // Divides a step's attention into items.  A sequence whose rows fill a row tile by themselves walks the prefix
@@ -552,6 +554,8 @@ int rv_step_create(int device, int32_t q_heads, int32_t kv_heads, int32_t head_d
   ok = ok && cudaHostAlloc(reinterpret_cast<void**>(&s->err_host), sizeof(unsigned int), cudaHostAllocMapped) == cudaSuccess;
   if (ok) *s->err_host = 0;
   ok = ok && cudaHostGetDevicePointer(reinterpret_cast<void**>(&s->err_dev), s->err_host, 0) == cudaSuccess;
+  ok = ok && cudaMalloc(reinterpret_cast<void**>(&s->counter), 2 * sizeof(int)) == cudaSuccess &&
+       cudaMemset(s->counter, 0, 2 * sizeof(int)) == cudaSuccess;
   if (!ok) {
     cudaGetLastError();
     rv_step_destroy(s);
@@ -575,6 +579,7 @@ void rv_step_destroy(rv_step* s) {
     }
     if (s->meta) cudaFree(s->meta);
     if (s->work) cudaFree(s->work);
+    if (s->counter) cudaFree(s->counter);
     if (s->err_host) cudaFreeHost(s->err_host);
     if (s->last) cudaEventDestroy(s->last);
   }
@@ -689,6 +694,7 @@ int rv_step_attend(rv_step* s, const rv_kv_cache* cache, const void* q, int64_t 
     a.part_l = s->work + s->n_parts * s->q_heads * s->head_dim;
     a.num_pages = cache->num_pages;
     a.err = s->err_dev;
+    a.counter = s->counter;
     a.q_heads = s->q_heads;
     a.kv_heads = s->kv_heads;
     a.head_dim = s->head_dim;

@@ -83,6 +83,7 @@ struct AttendArgs {
   int64_t num_pages;
   float scale;
   unsigned int* err;  // error word that the host reads
+  int* counter;       // [2] zeros, left as zeros
 };
 cudaError_t step_attend(Act act, const AttendArgs& a, cudaStream_t st);
 

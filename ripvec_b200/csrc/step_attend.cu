@@ -105,6 +105,7 @@ cudaError_t step_attend(Act act, const AttendArgs& a, cudaStream_t st) {
   p.part_l = a.part_l;
   p.scale_log2 = a.scale * 1.4426950408889634f;
   p.err = a.err;
+  p.counter = a.counter;
   CUtensorMap mk, mv, mq;
   cudaError_t e = cudaSuccess;
   if (a.n_tile_items > 0) {

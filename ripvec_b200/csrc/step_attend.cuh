@@ -23,6 +23,7 @@ struct AttendParams {
   float *lse, *part_o, *part_l;
   float scale_log2;
   unsigned int* err;
+  int* counter;  // [2] of the few-row kernel: work taken, CTAs done; 0 between launches
 };
 
 __device__ __forceinline__ float ex2_approx(float x) {
