@@ -269,7 +269,9 @@ __global__ void __launch_bounds__(kThreads, kPerSm<D>) attend_rows_kernel(const 
       const int k0 = 16 * warp;
       if (k0 < t.valid) {
         const uint32_t kb = smem_u32(ring + 2 * s * kTileBytes<D>), vb = kb + kTileBytes<D>;
-        float x[2][4] = {};
+        // Two chains of sums a block, over every other step of 16 values: the products of one chain wait for one
+        // another.
+        float x[2][4] = {}, y[2][4] = {};
 #pragma unroll
         for (int k = 0; k < kSteps; k += 2) {
 #pragma unroll
@@ -279,9 +281,13 @@ __global__ void __launch_bounds__(kThreads, kPerSm<D>) attend_rows_kernel(const 
             const int row = k0 + 8 * n + (lane & 7), chunk = 2 * k + (lane >> 3);
             ldmatrix4(swizzled(kb + (chunk >> 3) * (kRowKeys * 128), row, chunk & 7), b);
             mma16816<T>(x[n], a[k], b[0], b[1]);
-            mma16816<T>(x[n], a[k + 1], b[2], b[3]);
+            mma16816<T>(y[n], a[k + 1], b[2], b[3]);
           }
         }
+#pragma unroll
+        for (int n = 0; n < 2; ++n)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) x[n][e] += y[n][e];
         // Score e of block n: row lane / 4 (+ 8 for e >= 2), key k0 + 8 n + 2 (lane % 4) + (e & 1).
         uint32_t w[4];
 #pragma unroll
