@@ -79,11 +79,6 @@ struct TEpiResidualStats {
   }
 };
 
-__device__ __forceinline__ uint64_t f2_mul(uint64_t a, uint64_t b) {
-  uint64_t r;
-  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-  return r;
-}
 
 // Folded LayerNorm of four values, two per instruction: rstd * (v - mu * c) evaluated as
 // v * rstd + (-rstd * mu) * c (r2 = {rstd, rstd}, nm2 = {-rstd * mu, -rstd * mu}).

@@ -15,53 +15,60 @@ namespace {
 constexpr float kE4m3Max = 448.f;
 constexpr float kScaleFloor = 1e-12f;  // of a group whose values are all zero: codes 0, scale 1e-12 / 448
 
-// Sum and maximum over the block.  The caller alternates between two `sh` arrays, so that one barrier a call
-// is enough.
-__device__ __forceinline__ float block_sum(float v, float* sh) {
+// Sum and maximum over the block's up to 16 warps.  The caller alternates between two `sh` arrays, so that one
+// barrier a call is enough.
+template <class F>
+__device__ __forceinline__ float block_reduce(float v, float* sh, float none, F&& f) {
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-  if ((threadIdx.x & 31) == 0) sh[threadIdx.x >> 5] = v;
+  for (int o = 16; o > 0; o >>= 1) v = f(v, __shfl_xor_sync(0xffffffffu, v, o));
+  const int lane = threadIdx.x & 31;
+  if (lane == 0) sh[threadIdx.x >> 5] = v;
   __syncthreads();
-  float s = 0.f;
-  for (int w = 0; w < (blockDim.x >> 5); ++w) s += sh[w];
-  return s;
+  v = lane < (blockDim.x >> 5) ? sh[lane] : none;
+#pragma unroll
+  for (int o = 8; o > 0; o >>= 1) v = f(v, __shfl_xor_sync(0xffffffffu, v, o));
+  return __shfl_sync(0xffffffffu, v, 0);
+}
+__device__ __forceinline__ float block_sum(float v, float* sh) {
+  return block_reduce(v, sh, 0.f, [](float a, float b) { return a + b; });
 }
 __device__ __forceinline__ float block_max(float v, float* sh) {
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, o));
-  if ((threadIdx.x & 31) == 0) sh[threadIdx.x >> 5] = v;
-  __syncthreads();
-  float s = 0.f;
-  for (int w = 0; w < (blockDim.x >> 5); ++w) s = fmaxf(s, sh[w]);
-  return s;
+  return block_reduce(v, sh, 0.f, [](float a, float b) { return fmaxf(a, b); });
 }
 
 // kVec consecutive 16-bit values, as loaded and as f32.
 template <typename T, int kVec>
 using Raw = std::conditional_t<kVec == 8, uint4, T>;
 template <typename T, int kVec>
-__device__ __forceinline__ void widen(const Raw<T, kVec>& r, float (&v)[kVec]) {
+__device__ __forceinline__ void widen(const Raw<T, kVec>& r, float* v) {
   if constexpr (kVec == 8) unpack8<T>(r, v);
   else v[0] = Elem<T>::to_f(r);
 }
-template <typename T, int kVec>
-__device__ __forceinline__ void store_vec(T* p, const float (&v)[kVec]) {
-  if constexpr (kVec == 8) *reinterpret_cast<uint4*>(p) = pack8<T>(v);
-  else *p = Elem<T>::from_f(v[0]);
+template <typename T, int kVec, int kPairs>
+__device__ __forceinline__ void store_vec(T* p, const uint64_t (&v)[kPairs]) {
+  float f[2 * kPairs];
+#pragma unroll
+  for (int e = 0; e < kPairs; ++e) f2_unpack(v[e], f[2 * e], f[2 * e + 1]);
+  if constexpr (kVec == 8) *reinterpret_cast<uint4*>(p) = pack8<T>(f);
+  else *p = Elem<T>::from_f(f[0]);
 }
-template <int kVec>
-__device__ __forceinline__ void store_codes(uint8_t* p, const float (&v)[kVec], float mul) {
+template <int kVec, int kPairs>
+__device__ __forceinline__ void store_codes(uint8_t* p, const uint64_t (&v)[kPairs], float mul) {
+  const uint64_t mul2 = f2_pack(mul, mul);
+  float f[2 * kPairs];
+#pragma unroll
+  for (int e = 0; e < kPairs; ++e) f2_unpack(f2_mul(v[e], mul2), f[2 * e], f[2 * e + 1]);
   if constexpr (kVec == 8) {
     uint32_t w[2];
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
-      const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(v[4 * i] * mul, v[4 * i + 1] * mul), __NV_SATFINITE, __NV_E4M3);
-      const uint32_t hi = __nv_cvt_float2_to_fp8x2(make_float2(v[4 * i + 2] * mul, v[4 * i + 3] * mul), __NV_SATFINITE, __NV_E4M3);
+      const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(f[4 * i], f[4 * i + 1]), __NV_SATFINITE, __NV_E4M3);
+      const uint32_t hi = __nv_cvt_float2_to_fp8x2(make_float2(f[4 * i + 2], f[4 * i + 3]), __NV_SATFINITE, __NV_E4M3);
       w[i] = lo | (hi << 16);
     }
     *reinterpret_cast<uint2*>(p) = make_uint2(w[0], w[1]);
   } else {
-    *p = __nv_cvt_float_to_fp8(v[0] * mul, __NV_SATFINITE, __NV_E4M3);
+    *p = __nv_cvt_float_to_fp8(f[0], __NV_SATFINITE, __NV_E4M3);
   }
 }
 
@@ -71,111 +78,120 @@ __device__ __forceinline__ void store_codes(uint8_t* p, const float (&v)[kVec], 
 // Threads of a CTA at most, and threads that an SM holds, by the registers that the row, its weights and the
 // next row take.
 template <int kVec, int kN>
-constexpr int kMaxThreads = kVec * kN >= 32 ? 512 : kVec * kN >= 16 ? 384 : 256;
+constexpr int kMaxThreads = kVec == 1 || kN == 4 ? 512 : kN == 2 ? 384 : 256;
 template <int kVec, int kN>
-constexpr int kResident = kVec * kN >= 32 ? 512 : kN >= 16 ? 384 : kVec * kN >= 16 ? 768 : 1024;
+constexpr int kResident = kVec == 1 ? (kN == 16 ? 512 : 1024) : kN == 4 ? 512 : kN == 2 ? 768 : 1024;
 
 template <typename T, int kVec, int kN, bool kCodes>
-__global__ void __launch_bounds__(kMaxThreads<kVec, kN>, kResident<kVec, kN> / kMaxThreads<kVec, kN>) rms_norm_kernel(const NormArgs a) {
+__global__ void __launch_bounds__(kMaxThreads<kVec, kN>, kResident<kVec, kN> / kMaxThreads<kVec, kN>)
+    rms_norm_kernel(const NormArgs a) {
   __shared__ float sh[4][16];
-  float w[kN][kVec];
+  // Values in pairs (a lone value has a zero beside it): one instruction works on both.
+  constexpr int kPairs = (kVec + 1) / 2;
+  using R = Raw<T, kVec>;
+  uint64_t w[kN][kPairs];
+  bool in[kN];
 #pragma unroll
   for (int n = 0; n < kN; ++n) {
     const int i = (n * blockDim.x + threadIdx.x) * kVec;
+    in[n] = i < a.hidden;
 #pragma unroll
-    for (int e = 0; e < kVec; ++e) w[n][e] = i < a.hidden ? a.weight[i + e] : 0.f;
+    for (int e = 0; e < kPairs; ++e)
+      w[n][e] = f2_pack(in[n] ? a.weight[i + 2 * e] : 0.f, in[n] && kVec > 1 ? a.weight[i + 2 * e + 1] : 0.f);
   }
-  using R = Raw<T, kVec>;
+  const float inv_hidden = 1.f / a.hidden;
+  const int64_t at = int64_t(threadIdx.x) * kVec;
+  const int step = blockDim.x * kVec;  // between a thread's vectors
+  const T* x = static_cast<const T*>(a.x) + blockIdx.x * a.x_stride + at;
+  const T* r = static_cast<const T*>(a.residual) + blockIdx.x * a.residual_stride + at;
+  T* ro = static_cast<T*>(a.residual_out) + blockIdx.x * a.residual_out_stride + at;
   R rx[kN], rr[kN];  // the next row, loaded while the present one is worked on
-  auto load = [&](int64_t row) {
-    const T* x = static_cast<const T*>(a.x) + row * a.x_stride;
-    const T* r = static_cast<const T*>(a.residual) + row * a.residual_stride;
+  auto load = [&]() {
 #pragma unroll
-    for (int n = 0; n < kN; ++n) {
-      const int i = (n * blockDim.x + threadIdx.x) * kVec;
-      if (i < a.hidden) rx[n] = *reinterpret_cast<const R*>(x + i);
-    }
+    for (int n = 0; n < kN; ++n)
+      if (in[n]) rx[n] = *reinterpret_cast<const R*>(x + n * step);
     if (a.residual) {
 #pragma unroll
-      for (int n = 0; n < kN; ++n) {
-        const int i = (n * blockDim.x + threadIdx.x) * kVec;
-        if (i < a.hidden) rr[n] = *reinterpret_cast<const R*>(r + i);
-      }
+      for (int n = 0; n < kN; ++n)
+        if (in[n]) rr[n] = *reinterpret_cast<const R*>(r + n * step);
     }
+    x += gridDim.x * a.x_stride;
+    r += gridDim.x * a.residual_stride;
   };
   int turn = 0;
-  if (blockIdx.x < a.rows) load(blockIdx.x);
+  if (blockIdx.x < a.rows) load();
   for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x, turn ^= 1) {
-    float h[kN][kVec];
-    float ss = 0.f;
+    uint64_t h[kN][kPairs];
+    uint64_t ss = 0;
 #pragma unroll
     for (int n = 0; n < kN; ++n) {
-      const int i = (n * blockDim.x + threadIdx.x) * kVec;
-      if (i < a.hidden) {
-        widen<T, kVec>(rx[n], h[n]);
-        if (a.residual) {
-          float y[kVec];
-          widen<T, kVec>(rr[n], y);
+      float v[2 * kPairs] = {};
+      if (in[n]) widen<T, kVec>(rx[n], v);
 #pragma unroll
-          for (int e = 0; e < kVec; ++e) h[n][e] += y[e];
-        }
-      } else {
+      for (int e = 0; e < kPairs; ++e) h[n][e] = f2_pack(v[2 * e], v[2 * e + 1]);
+      if (a.residual) {
+        if (in[n]) widen<T, kVec>(rr[n], v);
 #pragma unroll
-        for (int e = 0; e < kVec; ++e) h[n][e] = 0.f;
+        for (int e = 0; e < kPairs; ++e) h[n][e] = f2_add(h[n][e], f2_pack(v[2 * e], v[2 * e + 1]));
       }
     }
-    if (row + gridDim.x < a.rows) load(row + gridDim.x);
-    T* ro = static_cast<T*>(a.residual_out) + row * a.residual_out_stride;
+    if (row + gridDim.x < a.rows) load();
 #pragma unroll
     for (int n = 0; n < kN; ++n) {
-      const int i = (n * blockDim.x + threadIdx.x) * kVec;
-      if (a.residual_out && i < a.hidden) store_vec<T, kVec>(ro + i, h[n]);
+      if (a.residual_out && in[n]) store_vec<T, kVec>(ro + n * step, h[n]);
 #pragma unroll
-      for (int e = 0; e < kVec; ++e) ss += h[n][e] * h[n][e];
+      for (int e = 0; e < kPairs; ++e) ss = f2_fma(h[n][e], h[n][e], ss);
     }
-    const float inv = rsqrtf(block_sum(ss, sh[turn]) / a.hidden + a.eps);
+    ro += gridDim.x * a.residual_out_stride;
+    float s0, s1;
+    f2_unpack(ss, s0, s1);
+    const float inv = rsqrtf(block_sum(s0 + s1, sh[turn]) * inv_hidden + a.eps);
+    const uint64_t inv2 = f2_pack(inv, inv);
 #pragma unroll
     for (int n = 0; n < kN; ++n)
 #pragma unroll
-      for (int e = 0; e < kVec; ++e) h[n][e] = h[n][e] * inv * w[n][e];
+      for (int e = 0; e < kPairs; ++e) h[n][e] = f2_mul(f2_mul(h[n][e], inv2), w[n][e]);
     if constexpr (!kCodes) {
-      T* o = static_cast<T*>(a.out) + row * a.out_stride;
+      T* o = static_cast<T*>(a.out) + row * a.out_stride + at;
 #pragma unroll
-      for (int n = 0; n < kN; ++n) {
-        const int i = (n * blockDim.x + threadIdx.x) * kVec;
-        if (i < a.hidden) store_vec<T, kVec>(o + i, h[n]);
-      }
+      for (int n = 0; n < kN; ++n)
+        if (in[n]) store_vec<T, kVec>(o + n * step, h[n]);
     } else {
-      uint8_t* o = static_cast<uint8_t*>(a.out) + row * a.out_stride;
+      uint8_t* o = static_cast<uint8_t*>(a.out) + row * a.out_stride + at;
       float mx[kN], all = 0.f;
 #pragma unroll
       for (int n = 0; n < kN; ++n) {
         mx[n] = 0.f;
 #pragma unroll
-        for (int e = 0; e < kVec; ++e) mx[n] = fmaxf(mx[n], fabsf(h[n][e]));
+        for (int e = 0; e < kPairs; ++e) {
+          f2_unpack(h[n][e], s0, s1);
+          mx[n] = fmax3(mx[n], fabsf(s0), fabsf(s1));
+        }
         all = fmaxf(all, mx[n]);
       }
       if (a.group == a.hidden) {
         const float top = fmaxf(block_max(all, sh[2 + turn]), kScaleFloor);
-        if (threadIdx.x == 0) a.scales[row] = top / kE4m3Max;
+        if (threadIdx.x == 0) a.scales[row] = top * (1.f / kE4m3Max);
 #pragma unroll
         for (int n = 0; n < kN; ++n) mx[n] = top;
       } else {
-        // A group of 32 .. 256 values is 4 .. 32 neighbouring lanes of one vector step (kVec 8).
-        const int lanes = a.group / kVec;
+        // A group of 32, 64, 128 or 256 values is 4 to 32 neighbouring lanes of one vector step (kVec 8).
+        const int lanes = a.group / kVec, shift = 31 - __clz(a.group);
+        float* sc = a.scales + row * (a.hidden >> shift) + (at >> shift);
 #pragma unroll
         for (int n = 0; n < kN; ++n) {
-          for (int off = 1; off < lanes; off <<= 1) mx[n] = fmaxf(mx[n], __shfl_xor_sync(0xffffffffu, mx[n], off));
+          mx[n] = fmaxf(mx[n], __shfl_xor_sync(0xffffffffu, mx[n], 1));
+          mx[n] = fmaxf(mx[n], __shfl_xor_sync(0xffffffffu, mx[n], 2));
+          if (lanes > 4) mx[n] = fmaxf(mx[n], __shfl_xor_sync(0xffffffffu, mx[n], 4));
+          if (lanes > 8) mx[n] = fmaxf(mx[n], __shfl_xor_sync(0xffffffffu, mx[n], 8));
+          if (lanes > 16) mx[n] = fmaxf(mx[n], __shfl_xor_sync(0xffffffffu, mx[n], 16));
           mx[n] = fmaxf(mx[n], kScaleFloor);
-          const int i = (n * blockDim.x + threadIdx.x) * kVec;
-          if (i < a.hidden && threadIdx.x % lanes == 0) a.scales[row * (a.hidden / a.group) + i / a.group] = mx[n] / kE4m3Max;
+          if (in[n] && (threadIdx.x & (lanes - 1)) == 0) sc[n * step >> shift] = mx[n] * (1.f / kE4m3Max);
         }
       }
 #pragma unroll
-      for (int n = 0; n < kN; ++n) {
-        const int i = (n * blockDim.x + threadIdx.x) * kVec;
-        if (i < a.hidden) store_codes<kVec>(o + i, h[n], kE4m3Max / mx[n]);
-      }
+      for (int n = 0; n < kN; ++n)
+        if (in[n]) store_codes<kVec>(o + n * step, h[n], __fdividef(kE4m3Max, mx[n]));
     }
   }
 }
@@ -213,11 +229,11 @@ __global__ void __launch_bounds__(256) rms_norm_any_kernel(NormArgs a) {
       for (int i = g * a.group + threadIdx.x; i < (g + 1) * a.group; i += blockDim.x)
         mx = fmaxf(mx, fabsf(at(i) * inv * a.weight[i]));
       __syncthreads();
-      const float scale = fmaxf(block_max(mx, sh), kScaleFloor) / kE4m3Max;
-      if (threadIdx.x == 0) a.scales[row * groups + g] = scale;
+      const float top = fmaxf(block_max(mx, sh), kScaleFloor), mul = __fdividef(kE4m3Max, top);
+      if (threadIdx.x == 0) a.scales[row * groups + g] = top * (1.f / kE4m3Max);
       for (int i = g * a.group + threadIdx.x; i < (g + 1) * a.group; i += blockDim.x) {
         const float h = at(i);
-        o[i] = __nv_cvt_float_to_fp8(h * inv * a.weight[i] / scale, __NV_SATFINITE, __NV_E4M3);
+        o[i] = __nv_cvt_float_to_fp8(h * inv * a.weight[i] * mul, __NV_SATFINITE, __NV_E4M3);
         if (ro) ro[i] = Elem<T>::from_f(h);
       }
     }
@@ -243,8 +259,9 @@ cudaError_t launch(const NormArgs& a, cudaStream_t st) {
     if (vecs <= 768) return run<T, 8, 2>(a, (vecs + 63) / 64 * 32, st);
     return run<T, 8, 4>(a, (vecs + 127) / 128 * 32, st);
   }
-  if (!vec && a.hidden <= 6144 && a.group == a.hidden) {
+  if (!vec && a.hidden <= 8192 && a.group == a.hidden) {
     if (a.hidden <= 1024) return run<T, 1, 4>(a, (a.hidden + 127) / 128 * 32, st);
+    if (a.hidden <= 4096) return run<T, 1, 8>(a, (a.hidden + 255) / 256 * 32, st);
     return run<T, 1, 16>(a, (a.hidden + 511) / 512 * 32, st);
   }
   const int64_t blocks = a.rows < 65536 ? a.rows : 65536;

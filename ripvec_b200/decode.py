@@ -29,7 +29,7 @@ _current_stream = torch._C._cuda_getCurrentRawStream
 
 def _rows(name: str, t, shape: tuple, cache: "PagedCache") -> tuple:
     """Address, token stride and head stride of ``t``, which must be ``shape`` rows like the cache's."""
-    st, sh, sd = t.stride() if t.ndim == 3 else (0, 0, 0)
+    st, sh, sd = t.stride() if t.dim() == 3 else (0, 0, 0)
     if sd != 1 or t.shape != shape or t.dtype is not cache.dtype or t.get_device() != cache.device_index:
         raise ValueError(f"{name} must be {shape} {cache.dtype} on {cache.device} with unit stride along the last "
                          f"axis, got {tuple(t.shape)} {t.dtype} on {t.device} with strides {t.stride()}")
@@ -189,42 +189,54 @@ def rms_norm(x, weight, *, residual=None, residual_out=None, out=None, eps: floa
     ``out = h / sqrt(mean(h^2) + eps) * weight``; ``h`` in 16 bits goes to ``residual_out`` where given (it may
     be ``residual`` or ``x``).  Returns ``(out, scales)``: 16-bit rows and ``None``, or with ``out_8bit`` e4m3
     codes and their f32 scales ``[rows, hidden / group]`` (``group = 0``: one scale a row)."""
-    code, dev = _DTYPES.get(x.dtype), x.get_device()
-    if code is None or x.ndim != 2 or dev < 0 or (x.shape[1] > 1 and x.stride(1) != 1):
-        raise ValueError("x must be a 2-D bf16 or f16 CUDA tensor with unit stride along the last axis")
-    shape = rows, hidden = x.shape
+    dtype, dev, shape = x.dtype, x.get_device(), x.shape
+    code = _DTYPES.get(dtype)
+    if code is None or dev < 0 or len(shape) != 2:
+        raise ValueError("x must be a 2-D bf16 or f16 CUDA tensor")
+    rows, hidden = shape
+    xs, unit = x.stride()
+    rs = ros = 0
+    rp = rop = None
+    if residual is not None:
+        rp, (rs, u) = residual.data_ptr(), residual.stride()
+        if residual.shape != shape or residual.dtype is not dtype or residual.get_device() != dev or u != 1 < hidden:
+            raise ValueError("residual must be like x, with unit stride along the last axis")
+    if residual_out is not None:
+        rop, (ros, u) = residual_out.data_ptr(), residual_out.stride()
+        if residual_out.shape != shape or residual_out.dtype is not dtype or residual_out.get_device() != dev \
+                or u != 1 < hidden:
+            raise ValueError("residual_out must be like x, with unit stride along the last axis")
+    if unit != 1 < hidden:
+        raise ValueError("x must have unit stride along the last axis")
     if weight.shape != shape[1:] or weight.dtype is not torch.float32 or weight.get_device() != dev \
             or not weight.is_contiguous():
         raise ValueError("weight must be a contiguous f32 [hidden] tensor on x's device")
-
-    def like(name, t, dtype):
-        if t.shape != shape or t.dtype is not dtype or t.get_device() != dev or (hidden > 1 and t.stride(1) != 1):
-            raise ValueError(f"{name} must be {tuple(shape)} {dtype} on x's device, with unit stride along the last axis")
-        return t.data_ptr(), t.stride(0)
-
-    ra = (None, 0) if residual is None else like("residual", residual, x.dtype)
-    roa = (None, 0) if residual_out is None else like("residual_out", residual_out, x.dtype)
-    if group and (not out_8bit or group not in (32, 64, 128, 256) or hidden % group):
-        raise ValueError("group must be 32, 64, 128 or 256, divide hidden, and comes with out_8bit")
-    dt = torch.float8_e4m3fn if out_8bit else x.dtype
-    if out is None:
-        out = torch.empty(shape, dtype=dt, device=x.device)
-    oa = like("out", out, dt)
-    if not out_8bit:
-        if scales is not None:
-            raise ValueError("scales come with out_8bit")
-    else:
+    if out_8bit:
+        if group and (group not in (32, 64, 128, 256) or hidden % group):
+            raise ValueError("group must be 32, 64, 128 or 256 and divide hidden")
+        dtype, code_out = torch.float8_e4m3fn, L.RV_DTYPE_E4M3
         per_row = hidden // group if group else 1
         if scales is None:
             scales = torch.empty((rows, per_row), dtype=torch.float32, device=x.device)
         elif scales.shape != (rows, per_row) or scales.dtype is not torch.float32 or scales.get_device() != dev \
                 or not scales.is_contiguous():
             raise ValueError(f"scales must be a contiguous {(rows, per_row)} f32 tensor on x's device")
+        sp = scales.data_ptr()
+    else:
+        if group or scales is not None:
+            raise ValueError("group and scales come with out_8bit")
+        code_out, sp = code, None
+    if out is None:
+        out = torch.empty_like(x, dtype=dtype, memory_format=torch.contiguous_format)
+        os = hidden
+    else:
+        os, u = out.stride()
+        if out.shape != shape or out.dtype is not dtype or out.get_device() != dev or u != 1 < hidden:
+            raise ValueError(f"out must be {tuple(shape)} {dtype} on x's device, with unit stride along the last axis")
     if rows == 0:
         return out, scales
-    args = (code, x.data_ptr(), x.stride(0), *ra, weight.data_ptr(), *roa, *oa, L.RV_DTYPE_E4M3 if out_8bit else code,
-            scales.data_ptr() if out_8bit else None, group, rows, hidden, eps,
-            _current_stream(dev) if stream is None else stream)
+    args = (code, x.data_ptr(), xs, rp, rs, weight.data_ptr(), rop, ros, out.data_ptr(), os, code_out, sp, group, rows,
+            hidden, eps, _current_stream(dev) if stream is None else stream)
     if torch.cuda.current_device() == dev:
         rc = L.lib().rv_rms_norm(*args)
     else:
