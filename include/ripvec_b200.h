@@ -327,7 +327,8 @@ int rv_index_find_duplicates(rv_index* idx, float threshold, int64_t max_pairs, 
  * serves every layer.  rv_step_append, rv_step_attend and rv_rms_norm queue their kernels on `stream`
  * (0 = the legacy default stream) and return; the tensors they are given must be ready in that
  * stream's order.  Calls on one step from different streams are ordered by the library, except while
- * a stream is being captured. */
+ * a stream is being captured.  A kernel that gave up waiting (RV_E_DEVICE) is reported by the step's
+ * next call. */
 
 /* One layer's key and value pools, [num_pages, kv_heads, page_size, head_dim] in any order of memory:
  * strides in elements, unit stride along head_dim; pools and strides multiples of 16 bytes. */
@@ -366,7 +367,7 @@ int rv_step_plan(rv_step* step, int32_t n_seqs, const int32_t* q_lens, const int
  * with strides in elements and unit stride along head_dim.  The first `rot` values of a head turn by
  * cos / sin [positions, rot / 2] (f32), as pairs (i, i + rot / 2), or (2i, 2i + 1) when interleaved;
  * f32 arithmetic, rounded once.  RV_E_INVALID where own_lens < q_lens, and where a page that new
- * tokens go to is also another sequence's or a prefix's. */
+ * tokens go to takes another sequence's new tokens too or is a prefix's. */
 int rv_step_append(rv_step* step, const rv_kv_cache* cache, const void* q, int64_t q_token_stride,
                    int64_t q_head_stride, const void* k, int64_t k_token_stride, int64_t k_head_stride, const void* v,
                    int64_t v_token_stride, int64_t v_head_stride, void* q_out, int64_t q_out_token_stride,
@@ -376,8 +377,10 @@ int rv_step_append(rv_step* step, const rv_kv_cache* cache, const void* q, int64
  * cache's dtype.  lse (optional, f32 [tokens, q_heads], contiguous): the natural logarithm of the
  * softmax's denominator, with which results over disjoint sets of keys can be joined.  A query that
  * sees no key gets zeros and -inf.  Softmax statistics and sums are f32; the softmax's weights enter
- * the second product in the cache's 16-bit type.  What a page holds past the last key is not used.
- * q and out start on 16 bytes with strides of 16 bytes; scale > 0. */
+ * the second product in the cache's 16-bit type.  What a page holds past the last key is not used;
+ * an infinity or NaN among a sequence's own values may reach the sequence's earlier queries of the
+ * same call, whose weight for it is 0.  The same inputs give the same bits.  q and out start on 16
+ * bytes with strides of 16 bytes and do not overlap; scale > 0. */
 int rv_step_attend(rv_step* step, const rv_kv_cache* cache, const void* q, int64_t q_token_stride,
                    int64_t q_head_stride, void* out, int64_t out_token_stride, int64_t out_head_stride, float* lse,
                    float scale, void* stream);

@@ -37,8 +37,10 @@ struct Staging {
   char* p = nullptr;
   size_t cap = 0;
   cudaEvent_t done = nullptr;
+  bool own = false;  // allocated by itself
 };
 
+constexpr size_t kSmallPlan = 64 * 1024;          // bytes of records that a new step has room for
 constexpr int64_t kMaxTokens = int64_t(1) << 24;  // of one step
 constexpr int64_t kMaxKeys = int64_t(1) << 30;    // of one sequence or prefix
 
@@ -73,6 +75,7 @@ struct rv_step {
   int last_pos = -1;  // largest position of a new token
   char* meta = nullptr;
   size_t meta_cap = 0;
+  bool own_meta = false;
   int fold = 1;  // query heads of a key/value head that share a row tile: the largest divisor up to kRowTile
   const rv::StepToken* tokens = nullptr;
   const rv::StepParts* parts = nullptr;
@@ -82,6 +85,8 @@ struct rv_step {
   float* work = nullptr;  // partial results
   size_t work_cap = 0;    // floats
   int64_t n_parts = 0;
+  char* base_host = nullptr;         // pinned: the error word, and staging until a plan needs more
+  char* base_dev = nullptr;          // the few-row kernel's counters, and records until a plan needs more
   unsigned int* err_host = nullptr;  // error word in mapped host memory: kernels write it, calls look at it
   unsigned int* err_dev = nullptr;
   int* counter = nullptr;
@@ -91,7 +96,7 @@ struct rv_step {
   std::vector<rv::StepToken> tok;
   std::vector<StepSeq> seq;
   std::vector<int> group_first, pg;
-  std::vector<int> writer;  // by page: 1 + the sequence that writes to it
+  std::vector<int> written;  // pages that new tokens go to
   Schedule sched;
   // Calls on different streams wait for one another: plan, append and attend share the plan's device
   // records and the workspace.
@@ -415,7 +420,8 @@ int plan(rv_step* s, int32_t n_seqs, const int32_t* q_lens, const int32_t* own_l
   std::vector<int>& pg = s->pg;
   pg.assign(prefix_pages, prefix_pages + n_prefix_pages);
   pg.insert(pg.end(), own_pages, own_pages + n_own_pages);
-  s->writer.assign(size_t(num_pages), 0);
+  std::vector<int>& written = s->written;
+  written.clear();
   int t = 0, b = 0, last_pos = -1;
   int64_t pa = 0, pb = n_prefix_pages;
   for (int g = 0; g < n_groups; ++g) {
@@ -427,9 +433,7 @@ int plan(rv_step* s, int32_t n_seqs, const int32_t* q_lens, const int32_t* own_l
         const int page = place >= 0 ? pg[size_t(pb + place / ps)] : 0;
         tk[t++] = {page, place >= 0 ? place % ps : 0, prefix_lens[g] + place, b};
         if (place < 0) continue;
-        int& w = s->writer[size_t(page)];
-        if (w && w != b + 1) can_append = false;
-        w = b + 1;
+        if (i == 0 || place % ps == 0) written.push_back(page);
         if (prefix_lens[g] + place > last_pos) last_pos = prefix_lens[g] + place;
       }
       pb += count(own);
@@ -437,9 +441,11 @@ int plan(rv_step* s, int32_t n_seqs, const int32_t* q_lens, const int32_t* own_l
     pa += count(prefix_lens[g]);
     s->group_first.push_back(b);
   }
-  // A page that new tokens go to belongs to no prefix.
-  for (int64_t i = 0; i < n_prefix_pages; ++i)
-    if (s->writer[size_t(prefix_pages[i])]) can_append = false;
+  // A page that new tokens go to stands in the step's lists once.  (A sequence's new tokens take consecutive places.)
+  std::sort(written.begin(), written.end());
+  if (std::adjacent_find(written.begin(), written.end()) != written.end()) can_append = false;
+  for (int64_t i = 0; i < n_prefix_pages && can_append && !written.empty(); ++i)
+    if (std::binary_search(written.begin(), written.end(), prefix_pages[i])) can_append = false;
 
   Schedule& sc = s->sched;
   sc.row_items.clear();
@@ -447,7 +453,7 @@ int plan(rv_step* s, int32_t n_seqs, const int32_t* q_lens, const int32_t* own_l
   sc.joined.clear();
   sc.n_parts = 0;
   schedule(s->seq, s->group_first, int(tokens), s->fold, s->q_heads / s->fold, s->head_dim, rv::device_sm_count(), &sc);
-  if (sc.n_parts > INT_MAX ||
+  if (sc.n_parts > INT_MAX || int64_t(sc.joined.size()) * s->q_heads > INT_MAX ||
       (int64_t(sc.row_items.size()) + int64_t(sc.tile_items.size())) * (s->q_heads / s->fold) > INT_MAX)
     return fail(s, RV_E_INVALID, "the step is too large");
 
@@ -471,18 +477,18 @@ int plan(rv_step* s, int32_t n_seqs, const int32_t* q_lens, const int32_t* own_l
   cudaError_t e = cudaEventSynchronize(sg.done);  // the copy before last has left this buffer
   if (e != cudaSuccess) return cuda_fail(s, "waiting for an earlier plan", e);
   if (sg.cap < bytes) {
-    if (sg.p) cudaFreeHost(sg.p);
-    sg.p = nullptr;
-    sg.cap = 0;
+    if (sg.own) cudaFreeHost(sg.p);
+    sg = {nullptr, 0, sg.done, true};
     const size_t want = bytes + bytes / 2 + 4096;
     if ((e = cudaMallocHost(reinterpret_cast<void**>(&sg.p), want)) != cudaSuccess)
       return cuda_fail(s, "pinned staging", e);
     sg.cap = want;
   }
   if (s->meta_cap < bytes) {
-    if (s->meta) cudaFree(s->meta);  // waits for the kernels that still read it
+    if (s->own_meta) cudaFree(s->meta);  // waits for the kernels that still read it
     s->meta = nullptr;
     s->meta_cap = 0;
+    s->own_meta = true;
     const size_t want = bytes + bytes / 2 + 4096;
     if ((e = cudaMalloc(reinterpret_cast<void**>(&s->meta), want)) != cudaSuccess)
       return cuda_fail(s, "plan records", e);
@@ -551,11 +557,22 @@ int rv_step_create(int device, int32_t q_heads, int32_t kv_heads, int32_t head_d
   DeviceGuard g(device);
   bool ok = g.ok && cudaEventCreateWithFlags(&s->last, cudaEventDisableTiming) == cudaSuccess;
   for (auto& sg : s->staging) ok = ok && cudaEventCreateWithFlags(&sg.done, cudaEventDisableTiming) == cudaSuccess;
-  ok = ok && cudaHostAlloc(reinterpret_cast<void**>(&s->err_host), sizeof(unsigned int), cudaHostAllocMapped) == cudaSuccess;
-  if (ok) *s->err_host = 0;
-  ok = ok && cudaHostGetDevicePointer(reinterpret_cast<void**>(&s->err_dev), s->err_host, 0) == cudaSuccess;
-  ok = ok && cudaMalloc(reinterpret_cast<void**>(&s->counter), 2 * sizeof(int)) == cudaSuccess &&
-       cudaMemset(s->counter, 0, 2 * sizeof(int)) == cudaSuccess;
+  // Allocations of pinned memory take most of the time that making a step takes, so one serves its small needs.
+  ok = ok && cudaHostAlloc(reinterpret_cast<void**>(&s->base_host), 2 * kSmallPlan + 256, cudaHostAllocMapped) == cudaSuccess;
+  ok = ok && cudaMalloc(reinterpret_cast<void**>(&s->base_dev), kSmallPlan + 256) == cudaSuccess;
+  ok = ok && cudaMemset(s->base_dev, 0, 256) == cudaSuccess;
+  if (ok) {
+    s->err_host = reinterpret_cast<unsigned int*>(s->base_host);
+    *s->err_host = 0;
+    ok = cudaHostGetDevicePointer(reinterpret_cast<void**>(&s->err_dev), s->err_host, 0) == cudaSuccess;
+    for (int i = 0; i < 2; ++i) {
+      s->staging[i].p = s->base_host + 256 + i * kSmallPlan;
+      s->staging[i].cap = kSmallPlan;
+    }
+    s->counter = reinterpret_cast<int*>(s->base_dev);
+    s->meta = s->base_dev + 256;
+    s->meta_cap = kSmallPlan;
+  }
   if (!ok) {
     cudaGetLastError();
     rv_step_destroy(s);
@@ -575,12 +592,12 @@ void rv_step_destroy(rv_step* s) {
         cudaEventSynchronize(sg.done);
         cudaEventDestroy(sg.done);
       }
-      if (sg.p) cudaFreeHost(sg.p);
+      if (sg.own) cudaFreeHost(sg.p);
     }
-    if (s->meta) cudaFree(s->meta);
+    if (s->own_meta) cudaFree(s->meta);
     if (s->work) cudaFree(s->work);
-    if (s->counter) cudaFree(s->counter);
-    if (s->err_host) cudaFreeHost(s->err_host);
+    if (s->base_dev) cudaFree(s->base_dev);
+    if (s->base_host) cudaFreeHost(s->base_host);
     if (s->last) cudaEventDestroy(s->last);
   }
   delete s;

@@ -13,6 +13,7 @@ return.  The reference has no decoder; there is nothing of it to cite here.
 from __future__ import annotations
 
 import ctypes as C
+from itertools import chain
 from typing import Sequence
 
 import numpy as np
@@ -102,8 +103,9 @@ class DecodeStep:
              num_pages: int, prefix_lens: Sequence[int] = (), prefix_pages: Sequence[Sequence[int]] = (),
              group_sizes: Sequence[int] | None = None, causal: bool = True, stream: int | None = None) -> None:
         """``rv_step_plan``: sequence ``b`` brings ``q_lens[b]`` new tokens and has ``own_lens[b]`` keys of
-        its own, these included, in ``own_pages[b]`` (longer lists are cut).  Consecutive sequences form
-        groups that share a prefix; by default one group of all, with no prefix or the one given."""
+        its own, these included, in ``own_pages[b]`` (longer lists are cut; a padded 2-D numpy table will do
+        and is the quickest).  Consecutive sequences form groups that share a prefix; by default one group
+        of all, with no prefix or the one given."""
         self.tokens = None
         ps = self.page_size
         ql, ol, pl = _i32(q_lens), _i32(own_lens), _i32(prefix_lens)
@@ -122,9 +124,15 @@ class DecodeStep:
 
         def flat(lists, lens):
             need = -(-lens.astype(np.int64) // ps)
+            if isinstance(lists, np.ndarray) and lists.ndim == 2:  # a page table, padded rows
+                if len(need) and need.max() > lists.shape[1]:
+                    raise ValueError("a page list is shorter than its length needs")
+                return _i32(lists[np.arange(lists.shape[1]) < need[:, None]])
+            need = need.tolist()
             if any(len(p) < k for p, k in zip(lists, need)):
                 raise ValueError("a page list is shorter than its length needs")
-            return _i32([x for p, k in zip(lists, need.tolist()) for x in p[:k]])
+            kept = (p if len(p) == k else p[:k] for p, k in zip(lists, need))
+            return _i32(np.fromiter(chain.from_iterable(kept), np.int64, sum(need)))
 
         op, pp = flat(own_pages, ol), flat(prefix_pages, pl)
         self._check(self._lib.rv_step_plan(self._h, len(ql), ql.ctypes.data, ol.ctypes.data, op.ctypes.data, len(gs),

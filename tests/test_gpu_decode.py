@@ -518,3 +518,63 @@ def test_empty_calls(cuda_device):
     assert b.step.attend(b.cache, b.queries).shape == (0, 8, 128)
     out, scales = rms_norm(torch.zeros(0, 256, dtype=torch.bfloat16, device="cuda"), torch.ones(256, device="cuda"), out_8bit=True)
     assert out.shape == (0, 256) and scales.shape == (0, 1)
+
+
+# ------------------------------------------------------------------ together
+def test_decoder_example(cuda_device):
+    """The example decoder, a context read once and shared by answers that go on from it token by token, against
+    the same network in f32 without a cache: cosine of every logits row at least 0.999, the bar of the encoder's
+    embeddings in 16 bits."""
+    import importlib.util
+    from pathlib import Path
+
+    torch = _torch()
+    spec = importlib.util.spec_from_file_location("answer_over_context",
+                                                  Path(__file__).resolve().parent.parent / "examples" / "answer_over_context.py")
+    ex = importlib.util.module_from_spec(spec)
+    import sys
+
+    sys.modules[spec.name] = ex
+    spec.loader.exec_module(ex)
+    d = ex.Decoder(ex.DecoderSpec(pages=64), seed=3)
+    s = d.spec
+    g = torch.Generator(device="cuda").manual_seed(4)
+    context = torch.randint(0, s.vocab, (300,), generator=g, device="cuda")
+    answers = torch.randint(0, s.vocab, (5, 9), generator=g, device="cuda")
+
+    def plain(ids):
+        n = len(ids)
+        x = d.embedding[ids].float()
+        norm = lambda x, w: x * torch.rsqrt(x.square().mean(-1, keepdim=True) + s.eps) * w  # noqa: E731
+        see = torch.ones(n, n, device="cuda", dtype=torch.bool).tril()
+
+        def turn(x):
+            a, b = x.chunk(2, -1)
+            c, si = d.cos[:n, None], d.sin[:n, None]
+            return torch.cat((a * c - b * si, b * c + a * si), -1)
+
+        for l in d.layers:
+            q, k, v = (norm(x, l["norm1"]) @ l["qkv"].float().T).view(n, -1, s.head_dim).split((s.q_heads, s.kv_heads, s.kv_heads), 1)
+            q, k = turn(q), turn(k)
+            k, v = (y.repeat_interleave(s.q_heads // s.kv_heads, 1) for y in (k, v))
+            p = (torch.einsum("ihd,jhd->hij", q, k) * s.head_dim ** -0.5).masked_fill(~see, -math.inf).softmax(-1)
+            x = x + torch.einsum("hij,jhd->ihd", p, v).reshape(n, -1) @ l["o"].float().T
+            gate, up = (norm(x, l["norm2"]) @ l["up"].float().T).chunk(2, -1)
+            x = x + (torch.nn.functional.silu(gate) * up) @ l["down"].float().T
+        return norm(x, d.norm) @ d.embedding.float().T
+
+    want = torch.stack([plain(torch.cat((context, a)))[len(context):] for a in answers])
+    read = d.read(context)
+    pages = [d.take_pages(answers.shape[1]) for _ in answers]
+    got, own = [], 0
+    for new in (4, 1, 1, 1, 2):  # a prompt, single tokens, two at once
+        ids = answers[:, own:own + new].reshape(-1)
+        own += new
+        d.step.plan(q_lens=[new] * 5, own_lens=[own] * 5, own_pages=pages, prefix_lens=[read["length"]],
+                    prefix_pages=[read["pages"]], num_pages=s.pages)
+        got.append(d.forward(ids).float().view(5, new, -1))
+    got = torch.cat(got, 1)
+    cos = torch.nn.functional.cosine_similarity(got.double(), want.double(), dim=-1)
+    assert cos.min().item() >= 0.999, cos.min().item()
+    out = d.answer(read, [a[:n] for a, n in zip(answers, (4, 1, 9, 2, 3))], 6)
+    assert out.shape == (5, 6) and out.min() >= 0 and out.max() < s.vocab
