@@ -140,10 +140,8 @@ __global__ void __launch_bounds__(kThreads, kPerSm<D>) attend_rows_kernel(const 
     // Lanes 0..15 copy K, lanes 16..31 V (a 64-key tile is at most 4 boxes of 2 halves).
     const int side = lane >> 4, l16 = lane & 15;
     int issued = 0;
-    int w = lane == 0 ? atomicAdd(p.counter, 1) : 0;
-    w = __shfl_sync(0xffffffffu, w, 0);
-    StepItem it{};
-    if (w < total) it = p.items[w / p.groups];
+    int w = blockIdx.x;  // then what the counter gives, from gridDim.x on
+    StepItem it = p.items[w / p.groups];
     for (int turn = 0;; ++turn) {
       // Hand over the piece of work (or that there is none left), and ask for the next.
       Piece& pc = piece[turn & 1];
@@ -157,7 +155,7 @@ __global__ void __launch_bounds__(kThreads, kPerSm<D>) attend_rows_kernel(const 
         copies_arrive(&w_full[turn & 1]);
         break;
       }
-      const int next = lane == 0 ? atomicAdd(p.counter, 1) : 0;
+      const int next = lane == 0 ? gridDim.x + atomicAdd(p.counter, 1) : 0;
       const int hg = w % p.groups, rows = it.n * p.fold;
       KeyTile t = key_tile<kRowKeys>(it, 0);
       int page = TileCopy<kRowKeys, kHalves>::page_of(p, t, l16);

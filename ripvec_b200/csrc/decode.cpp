@@ -181,12 +181,15 @@ int tiles_of(const rv::StepItem& it, int keys) {
   return (it.a1 - it.a0 + keys - 1) / keys + (it.b1 - it.b0 + keys - 1) / keys;
 }
 
+// So many tiles of 64 keys are one part of the few-row kernel whatever there is to do: with 8 rows of 128 values,
+// 4 tiles whole take 8.3 us and 8 take 11.3, in parts with their join 8.4.
+constexpr int kWhole = 4;
+
 // Cuts an item's key tiles into parts of at most `most` tiles of about equal length.
 template <class F>
 void cut(const rv::StepItem& it, int keys, int most, F&& emit) {
   const int na = (it.a1 - it.a0 + keys - 1) / keys, n = tiles_of(it, keys);
-  // Up to 4 tiles of 64 keys are not worth a join of their own.
-  const int parts = keys == rv::kRowKeys && n <= 4 ? 1 : std::max(1, (n + most - 1) / most);
+  const int parts = keys == rv::kRowKeys && n <= kWhole ? 1 : std::max(1, (n + most - 1) / most);
   for (int k = 0; k < parts; ++k) {
     const int lo = int(int64_t(n) * k / parts), hi = int(int64_t(n) * (k + 1) / parts);
     rv::StepItem x = it;
@@ -277,8 +280,8 @@ int choose_row_cut(const std::vector<Job>& jobs, int groups, int sms) {
   return int(std::max<int64_t>(2, (total + 6 * sms - 1) / (6 * sms)));
 }
 
-// Divides a step's attention into items.  A sequence whose rows fill a row tile by themselves walks the prefix
-// and its own keys in one item, without partial results.  Sequences of few rows share the prefix: the rows of
+// Divides a step's attention into items.  A sequence whose rows fill half a row tile by themselves walks the prefix
+// and its own keys in one item, without partial results.  Sequences of fewer rows share the prefix: the rows of
 // all of them are packed into row tiles that read each prefix key once, and their own keys are separate items.
 void schedule(const std::vector<StepSeq>& seqs, const std::vector<int>& group_first, int n_tokens, int fold,
               int groups, int head_dim,
@@ -302,13 +305,24 @@ void schedule(const std::vector<StepSeq>& seqs, const std::vector<int>& group_fi
     const int end = group_first[g + 1];
     while (b < end) {
       // A run of sequences of few rows.
-      int e = b, live = 0, n = 0;
+      int e = b, live = 0, n = 0, longest = 0;
       while (e < end && seqs[e].n * fold < rv::kTileRows / 2) {
         live += seqs[e].n > 0;
         n += seqs[e].n;
+        if (seqs[e].n > 0) longest = std::max(longest, (seqs[e].len_b + rv::kRowKeys - 1) / rv::kRowKeys);
         ++e;
       }
-      if (live > 1 && seqs[b].len_a > 0) {
+      // Each by itself where there is nothing to share, and where prefix and own keys together are so few that an
+      // item takes them in one part: no join then (prefix 128, 40 own keys: 7.3 us against 8 to 11 for 2 to 64
+      // sequences).
+      const int shared = (seqs[b].len_a + rv::kRowKeys - 1) / rv::kRowKeys;
+      if (live == 1 || (live > 1 && (shared == 0 || shared + longest <= kWhole))) {
+        for (; b < e; ++b)
+          if (seqs[b].n > 0)
+            add(seqs[b].n * fold <= rv::kRowTile, seqs[b].tok0, seqs[b].n, seqs[b], true, true, seqs[b].diag, false);
+        continue;
+      }
+      if (live > 1) {
         const int t0 = seqs[b].tok0;
         // One kernel for all of a run, so that all its tokens get as many partials of the prefix.
         if (n * fold <= rv::kRowTile) add(true, t0, n, seqs[b], true, false, 0, true);
@@ -319,15 +333,12 @@ void schedule(const std::vector<StepSeq>& seqs, const std::vector<int>& group_fi
             add(seqs[b].n * fold <= rv::kRowTile, seqs[b].tok0, seqs[b].n, seqs[b], false, true, seqs[b].diag, false);
         continue;
       }
+      // A sequence of many rows (or a run without any).
       const StepSeq& s = seqs[b];
-      if (s.n * fold <= rv::kRowTile) {
-        if (s.n > 0) add(true, s.tok0, s.n, s, true, true, s.diag, false);
-      } else {
-        for (int t = 0; t < s.n; t += 2 * per)
-          add(false, s.tok0 + t, std::min(2 * per, s.n - t), s, true, true,
-              s.diag > INT_MAX / 4 ? s.diag : s.diag + t, false);
-      }
-      ++b;
+      for (int t = 0; t < s.n; t += 2 * per)
+        add(false, s.tok0 + t, std::min(2 * per, s.n - t), s, true, true, s.diag > INT_MAX / 4 ? s.diag : s.diag + t,
+            false);
+      b = std::max(e, b + 1);
     }
   }
   // Parts: a token's partials are numbered through its items in order.
