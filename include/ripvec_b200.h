@@ -409,8 +409,9 @@ int rv_op_attention(int32_t act_dtype, const void* qkv, void* ctx_out, const int
                     float scale, void* stream);
 /* Test hook of the device-side error path (no counterpart in the reference; the reference's
  * contract is that errors propagate, backend/mod.rs:53-54).  While enabled, every tcgen05
- * attention launch (rv_op_attention and the attention of rv_embed_*) withholds the score signal
- * of each persistent CTA's first tile and bounds every pipeline wait by wait_limit_cycles SM
+ * attention launch (rv_op_attention, the attention of rv_embed_* and of rv_step_attend) withholds
+ * the score signal (in rv_step_attend's few-row kernel the signal of the work) of each persistent
+ * CTA's first tile and bounds every pipeline wait by wait_limit_cycles SM
  * cycles: the softmax warps' wait expires, every role leaves through the kernel's bounded-wait
  * exit (copies and MMAs in flight are drained, TMEM is freed), and the call returns RV_E_DEVICE.
  * Nothing faults, traps or spins without bound.  enable = 0 restores normal launches.  Process

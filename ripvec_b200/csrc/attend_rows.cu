@@ -172,7 +172,8 @@ __global__ void __launch_bounds__(kThreads, kPerSm<D>) attend_rows_kernel(const 
           pc.it = it;
           pc.w = w;
         }
-        mbar_arrive(&w_full[turn & 1]);
+        // (Test hook: the first piece is never announced, and the consumers' wait for it runs out.)
+        if (!(p.stall && turn == 0)) mbar_arrive(&w_full[turn & 1]);
         copies_arrive(&w_full[turn & 1]);
       }
       const int tiles = key_tiles<kRowKeys>(it);
@@ -230,8 +231,15 @@ __global__ void __launch_bounds__(kThreads, kPerSm<D>) attend_rows_kernel(const 
     if (blockIdx.x == 0) wait_before();
     return;
   }
+  auto give_up = [&]() {  // a wait of this warp ran out: ends the others'
+    if (failed && lane == 0) {
+      *abort_flag = 1;
+      atomicOr_system(p.err, kErrWaitTimeout);
+    }
+  };
   for (int turn = 0;; ++turn) {
-    failed = !__all_sync(0xffffffffu, mbar_wait_spin(&w_full[turn & 1], (turn >> 1) & 1, abort_flag));
+    failed = !__all_sync(0xffffffffu, mbar_wait_spin(&w_full[turn & 1], (turn >> 1) & 1, abort_flag, p.wait_limit));
+    give_up();
     const Piece& pc = piece[turn & 1];
     const int w = failed ? total : pc.w;
     if (consumers_or(failed) || w >= total) break;
@@ -349,10 +357,7 @@ __global__ void __launch_bounds__(kThreads, kPerSm<D>) attend_rows_kernel(const 
         ph ^= 1u;
       }
     }
-    if (failed && lane == 0) {
-      *abort_flag = 1;
-      atomicOr_system(p.err, kErrWaitTimeout);
-    }
+    give_up();
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
       l[i] += __shfl_xor_sync(0xffffffffu, l[i], 1);

@@ -649,6 +649,11 @@ void attention_set_stall(int enable, long long wait_limit_cycles) {
   g_stall.store(enable ? 1 : 0, std::memory_order_relaxed);
 }
 
+void attention_get_stall(int* enable, long long* wait_limit_cycles) {
+  *enable = g_stall.load(std::memory_order_relaxed);
+  *wait_limit_cycles = *enable ? g_stall_limit.load(std::memory_order_relaxed) : kWaitLimitCycles;
+}
+
 int fill_attention_tiles(const int* cu_seqlens, int n_seqs, int2* out) {
   // Longest sequences first: the persistent CTAs take items in this order (per head), so the
   // items with the most key tiles start first and the short ones fill the end of each wave.

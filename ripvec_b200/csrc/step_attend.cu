@@ -106,6 +106,7 @@ cudaError_t step_attend(Act act, const AttendArgs& a, cudaStream_t st) {
   p.scale_log2 = a.scale * 1.4426950408889634f;
   p.err = a.err;
   p.counter = a.counter;
+  attention_get_stall(&p.stall, &p.wait_limit);
   CUtensorMap mk, mv, mq;
   cudaError_t e = cudaSuccess;
   if (a.n_tile_items > 0) {

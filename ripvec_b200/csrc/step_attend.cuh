@@ -24,6 +24,8 @@ struct AttendParams {
   float scale_log2;
   unsigned int* err;
   int* counter;  // [2] of the few-row kernel: work taken, CTAs done; 0 between launches
+  long long wait_limit;  // cycles after which the wait that the test hook starves gives up (and ends the others)
+  int stall;             // test hook: withhold each CTA's first signal to the consumers
 };
 
 __device__ __forceinline__ float ex2_approx(float x) {

@@ -578,3 +578,27 @@ def test_decoder_example(cuda_device):
     assert cos.min().item() >= 0.999, cos.min().item()
     out = d.answer(read, [a[:n] for a, n in zip(answers, (4, 1, 9, 2, 3))], 6)
     assert out.shape == (5, 6) and out.min() >= 0 and out.max() < s.vocab
+
+
+def test_waits_that_run_out_are_reported(cuda_device):
+    """The bounded-wait exits of both attention kernels: with the first signal of every CTA withheld and waits of
+    about a millisecond, the launch ends, the step's next call reports it, and the one after is right again."""
+    torch = _torch()
+    from ripvec_b200 import _lib as L
+
+    lib = L.lib()
+    for kw in (dict(q=(1, 2), own=(300, 40), prefix=(0,)),            # few-row kernel
+               dict(q=(200,), own=(260,), prefix=(300,)),             # tensor-core kernel
+               dict(q=(1,) * 40, own=(70,) * 40, prefix=(900,))):     # both, and the join
+        b = Batch(seed=26, **kw)
+        b.check()
+        assert lib.rv_debug_stall_attention(1, 2_000_000) == L.RV_OK
+        try:
+            b.step.attend(b.cache, b.queries)
+            torch.cuda.synchronize()
+        finally:
+            lib.rv_debug_stall_attention(0, 0)
+        with pytest.raises(L.RvError) as e:
+            b.step.attend(b.cache, b.queries)
+        assert e.value.code == L.RV_E_DEVICE
+        b.check()
