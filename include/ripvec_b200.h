@@ -357,7 +357,8 @@ int rv_step_tokens(const rv_step* step);
  * prefix_pages; a length of 0 is no prefix.  Every page is below num_pages.  A query sees its group's
  * whole prefix; with causal != 0, token i of q sees its own keys up to own_len - q + i, otherwise all
  * of them.  A key's position is prefix_len + its place among its sequence's own.  Replaces the
- * earlier plan once the calls queued with it are done; a failed plan leaves none. */
+ * earlier plan once the calls queued with it are done; a failed plan leaves none.  A captured call may
+ * be replayed until the next plan. */
 int rv_step_plan(rv_step* step, int32_t n_seqs, const int32_t* q_lens, const int32_t* own_lens,
                  const int32_t* own_pages, int32_t n_groups, const int32_t* group_sizes, const int32_t* prefix_lens,
                  const int32_t* prefix_pages, int64_t num_pages, int32_t causal, void* stream);

@@ -167,7 +167,7 @@ __global__ void __launch_bounds__(kThreads, kPerSm<D>) attend_rows_kernel(const 
                          (hg * p.fold + r % p.fold) * q.head_stride + 8 * k;
           copy16_async(swizzled(dst + (k >> 3) * (kRowTile * 128), r, k & 7), src);
         }
-        if (lane < it.n) pc.parts[lane] = p.parts[it.tok0 + lane];
+        if (lane < it.n) pc.parts[lane] = p.parts ? p.parts[it.tok0 + lane] : StepParts{0, 1};
         if (lane == 0) {
           pc.it = it;
           pc.w = w;

@@ -520,7 +520,7 @@ __global__ void __launch_bounds__(kThreads, 1) attend_tiles_kernel(const __grid_
       const float inv = 1.f / fin_l;
       uint8_t *dst = nullptr, *part = nullptr;
       if (fin_live) {
-        const StepParts pt = p.parts[fin_tok];
+        const StepParts pt = p.parts ? p.parts[fin_tok] : StepParts{0, 1};
         const float ls = none ? -INFINITY : fin_m + log2f(fin_l);
         if (pt.count == 1) {
           dst = reinterpret_cast<uint8_t*>(static_cast<T*>(p.out) + fin_tok * p.out_token + fin_head * p.out_head);

@@ -32,15 +32,14 @@ struct DeviceGuard {
   }
 };
 
-// Pinned staging of one plan's upload; reused once its copy has left it.
+// Pinned staging of a small plan's upload; reused once its copy has left it.
 struct Staging {
   char* p = nullptr;
-  size_t cap = 0;
   cudaEvent_t done = nullptr;
-  bool own = false;  // allocated by itself
 };
 
-constexpr size_t kSmallPlan = 64 * 1024;          // bytes of records that a new step has room for
+constexpr size_t kSmallPlan = 64 * 1024;          // bytes of records that go through pinned memory
+constexpr size_t kFirstRecords = 1024 * 1024;     // bytes of records that a new step has room for
 constexpr int64_t kMaxTokens = int64_t(1) << 24;  // of one step
 constexpr int64_t kMaxKeys = int64_t(1) << 30;    // of one sequence or prefix
 
@@ -85,7 +84,7 @@ struct rv_step {
   float* work = nullptr;  // partial results
   size_t work_cap = 0;    // floats
   int64_t n_parts = 0;
-  char* base_host = nullptr;         // pinned: the error word, and staging until a plan needs more
+  char* base_host = nullptr;         // pinned: the error word and the staging
   char* base_dev = nullptr;          // the few-row kernel's counters, and records until a plan needs more
   unsigned int* err_host = nullptr;  // error word in mapped host memory: kernels write it, calls look at it
   unsigned int* err_dev = nullptr;
@@ -93,6 +92,7 @@ struct rv_step {
   Staging staging[2];
   int turn = 0;
   // host side of the plan, kept for its memory
+  std::vector<char> host;
   std::vector<rv::StepToken> tok;
   std::vector<StepSeq> seq;
   std::vector<int> group_first, pg;
@@ -476,24 +476,29 @@ int plan(rv_step* s, int32_t n_seqs, const int32_t* q_lens, const int32_t* own_l
     return at;
   };
   const size_t o_tokens = place_of(s->tok.size() * sizeof(rv::StepToken));
-  const size_t o_parts = place_of(sc.parts.size() * sizeof(rv::StepParts));
+  // (Where every token is one item's, nothing is looked up by token.)
+  const size_t n_parts = sc.joined.empty() ? 0 : sc.parts.size();
+  const size_t o_parts = place_of(n_parts * sizeof(rv::StepParts));
   const size_t o_rows = place_of(sc.row_items.size() * sizeof(rv::StepItem));
   const size_t o_tiles = place_of(sc.tile_items.size() * sizeof(rv::StepItem));
   const size_t o_joined = place_of(sc.joined.size() * sizeof(int));
   const size_t o_pages = place_of(pg.size() * sizeof(int));
   const size_t floats = size_t(sc.n_parts) * size_t(s->q_heads) * size_t(s->head_dim + 1);
 
+  // Small plans, those of decoding steps, are copied from pinned memory and leave the host at once.  The records of
+  // long prompts come from pageable memory, which the copy takes over before it returns: pinned memory for them takes
+  // milliseconds to get.
   Staging& sg = s->staging[s->turn];
-  s->turn ^= 1;
-  cudaError_t e = cudaEventSynchronize(sg.done);  // the copy before last has left this buffer
-  if (e != cudaSuccess) return cuda_fail(s, "waiting for an earlier plan", e);
-  if (sg.cap < bytes) {
-    if (sg.own) cudaFreeHost(sg.p);
-    sg = {nullptr, 0, sg.done, true};
-    const size_t want = bytes + bytes / 2 + 4096;
-    if ((e = cudaMallocHost(reinterpret_cast<void**>(&sg.p), want)) != cudaSuccess)
-      return cuda_fail(s, "pinned staging", e);
-    sg.cap = want;
+  const bool small = bytes <= kSmallPlan;
+  char* from = sg.p;
+  cudaError_t e = cudaSuccess;
+  if (small) {
+    s->turn ^= 1;
+    e = cudaEventSynchronize(sg.done);  // the copy before last has left this buffer
+    if (e != cudaSuccess) return cuda_fail(s, "waiting for an earlier plan", e);
+  } else {
+    s->host.resize(bytes);
+    from = s->host.data();
   }
   if (s->meta_cap < bytes) {
     if (s->own_meta) cudaFree(s->meta);  // waits for the kernels that still read it
@@ -505,11 +510,11 @@ int plan(rv_step* s, int32_t n_seqs, const int32_t* q_lens, const int32_t* own_l
       return cuda_fail(s, "plan records", e);
     s->meta_cap = want;
   }
-  auto put = [&sg](size_t at, const void* p, size_t n) {
-    if (n) std::memcpy(sg.p + at, p, n);
+  auto put = [from](size_t at, const void* p, size_t n) {
+    if (n) std::memcpy(from + at, p, n);
   };
   put(o_tokens, s->tok.data(), s->tok.size() * sizeof(rv::StepToken));
-  put(o_parts, sc.parts.data(), sc.parts.size() * sizeof(rv::StepParts));
+  put(o_parts, sc.parts.data(), n_parts * sizeof(rv::StepParts));
   put(o_rows, sc.row_items.data(), sc.row_items.size() * sizeof(rv::StepItem));
   put(o_tiles, sc.tile_items.data(), sc.tile_items.size() * sizeof(rv::StepItem));
   put(o_joined, sc.joined.data(), sc.joined.size() * sizeof(int));
@@ -524,12 +529,12 @@ int plan(rv_step* s, int32_t n_seqs, const int32_t* q_lens, const int32_t* own_l
     s->work_cap = want;
   }
   if ((e = enter(s, st)) != cudaSuccess) return cuda_fail(s, "ordering streams", e);
-  if (bytes && (e = cudaMemcpyAsync(s->meta, sg.p, bytes, cudaMemcpyHostToDevice, st)) != cudaSuccess)
+  if (bytes && (e = cudaMemcpyAsync(s->meta, from, bytes, cudaMemcpyHostToDevice, st)) != cudaSuccess)
     return cuda_fail(s, "plan upload", e);
-  if ((e = cudaEventRecord(sg.done, st)) != cudaSuccess) return cuda_fail(s, "plan upload", e);
+  if (small && (e = cudaEventRecord(sg.done, st)) != cudaSuccess) return cuda_fail(s, "plan upload", e);
   if ((e = leave(s, st)) != cudaSuccess) return cuda_fail(s, "ordering streams", e);
   s->tokens = reinterpret_cast<rv::StepToken*>(s->meta + o_tokens);
-  s->parts = reinterpret_cast<rv::StepParts*>(s->meta + o_parts);
+  s->parts = n_parts ? reinterpret_cast<rv::StepParts*>(s->meta + o_parts) : nullptr;
   s->row_items = reinterpret_cast<rv::StepItem*>(s->meta + o_rows);
   s->tile_items = reinterpret_cast<rv::StepItem*>(s->meta + o_tiles);
   s->joined = reinterpret_cast<int*>(s->meta + o_joined);
@@ -570,7 +575,7 @@ int rv_step_create(int device, int32_t q_heads, int32_t kv_heads, int32_t head_d
   for (auto& sg : s->staging) ok = ok && cudaEventCreateWithFlags(&sg.done, cudaEventDisableTiming) == cudaSuccess;
   // Allocations of pinned memory take most of the time that making a step takes, so one serves its small needs.
   ok = ok && cudaHostAlloc(reinterpret_cast<void**>(&s->base_host), 2 * kSmallPlan + 256, cudaHostAllocMapped) == cudaSuccess;
-  ok = ok && cudaMalloc(reinterpret_cast<void**>(&s->base_dev), kSmallPlan + 256) == cudaSuccess;
+  ok = ok && cudaMalloc(reinterpret_cast<void**>(&s->base_dev), kFirstRecords + 256) == cudaSuccess;
   ok = ok && cudaMemset(s->base_dev, 0, 256) == cudaSuccess;
   if (ok) {
     s->err_host = reinterpret_cast<unsigned int*>(s->base_host);
@@ -578,11 +583,10 @@ int rv_step_create(int device, int32_t q_heads, int32_t kv_heads, int32_t head_d
     ok = cudaHostGetDevicePointer(reinterpret_cast<void**>(&s->err_dev), s->err_host, 0) == cudaSuccess;
     for (int i = 0; i < 2; ++i) {
       s->staging[i].p = s->base_host + 256 + i * kSmallPlan;
-      s->staging[i].cap = kSmallPlan;
     }
     s->counter = reinterpret_cast<int*>(s->base_dev);
     s->meta = s->base_dev + 256;
-    s->meta_cap = kSmallPlan;
+    s->meta_cap = kFirstRecords;
   }
   if (!ok) {
     cudaGetLastError();
@@ -603,7 +607,6 @@ void rv_step_destroy(rv_step* s) {
         cudaEventSynchronize(sg.done);
         cudaEventDestroy(sg.done);
       }
-      if (sg.own) cudaFreeHost(sg.p);
     }
     if (s->own_meta) cudaFree(s->meta);
     if (s->work) cudaFree(s->work);

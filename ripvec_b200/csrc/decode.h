@@ -67,7 +67,7 @@ constexpr int kTileKeys = 128;       // keys of its tile
 struct AttendArgs {
   const StepItem* row_items;   // for attend_rows: n * fold <= kRowTile
   const StepItem* tile_items;  // for attend_tiles: n <= 2 * (kTileRows / fold), most work first
-  const StepParts* parts;      // by token
+  const StepParts* parts;      // by token; null where every token has one partial
   const int* joined;           // tokens with a partial count other than 1
   const int* pages;
   int n_row_items, n_tile_items, n_joined;

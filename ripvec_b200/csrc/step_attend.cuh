@@ -12,7 +12,7 @@ namespace rv {
 // What a launch of either kernel needs beside its tensor maps.
 struct AttendParams {
   const StepItem* items;
-  const StepParts* parts;
+  const StepParts* parts;  // null: one partial a token
   const int* pages;
   int n_items, q_heads, fold;
   int groups, per_kv;  // head groups of `fold` query heads: all, and to a key/value head
