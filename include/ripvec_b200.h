@@ -395,6 +395,54 @@ int rv_rms_norm(int32_t act_dtype, const void* x, int64_t x_stride, const void* 
                 const float* weight, void* residual_out, int64_t residual_out_stride, void* out, int64_t out_stride,
                 int32_t out_dtype, float* scales, int32_t group, int64_t rows, int32_t hidden, float eps,
                 void* stream);
+/* The same three with their arguments in one record, for callers in languages where each argument of
+ * a foreign call costs time.  A null record is RV_E_INVALID; scale and eps are rounded to f32. */
+typedef struct rv_step_append_args {
+  const rv_kv_cache* cache;
+  const void* q;
+  int64_t q_token_stride, q_head_stride;
+  const void* k;
+  int64_t k_token_stride, k_head_stride;
+  const void* v;
+  int64_t v_token_stride, v_head_stride;
+  void* q_out;
+  int64_t q_out_token_stride, q_out_head_stride;
+  const float* cos;
+  const float* sin;
+  int64_t positions;
+  int32_t rot, interleaved;
+  void* stream;
+} rv_step_append_args;
+typedef struct rv_step_attend_args {
+  const rv_kv_cache* cache;
+  const void* q;
+  int64_t q_token_stride, q_head_stride;
+  void* out;
+  int64_t out_token_stride, out_head_stride;
+  float* lse;
+  double scale;
+  void* stream;
+} rv_step_attend_args;
+typedef struct rv_rms_norm_args {
+  const void* x;
+  int64_t x_stride;
+  const void* residual;
+  int64_t residual_stride;
+  const float* weight;
+  void* residual_out;
+  int64_t residual_out_stride;
+  void* out;
+  int64_t out_stride;
+  float* scales;
+  int64_t rows;
+  int32_t hidden, act_dtype, out_dtype, group;
+  double eps;
+  int32_t device; /* runs there; below 0: on the current device, as rv_rms_norm does */
+  void* stream;
+} rv_rms_norm_args;
+int rv_step_append_record(rv_step* step, const rv_step_append_args* args);
+int rv_step_attend_record(rv_step* step, const rv_step_attend_args* args);
+int rv_rms_norm_record(const rv_rms_norm_args* args);
 
 /* ---------------------------------------------------------------- single-kernel entry points
  * Used by the parity tests to check one kernel against the CPU oracle.  Device pointers. */

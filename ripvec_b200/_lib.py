@@ -140,6 +140,10 @@ SIGNATURES = {
     "rv_step_append": (C.c_int, [vp, vp] + [vp, i64, i64] * 4 + [vp, vp, i64, i32, i32, vp]),
     "rv_step_attend": (C.c_int, [vp, vp] + [vp, i64, i64] * 2 + [vp, f32, vp]),
     "rv_rms_norm": (C.c_int, [i32, vp, i64, vp, i64, vp, vp, i64, vp, i64, i32, vp, i32, i64, i32, f32, vp]),
+    # (records, as bytes)
+    "rv_step_append_record": (C.c_int, [vp, C.c_char_p]),
+    "rv_step_attend_record": (C.c_int, [vp, C.c_char_p]),
+    "rv_rms_norm_record": (C.c_int, [C.c_char_p]),
     "rv_op_gemm": (C.c_int, [i32, vp, vp, vp, i32, i32, i32, i32, i32, vp]),
     "rv_op_attention": (C.c_int, [i32, vp, vp, vp, i32, i32, i32, i32, f32, vp]),
     "rv_debug_stall_attention": (C.c_int, [i32, i64]),

@@ -4,6 +4,7 @@
 #include "decode.h"
 
 #include <algorithm>
+#include <cfloat>
 #include <climits>
 #include <cmath>
 #include <cstring>
@@ -117,6 +118,11 @@ int cuda_fail(rv_step* s, const char* what, cudaError_t e) {
 }
 
 // An error that an earlier call's kernels reported (without waiting for those still queued).
+// A record's double as f32; what is beyond its range becomes an infinity.
+float to_float(double v) {
+  return std::fabs(v) > double(FLT_MAX) ? float(std::copysign(HUGE_VAL, v)) : float(v);
+}
+
 bool device_error(rv_step* s) {
   volatile unsigned int* w = s->err_host;
   if (!*w) return false;
@@ -785,6 +791,31 @@ int rv_rms_norm(int32_t act_dtype, const void* x, int64_t x_stride, const void* 
   const cudaError_t e =
       rv::rms_norm(act_dtype == RV_DTYPE_BF16 ? rv::Act::kBf16 : rv::Act::kF16, a, static_cast<cudaStream_t>(stream));
   return e == cudaSuccess ? RV_OK : RV_E_CUDA;
+}
+
+int rv_step_append_record(rv_step* s, const rv_step_append_args* a) {
+  if (!a) return RV_E_INVALID;
+  return rv_step_append(s, a->cache, a->q, a->q_token_stride, a->q_head_stride, a->k, a->k_token_stride,
+                        a->k_head_stride, a->v, a->v_token_stride, a->v_head_stride, a->q_out, a->q_out_token_stride,
+                        a->q_out_head_stride, a->cos, a->sin, a->positions, a->rot, a->interleaved, a->stream);
+}
+
+int rv_step_attend_record(rv_step* s, const rv_step_attend_args* a) {
+  if (!a) return RV_E_INVALID;
+  return rv_step_attend(s, a->cache, a->q, a->q_token_stride, a->q_head_stride, a->out, a->out_token_stride,
+                        a->out_head_stride, a->lse, to_float(a->scale), a->stream);
+}
+
+int rv_rms_norm_record(const rv_rms_norm_args* a) {
+  if (!a) return RV_E_INVALID;
+  auto go = [a] {
+    return rv_rms_norm(a->act_dtype, a->x, a->x_stride, a->residual, a->residual_stride, a->weight, a->residual_out,
+                       a->residual_out_stride, a->out, a->out_stride, a->out_dtype, a->scales, a->group, a->rows,
+                       a->hidden, to_float(a->eps), a->stream);
+  };
+  if (a->device < 0) return go();
+  DeviceGuard g(a->device);
+  return g.ok ? go() : RV_E_CUDA;
 }
 
 }  // extern "C"

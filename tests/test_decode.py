@@ -79,3 +79,55 @@ def test_cache_layout_matches_header(tmp_path):
     subprocess.run([cc, f"-I{HEADER.parent}", str(src), "-o", str(exe)], check=True)
     got = list(map(int, subprocess.run([str(exe)], capture_output=True, text=True).stdout.split()))
     assert got == [C.sizeof(L.KvCache)] + [getattr(L.KvCache, f).offset for f in fields]
+
+
+RECORDS = {
+    "append": ("rv_step_append_args", "_append_args",
+               "cache q q_token_stride q_head_stride k k_token_stride k_head_stride v v_token_stride v_head_stride q_out "
+               "q_out_token_stride q_out_head_stride cos sin positions rot interleaved stream"),
+    "attend": ("rv_step_attend_args", "_attend_args",
+               "cache q q_token_stride q_head_stride out out_token_stride out_head_stride lse scale stream"),
+    "norm": ("rv_rms_norm_args", "_norm_args",
+             "x x_stride residual residual_stride weight residual_out residual_out_stride out out_stride scales rows hidden "
+             "act_dtype out_dtype group eps device stream"),
+}
+
+
+@pytest.mark.parametrize("kind", RECORDS)
+def test_records_match_header(tmp_path, kind):
+    """What Python packs is what C reads, field by field."""
+    import ripvec_b200.decode as D
+
+    cc = shutil.which("gcc") or shutil.which("cc")
+    if cc is None:
+        pytest.skip("no C compiler")
+    record, pack, fields = RECORDS[kind]
+    fields = fields.split()
+    data = getattr(D, pack)(*range(1, len(fields) + 1))
+    src = tmp_path / "record.c"
+    src.write_text('#include <stdio.h>\n#include "ripvec_b200.h"\n'
+                   f'int main(void){{{record} r; if (fread(&r, 1, sizeof r, stdin) != sizeof r || getchar() != EOF) return 1;'
+                   + "".join(f'printf("%lld ", (long long)r.{f});' for f in fields) + "return 0;}\n")
+    exe = tmp_path / "record"
+    subprocess.run([cc, f"-I{HEADER.parent}", str(src), "-o", str(exe)], check=True)
+    out = subprocess.run([str(exe)], input=data, capture_output=True, check=True).stdout
+    assert list(map(int, out.split())) == list(range(1, len(fields) + 1))
+
+
+def test_null_and_bad_records_are_refused():
+    import ripvec_b200.decode as D
+
+    lib = L.lib()
+    assert lib.rv_step_append_record(None, None) == L.RV_E_INVALID
+    assert lib.rv_step_attend_record(None, None) == L.RV_E_INVALID
+    assert lib.rv_step_append_record(None, D._append_args(*[0] * 19)) == L.RV_E_INVALID
+    assert lib.rv_step_attend_record(None, D._attend_args(*[0] * 10)) == L.RV_E_INVALID
+    assert lib.rv_rms_norm_record(None) == L.RV_E_INVALID
+
+    def norm_record(eps, rows=2):
+        return lib.rv_rms_norm_record(D._norm_args(16, 64, 0, 0, 16, 0, 0, 16, 64, 0, rows, 64, L.RV_DTYPE_BF16,
+                                                   L.RV_DTYPE_BF16, 0, eps, -1, 0))
+
+    assert norm_record(1e-5, rows=0) == L.RV_OK
+    for eps in (-1.0, math.nan, math.inf, 1e300, -1e300):
+        assert norm_record(eps) == L.RV_E_INVALID

@@ -602,3 +602,41 @@ def test_waits_that_run_out_are_reported(cuda_device):
             b.step.attend(b.cache, b.queries)
         assert e.value.code == L.RV_E_DEVICE
         b.check()
+
+
+def test_long_forms_and_records_agree(cuda_device):
+    """The C entries with one argument each give the bits of those with a record, which Python calls."""
+    torch = _torch()
+    from ripvec_b200 import _lib as L
+    from ripvec_b200.decode import rms_norm
+
+    b = Batch(q=[3, 1, 20], own=[9, 40, 20], prefix=[100], seed=5)
+    lib, st = L.lib(), torch.cuda.current_stream().cuda_stream
+    cos, sin = (torch.randn(200, 32, generator=b.gen, device="cuda") for _ in range(2))
+    k, v = b.randn(b.t, b.hkv, b.d), b.randn(b.t, b.hkv, b.d)
+
+    def at(t):
+        return t.data_ptr(), t.stride(0), t.stride(1)
+
+    turned = b.step.append(b.cache, b.queries, k, v, cos, sin, interleaved=True)
+    pools = b.k.clone(), b.v.clone()
+    b.k.fill_(0)
+    b.v.fill_(0)
+    again = torch.empty_like(turned)
+    assert lib.rv_step_append(b.step._h, b.cache._ref, *at(b.queries), *at(k), *at(v), *at(again), cos.data_ptr(),
+                              sin.data_ptr(), 200, 64, 1, st) == L.RV_OK
+    assert torch.equal(turned, again)
+    for pool, want in zip((b.k, b.v), pools):
+        written = pool != 0
+        assert written.any() and torch.equal(pool[written], want[written])
+        pool.copy_(want)
+    out = b.step.attend(b.cache, turned, scale=0.1)
+    again = torch.empty_like(out)
+    assert lib.rv_step_attend(b.step._h, b.cache._ref, *at(turned), *at(again), None, 0.1, st) == L.RV_OK
+    assert torch.equal(out, again)
+    x, w = b.randn(5, 256), torch.rand(256, generator=b.gen, device="cuda")
+    y, scales = rms_norm(x, w, out_8bit=True, group=64)
+    y2, s2 = torch.empty_like(y), torch.empty_like(scales)
+    assert lib.rv_rms_norm(L.RV_DTYPE_BF16, x.data_ptr(), 256, None, 0, w.data_ptr(), None, 0, y2.data_ptr(), 256,
+                           L.RV_DTYPE_E4M3, s2.data_ptr(), 64, 5, 256, 1e-5, st) == L.RV_OK
+    assert torch.equal(y.view(torch.uint8), y2.view(torch.uint8)) and torch.equal(scales, s2)
