@@ -390,7 +390,8 @@ int rv_step_attend(rv_step* step, const rv_kv_cache* cache, const void* q, int64
  * Rows of `hidden` (1..65536) values of act_dtype with strides in elements; weight f32 [hidden].
  * out_dtype act_dtype: 16-bit rows.  RV_DTYPE_E4M3: 8-bit codes with out ~ code * scale, scales f32
  * [rows, hidden / group], scale = max(max |out|, 1e-12) / 448 over a group of 32, 64, 128 or 256
- * values (hidden a multiple of it) or, with group 0, over the row. */
+ * values (hidden a multiple of it) or, with group 0, over the row.  The same values give the same bits
+ * whatever their alignment and strides. */
 int rv_rms_norm(int32_t act_dtype, const void* x, int64_t x_stride, const void* residual, int64_t residual_stride,
                 const float* weight, void* residual_out, int64_t residual_out_stride, void* out, int64_t out_stride,
                 int32_t out_dtype, float* scales, int32_t group, int64_t rows, int32_t hidden, float eps,
