@@ -286,9 +286,24 @@ int choose_row_cut(const std::vector<Job>& jobs, int groups, int sms) {
   return int(std::max<int64_t>(2, (total + 6 * sms - 1) / (6 * sms)));
 }
 
-// Divides a step's attention into items.  A sequence whose rows fill half a row tile by themselves walks the prefix
-// and its own keys in one item, without partial results.  Sequences of fewer rows share the prefix: the rows of
-// all of them are packed into row tiles that read each prefix key once, and their own keys are separate items.
+// What is saved, in key tiles of two row tiles, where a sequence of `rows` rows shares the walk of its prefix of `keys`
+// keys with its neighbours.  By itself it walks the prefix once for every two row tiles, 0.7 as long for a last one
+// alone, however few rows that holds; packed with others for its share of them, at the cost of partial results: three
+// tiles of time for every two row tiles, one for its own keys, and 0.022 a row to write and join them.
+double packing_saves(int64_t rows, int keys) {
+  constexpr int kPair = 2 * rv::kTileRows;
+  const int rest = int(rows % kPair);
+  const double alone = double(rows / kPair) + (rest == 0 ? 0.0 : rest <= rv::kTileRows ? 0.7 : 1.0);
+  const double share = double(rows) / kPair;
+  return double(keys) / rv::kTileKeys * (alone - share) - 1.0 - 3.0 * share - 0.022 * double(rows);
+}
+
+// Divides a step's attention into items.  Sequences that pack share the prefix: the rows of all of them are packed
+// into row tiles that read each prefix key once, and their own keys are separate items.  The others walk the prefix
+// and their own keys in one item, without partial results.  Sequences of less than half a row tile pack; those of
+// more do where it saves time, up to four row tiles all of a group's or none, so that runs stay whole.  32 query and
+// 8 key/value heads of 128, packed against not: 64 sequences of 20 tokens over 32768 keys 714 and 1333 us, 16 of 30 to
+// 60 over 8000 121 and 135, 32 of 16 to 24 over 2000 57 and 63; over 1000 45 and 42, where they walk alone.
 void schedule(const std::vector<StepSeq>& seqs, const std::vector<int>& group_first, int n_tokens, int fold,
               int groups, int head_dim,
               int sms, Schedule* out) {
@@ -306,13 +321,29 @@ void schedule(const std::vector<StepSeq>& seqs, const std::vector<int>& group_fi
     if (it.a1 == 0 && it.b1 == 0) return;
     (to_rows ? rows : tiles).push_back({it, packed});
   };
+  // A sequence's keys, or its own ones only.
+  auto whole = [&](const StepSeq& s, bool prefix) {
+    if (s.n * fold <= rv::kRowTile) return add(true, s.tok0, s.n, s, prefix, true, s.diag, false);
+    for (int t = 0; t < s.n; t += 2 * per)
+      add(false, s.tok0 + t, std::min(2 * per, s.n - t), s, prefix, true, s.diag > INT_MAX / 4 ? s.diag : s.diag + t,
+          false);
+  };
   for (size_t g = 0; g + 1 < group_first.size(); ++g) {
     int b = group_first[g];
     const int end = group_first[g + 1];
+    double vote = 0;
+    for (int k = b; k < end; ++k) {
+      const int64_t r = int64_t(seqs[k].n) * fold;
+      if (r >= rv::kTileRows / 2 && r < 4 * rv::kTileRows) vote += packing_saves(r, seqs[k].len_a);
+    }
+    auto packs = [&](const StepSeq& q) {
+      const int64_t r = int64_t(q.n) * fold;
+      return r < rv::kTileRows / 2 || (r < 4 * rv::kTileRows ? vote : packing_saves(r, q.len_a)) > 0;
+    };
     while (b < end) {
-      // A run of sequences of few rows.
+      // A run of sequences that pack.
       int e = b, live = 0, n = 0, longest = 0;
-      while (e < end && seqs[e].n * fold < rv::kTileRows / 2) {
+      while (e < end && packs(seqs[e])) {
         live += seqs[e].n > 0;
         n += seqs[e].n;
         if (seqs[e].n > 0) longest = std::max(longest, (seqs[e].len_b + rv::kRowKeys - 1) / rv::kRowKeys);
@@ -324,8 +355,7 @@ void schedule(const std::vector<StepSeq>& seqs, const std::vector<int>& group_fi
       const int shared = (seqs[b].len_a + rv::kRowKeys - 1) / rv::kRowKeys;
       if (live == 1 || (live > 1 && (shared == 0 || shared + longest <= kWhole))) {
         for (; b < e; ++b)
-          if (seqs[b].n > 0)
-            add(seqs[b].n * fold <= rv::kRowTile, seqs[b].tok0, seqs[b].n, seqs[b], true, true, seqs[b].diag, false);
+          if (seqs[b].n > 0) whole(seqs[b], true);
         continue;
       }
       if (live > 1) {
@@ -335,15 +365,11 @@ void schedule(const std::vector<StepSeq>& seqs, const std::vector<int>& group_fi
         else
           for (int t = 0; t < n; t += 2 * per) add(false, t0 + t, std::min(2 * per, n - t), seqs[b], true, false, 0, true);
         for (; b < e; ++b)
-          if (seqs[b].n > 0)
-            add(seqs[b].n * fold <= rv::kRowTile, seqs[b].tok0, seqs[b].n, seqs[b], false, true, seqs[b].diag, false);
+          if (seqs[b].n > 0) whole(seqs[b], false);
         continue;
       }
-      // A sequence of many rows (or a run without any).
-      const StepSeq& s = seqs[b];
-      for (int t = 0; t < s.n; t += 2 * per)
-        add(false, s.tok0 + t, std::min(2 * per, s.n - t), s, true, true, s.diag > INT_MAX / 4 ? s.diag : s.diag + t,
-            false);
+      // A sequence that does not (or a run without any rows).
+      if (seqs[b].n > 0) whole(seqs[b], true);
       b = std::max(e, b + 1);
     }
   }

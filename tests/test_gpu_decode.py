@@ -177,6 +177,16 @@ def test_attend_long_keys(cuda_device):
     Batch(q=(1, 300, 1, 2), own=(1, 2300, 4000, 9), prefix=(3000,), page=32, seed=7).check()
 
 
+def test_attend_middle_lengths_over_a_long_prefix(cuda_device):
+    """Sequences of one to four row tiles over a prefix so long that they share its walk; beside longer and shorter ones."""
+    Batch(q=(20,) * 5, own=(20, 21, 150, 83, 400), prefix=(4000,), page=64, seed=31).check()
+    Batch(q=(1, 20, 30, 0, 250, 25, 300, 16), own=(1, 100, 30, 9, 250, 7, 310, 0), prefix=(9000,), page=128, seed=32).check()
+    Batch(q=(20, 33, 17), own=(20, 5, 90), prefix=(5000,), causal=False, hq=28, hkv=4, seed=33).check()
+    Batch(q=(70, 127, 129, 255, 64), own=(70, 300, 129, 0, 100), prefix=(12000,), hq=12, hkv=12, d=64, page=32, act="f16",
+          seed=34).check()
+    Batch(q=(17, 19, 40, 40, 18), own=(17, 30, 40, 41, 18), prefix=(6000, 100, 7000), groups=(2, 2, 1), page=256, seed=35).check()
+
+
 def test_attend_groups(cuda_device):
     """Several prefixes in one step, some empty, some groups without sequences or tokens."""
     Batch(q=(1, 1, 5, 0, 1, 64), own=(4, 9, 5, 30, 0, 64), prefix=(130, 0, 64, 10), groups=(2, 0, 3, 1), seed=8).check()
