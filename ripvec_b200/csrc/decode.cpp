@@ -286,6 +286,11 @@ int choose_row_cut(const std::vector<Job>& jobs, int groups, int sms) {
   return int(std::max<int64_t>(2, (total + 6 * sms - 1) / (6 * sms)));
 }
 
+// Sequences of half a row tile and more pack up to so many rows, and while two partial results of all their rows take no
+// more than so many bytes of workspace.
+constexpr int kPackRows = 4 * rv::kTileRows;
+constexpr int64_t kPackBytes = int64_t(1) << 30;
+
 // What is saved, in key tiles of two row tiles, where a sequence of `rows` rows shares the walk of its prefix of `keys`
 // keys with its neighbours.  By itself it walks the prefix once for every two row tiles, 0.7 as long for a last one
 // alone, however few rows that holds; packed with others for its share of them, at the cost of partial results: three
@@ -301,9 +306,10 @@ double packing_saves(int64_t rows, int keys) {
 // Divides a step's attention into items.  Sequences that pack share the prefix: the rows of all of them are packed
 // into row tiles that read each prefix key once, and their own keys are separate items.  The others walk the prefix
 // and their own keys in one item, without partial results.  Sequences of less than half a row tile pack; those of
-// more do where it saves time, up to four row tiles all of a group's or none, so that runs stay whole.  32 query and
+// more, up to kPackRows, do where it saves time, all of a group's or none, so that runs stay whole.  32 query and
 // 8 key/value heads of 128, packed against not: 64 sequences of 20 tokens over 32768 keys 714 and 1333 us, 16 of 30 to
-// 60 over 8000 121 and 135, 32 of 16 to 24 over 2000 57 and 63; over 1000 45 and 42, where they walk alone.
+// 60 over 8000 121 and 135, 32 of 20 to 120 over 8000 334 and 368, 32 of 16 to 24 over 2000 57 and 63; over 1000 45 and
+// 42, where they walk alone.
 void schedule(const std::vector<StepSeq>& seqs, const std::vector<int>& group_first, int n_tokens, int fold,
               int groups, int head_dim,
               int sms, Schedule* out) {
@@ -332,13 +338,17 @@ void schedule(const std::vector<StepSeq>& seqs, const std::vector<int>& group_fi
     int b = group_first[g];
     const int end = group_first[g + 1];
     double vote = 0;
+    int64_t middle = 0;  // rows of a key/value head that it is about
     for (int k = b; k < end; ++k) {
       const int64_t r = int64_t(seqs[k].n) * fold;
-      if (r >= rv::kTileRows / 2 && r < 4 * rv::kTileRows) vote += packing_saves(r, seqs[k].len_a);
+      if (r < rv::kTileRows / 2 || r >= kPackRows) continue;
+      vote += packing_saves(r, seqs[k].len_a);
+      middle += r;
     }
+    if (middle * groups * head_dim * 8 > kPackBytes) vote = 0;
     auto packs = [&](const StepSeq& q) {
       const int64_t r = int64_t(q.n) * fold;
-      return r < rv::kTileRows / 2 || (r < 4 * rv::kTileRows ? vote : packing_saves(r, q.len_a)) > 0;
+      return r < rv::kTileRows / 2 || (r < kPackRows && vote > 0);
     };
     while (b < end) {
       // A run of sequences that pack.
