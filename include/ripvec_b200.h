@@ -149,7 +149,8 @@ typedef struct rv_index rv_index;
 
 /* SearchIndex::new: a bf16 device copy of n rows of dimension dim.  src is f32, bf16 or f16
  * (src_dtype); src_on_device selects a device or host source.  Rows are stored as given (the
- * reference stores embed_batch output, already L2-normalised). */
+ * reference stores embed_batch output, already L2-normalised).  A device source is read after all work
+ * queued on its device so far, on any stream. */
 int rv_index_create(int device, const void* src, int64_t n, int32_t dim, int32_t src_dtype,
                     int32_t src_on_device, rv_index** out);
 void rv_index_destroy(rv_index* idx);

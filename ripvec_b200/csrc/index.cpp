@@ -302,6 +302,8 @@ int rv_index_create(int device, const void* src, int64_t n, int32_t dim, int32_t
   if (n > 0 && cudaMalloc(&x->db, elems * 2) != cudaSuccess) return bail(RV_E_NOMEM);
   if (n > 0) {
     if (src_on_device) {
+      // The index's stream is ordered with no other: whatever still writes the rows, on any stream, ends first.
+      if (cudaDeviceSynchronize() != cudaSuccess) return bail(RV_E_CUDA);
       if (src_dtype == RV_DTYPE_BF16) {
         if (cudaMemcpyAsync(x->db, src, elems * 2, cudaMemcpyDeviceToDevice, x->stream) != cudaSuccess)
           return bail(RV_E_CUDA);

@@ -192,3 +192,21 @@ def test_sharded_indexes_merge_on_device(cuda_device):
     mi, ms, m64 = merge_topk_device(torch.stack(idx_l), torch.stack(s64_l), k)
     np.testing.assert_array_equal(mi.cpu().numpy(), ei)
     np.testing.assert_array_equal(m64.cpu().numpy(), es)
+
+
+def test_index_waits_for_rows_that_are_still_being_written(cuda_device):
+    """A device source may still be on its way, on any stream, when the index is made from it."""
+    import torch
+
+    rows = torch.randn(4096, 128, device="cuda").to(torch.bfloat16)
+    torch.cuda.synchronize()
+    for stream in (torch.cuda.current_stream(), torch.cuda.Stream()):
+        db = torch.zeros_like(rows)
+        torch.cuda.synchronize()
+        with torch.cuda.stream(stream):
+            torch.cuda._sleep(200_000_000)  # a tenth of a second
+            db.copy_(rows)
+        idx = SearchIndex(db)
+        got = idx.export_rows(bf16_bits=True)
+        idx.close()
+        assert np.array_equal(got, rows.view(torch.int16).cpu().numpy().view(np.uint16))
