@@ -151,8 +151,9 @@ __global__ void __launch_bounds__(kThreads, kPerSm<D>) attend_rows_kernel(const 
         failed = true;
         break;
       }
-      if (w >= total) {
-        if (lane == 0) pc.w = w;
+      // (Unsigned: no value of the counter leads past the items.)
+      if (static_cast<unsigned>(w) >= static_cast<unsigned>(total)) {
+        if (lane == 0) pc.w = total;
         mbar_arrive(&w_full[turn & 1]);
         copies_arrive(&w_full[turn & 1]);
         break;
@@ -204,7 +205,7 @@ __global__ void __launch_bounds__(kThreads, kPerSm<D>) attend_rows_kernel(const 
         if (j == 0) {
           // The next piece's record is on its way while this one's keys are.
           w = __shfl_sync(0xffffffffu, next, 0);
-          if (w < total) next_it = p.items[w / p.groups];
+          if (static_cast<unsigned>(w) < static_cast<unsigned>(total)) next_it = p.items[w / p.groups];
         }
         t = nt;
         page = next_page;

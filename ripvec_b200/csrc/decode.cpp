@@ -41,6 +41,7 @@ struct Staging {
 
 constexpr size_t kSmallPlan = 64 * 1024;          // bytes of records that go through pinned memory
 constexpr size_t kFirstRecords = 1024 * 1024;     // bytes of records that a new step has room for
+constexpr size_t kCounterBytes = 128;             // the two counters, at the head of a plan's records
 constexpr int64_t kMaxTokens = int64_t(1) << 24;  // of one step
 constexpr int64_t kMaxKeys = int64_t(1) << 30;    // of one sequence or prefix
 
@@ -86,7 +87,7 @@ struct rv_step {
   size_t work_cap = 0;    // floats
   int64_t n_parts = 0;
   char* base_host = nullptr;         // pinned: the error word and the staging
-  char* base_dev = nullptr;          // the few-row kernel's counters, and records until a plan needs more
+  char* base_dev = nullptr;          // records until a plan needs more
   unsigned int* err_host = nullptr;  // error word in mapped host memory: kernels write it, calls look at it
   unsigned int* err_dev = nullptr;
   int* counter = nullptr;
@@ -517,6 +518,9 @@ int plan(rv_step* s, int32_t n_seqs, const int32_t* q_lens, const int32_t* own_l
     bytes += (n + 15) / 16 * 16;
     return at;
   };
+  // The few-row kernel's counters come first, as zeros, on a cache line of their own: uploaded with the plan, they are
+  // in the order of streams that every call on the plan is in.
+  place_of(kCounterBytes);
   const size_t o_tokens = place_of(s->tok.size() * sizeof(rv::StepToken));
   // (Where every token is one item's, nothing is looked up by token.)
   const size_t n_parts = sc.joined.empty() ? 0 : sc.parts.size();
@@ -555,6 +559,7 @@ int plan(rv_step* s, int32_t n_seqs, const int32_t* q_lens, const int32_t* own_l
   auto put = [from](size_t at, const void* p, size_t n) {
     if (n) std::memcpy(from + at, p, n);
   };
+  std::memset(from, 0, kCounterBytes);
   put(o_tokens, s->tok.data(), s->tok.size() * sizeof(rv::StepToken));
   put(o_parts, sc.parts.data(), n_parts * sizeof(rv::StepParts));
   put(o_rows, sc.row_items.data(), sc.row_items.size() * sizeof(rv::StepItem));
@@ -571,10 +576,11 @@ int plan(rv_step* s, int32_t n_seqs, const int32_t* q_lens, const int32_t* own_l
     s->work_cap = want;
   }
   if ((e = enter(s, st)) != cudaSuccess) return cuda_fail(s, "ordering streams", e);
-  if (bytes && (e = cudaMemcpyAsync(s->meta, from, bytes, cudaMemcpyHostToDevice, st)) != cudaSuccess)
+  if ((e = cudaMemcpyAsync(s->meta, from, bytes, cudaMemcpyHostToDevice, st)) != cudaSuccess)
     return cuda_fail(s, "plan upload", e);
   if (small && (e = cudaEventRecord(sg.done, st)) != cudaSuccess) return cuda_fail(s, "plan upload", e);
   if ((e = leave(s, st)) != cudaSuccess) return cuda_fail(s, "ordering streams", e);
+  s->counter = reinterpret_cast<int*>(s->meta);
   s->tokens = reinterpret_cast<rv::StepToken*>(s->meta + o_tokens);
   s->parts = n_parts ? reinterpret_cast<rv::StepParts*>(s->meta + o_parts) : nullptr;
   s->row_items = reinterpret_cast<rv::StepItem*>(s->meta + o_rows);
@@ -617,8 +623,7 @@ int rv_step_create(int device, int32_t q_heads, int32_t kv_heads, int32_t head_d
   for (auto& sg : s->staging) ok = ok && cudaEventCreateWithFlags(&sg.done, cudaEventDisableTiming) == cudaSuccess;
   // Allocations of pinned memory take most of the time that making a step takes, so one serves its small needs.
   ok = ok && cudaHostAlloc(reinterpret_cast<void**>(&s->base_host), 2 * kSmallPlan + 256, cudaHostAllocMapped) == cudaSuccess;
-  ok = ok && cudaMalloc(reinterpret_cast<void**>(&s->base_dev), kFirstRecords + 256) == cudaSuccess;
-  ok = ok && cudaMemset(s->base_dev, 0, 256) == cudaSuccess;
+  ok = ok && cudaMalloc(reinterpret_cast<void**>(&s->base_dev), kFirstRecords) == cudaSuccess;
   if (ok) {
     s->err_host = reinterpret_cast<unsigned int*>(s->base_host);
     *s->err_host = 0;
@@ -626,8 +631,7 @@ int rv_step_create(int device, int32_t q_heads, int32_t kv_heads, int32_t head_d
     for (int i = 0; i < 2; ++i) {
       s->staging[i].p = s->base_host + 256 + i * kSmallPlan;
     }
-    s->counter = reinterpret_cast<int*>(s->base_dev);
-    s->meta = s->base_dev + 256;
+    s->meta = s->base_dev;
     s->meta_cap = kFirstRecords;
   }
   if (!ok) {
