@@ -378,7 +378,8 @@ int rv_step_append(rv_step* step, const rv_kv_cache* cache, const void* q, int64
 /* out = softmax(scale q K^T) V over the keys each query sees; out [tokens, q_heads, head_dim] of the
  * cache's dtype.  lse (optional, f32 [tokens, q_heads], contiguous): the natural logarithm of the
  * softmax's denominator, with which results over disjoint sets of keys can be joined.  A query that
- * sees no key gets zeros and -inf.  Softmax statistics and sums are f32; the softmax's weights enter
+ * sees no key gets zeros and -inf.  A score that is NaN or +inf makes its row and lse NaN; scores of
+ * -inf have no weight beside others, and alone make a row of NaN and an lse of -inf.  Softmax statistics and sums are f32; the softmax's weights enter
  * the second product in the cache's 16-bit type.  What a page holds past the last key is not used;
  * an infinity or NaN among a sequence's own values may reach the sequence's earlier queries of the
  * same call, whose weight for it is 0.  The same inputs give the same bits.  q and out start on 16

@@ -384,21 +384,23 @@ __global__ void __launch_bounds__(kThreads, kPerSm<D>) attend_rows_kernel(const 
       float top = -INFINITY;
 #pragma unroll
       for (int w = 0; w < kWarps; ++w) top = fmaxf(top, sm[w * kRowTile + r]);
+      // A warp without a key brings m = -inf, l = 0 and zeros; one whose scores are NaN m = -inf (fmaxf passes NaN over)
+      // and l = NaN, which has to reach the row.  So the keys, not the maximum, tell a row that sees none.
+      const bool sees = it.a1 > it.a0 || min(it.b1, it.diag + r / p.fold + 1) > it.b0;
+      const float ref = top == -INFINITY ? 0.f : top;
       float sum = 0.f, v[8] = {};
-      if (top != -INFINITY) {
 #pragma unroll
-        for (int w = 0; w < kWarps; ++w) {
-          const float f = ex2_approx(sm[w * kRowTile + r] - top);
-          sum += f * sm[(kWarps + w) * kRowTile + r];
-          const float* src = &so[(w * kRowTile + r) * (D + 4) + d];
+      for (int w = 0; w < kWarps; ++w) {
+        const float f = ex2_approx(sm[w * kRowTile + r] - ref);
+        sum += f * sm[(kWarps + w) * kRowTile + r];
+        const float* src = &so[(w * kRowTile + r) * (D + 4) + d];
 #pragma unroll
-          for (int e = 0; e < 8; ++e) v[e] += f * src[e];
-        }
-        const float inv = 1.f / sum;
-#pragma unroll
-        for (int e = 0; e < 8; ++e) v[e] *= inv;
+        for (int e = 0; e < 8; ++e) v[e] += f * src[e];
       }
-      const float ls = top == -INFINITY ? -INFINITY : top + log2f(sum);
+      const float inv = 1.f / sum;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) v[e] = sees ? v[e] * inv : 0.f;
+      const float ls = top + log2f(sum);
       const int tok = it.tok0 + r / p.fold, head = hg * p.fold + r % p.fold;
       const StepParts pt = pc.parts[r / p.fold];
       if (pt.count == 1) {

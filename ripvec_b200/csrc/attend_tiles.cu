@@ -517,7 +517,7 @@ __global__ void __launch_bounds__(kThreads, 1) attend_tiles_kernel(const __grid_
       __syncwarp();
     };
     auto read_out = [&]() {
-      const bool none = fin_l == 0.f;  // the row saw no key
+      const bool none = fin_l < 0.f;  // the row saw no key
       const float inv = 1.f / fin_l;
       uint8_t *dst = nullptr, *part = nullptr;
       if (fin_live) {
@@ -569,8 +569,10 @@ __global__ void __launch_bounds__(kThreads, 1) attend_tiles_kernel(const __grid_
     };
     while (!fail && wk.w < total) {
       const int n = i ? wk.count[1] : wk.count[0];
-      float m = kNone, l = 0.f;
       const int own = wk.it.diag + my_tok + 1 - wk.it.b0;  // own keys from b0 on that the row sees
+      // A row that sees no key keeps l = -inf.  (One whose scores are all -inf gets to 0, and NaN for its result.)
+      const bool sees = wk.it.a1 > wk.it.a0 || min(wk.it.b1 - wk.it.b0, own) > 0;
+      float m = kNone, l = sees ? 0.f : -INFINITY;
       for (int j = 0; !fail && j < n; ++j) {
         const int seen = wk.seen16(j, i);
         const int left = j < wk.na ? wk.it.a1 - wk.it.a0 - j * kTileKeys

@@ -8,8 +8,10 @@ namespace rv {
 
 namespace {
 
-// One warp per (token, query head): out = sum_i 2^(l_i - max) o_i / sum_i 2^(l_i - max).  A token without any
-// item sees no key: zeros and -inf.
+// One warp per (token, query head): out = sum_i 2^(l_i - max) o_i / sum_i 2^(l_i - max) over the partials with any
+// weight.  A partial without has l = -inf, and o = 0 where it has no key for the row, NaN where it has (scores of -inf
+// only); a partial with a NaN among its scores has l = NaN and so makes the row.  A row without any weight gets the sum
+// of its o: zeros, or NaN as a softmax of -inf alone; and -inf.
 template <typename T, int D>
 __global__ void __launch_bounds__(128) join_kernel(const int* __restrict__ tokens, int n, const AttendParams p) {
   constexpr int kPer = D / 32;  // values a lane
@@ -28,9 +30,10 @@ __global__ void __launch_bounds__(128) join_kernel(const int* __restrict__ token
     float mx = ls;
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
-    const float now = fmaxf(top, mx);
-    if (now == -INFINITY) continue;
-    const float old = ex2_approx(top - now), f = ex2_approx(ls - now);
+    const unsigned weighs = __ballot_sync(0xffffffffu, ls != -INFINITY);
+    if (!weighs) continue;
+    const float now = fmaxf(top, mx), ref = now == -INFINITY ? 0.f : now;
+    const float old = ex2_approx(top - ref), f = ex2_approx(ls - ref);
     top = now;
     sum *= old;
 #pragma unroll
@@ -40,6 +43,7 @@ __global__ void __launch_bounds__(128) join_kernel(const int* __restrict__ token
     const int64_t step = int64_t(p.q_heads) * 32;  // in Vec
     int i = 0;
     auto add = [&](const Vec& x, int k) {
+      if (!(weighs >> k & 1)) return;
       const float g = __shfl_sync(0xffffffffu, f, k);
       sum += g;
       const float* y = reinterpret_cast<const float*>(&x);
@@ -55,7 +59,16 @@ __global__ void __launch_bounds__(128) join_kernel(const int* __restrict__ token
     }
     for (; i < m; ++i) add(src[i * step], i);
   }
-  const float inv = sum == 0.f ? 0.f : 1.f / sum;
+  float inv = 1.f / sum;
+  if (sum == 0.f) {
+    inv = 1.f;
+    const Vec* src = reinterpret_cast<const Vec*>(p.part_o + at * D) + lane;
+    for (int i = 0; i < pt.count; ++i, src += int64_t(p.q_heads) * 32) {
+      const float* y = reinterpret_cast<const float*>(src);
+#pragma unroll
+      for (int e = 0; e < kPer; ++e) v[e] += y[e];
+    }
+  }
   T* dst = static_cast<T*>(p.out) + tok * p.out_token + head * p.out_head + lane * kPer;
   if constexpr (kPer == 4) {
     auto lo = Elem<T>::pack(v[0] * inv, v[1] * inv), hi = Elem<T>::pack(v[2] * inv, v[3] * inv);
@@ -65,7 +78,7 @@ __global__ void __launch_bounds__(128) join_kernel(const int* __restrict__ token
     *reinterpret_cast<uint32_t*>(dst) = *reinterpret_cast<uint32_t*>(&x);
   }
   if (p.lse && lane == 0)
-    p.lse[int64_t(tok) * p.q_heads + head] = sum == 0.f ? -INFINITY : (top + log2f(sum)) * 0.6931471805599453f;
+    p.lse[int64_t(tok) * p.q_heads + head] = (top + log2f(sum)) * 0.6931471805599453f;
 }
 
 template <typename T>

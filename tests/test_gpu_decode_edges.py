@@ -4,8 +4,10 @@ near the largest, streams and pages that are shared.
 Tolerances as in the tests of the operators' formulas: u is the unit roundoff of the 16-bit type; an output is rounded
 once, every softmax weight once, and f32 scores are off by at most 2^-20 sum |q k| scale."""
 
+import math
+
 import pytest
-from test_gpu_decode import Batch
+from test_gpu_decode import UNIT, Batch
 
 pytestmark = pytest.mark.gpu
 
@@ -14,6 +16,122 @@ def _torch():
     import torch
 
     return torch
+
+
+# ------------------------------------------------------------------ values
+# (what the step is, and which kernels take it)
+STEPS = [
+    dict(q=(1, 1, 2), own=(5, 200, 64), prefix=(0,)),                            # few rows, one part
+    dict(q=(1, 1), own=(6000, 3), prefix=(0,)),                                  # few rows, cut keys, join
+    dict(q=(1, 1, 2), own=(5, 200, 64), prefix=(300,)),                          # few rows, shared prefix, join
+    dict(q=(200,), own=(260,), prefix=(0,)),                                     # row tiles, whole
+    dict(q=(70, 90), own=(70, 133), prefix=(300,), hq=12, hkv=4, d=64, page=32),  # row tiles behind a prefix
+    dict(q=(150,), own=(6000,), prefix=(0,), page=128),                          # row tiles, cut keys, join
+    dict(q=(1,) * 48, own=tuple(1 + 7 * i for i in range(48)), prefix=(3000,)),  # packed prefix, few-row own keys, join
+]
+
+
+def softmax64(b, scale):
+    """out, its tolerance, lse and its tolerance by a softmax in 64 bits, NaN and infinities as they come: zeros and
+    -inf for a row that sees no key."""
+    torch = _torch()
+    g, u = b.hq // b.hkv, UNIT[b.act]
+    out = torch.zeros(b.t, b.hq, b.d, dtype=torch.float64, device="cuda")
+    tol = torch.zeros_like(out)
+    lse = torch.full((b.t, b.hq), -math.inf, dtype=torch.float64, device="cuda")
+    lse_tol = torch.zeros_like(lse)
+    t0 = 0
+    for i, n in enumerate(b.q_lens):
+        k, v = (b.keys(x, i).repeat_interleave(g, 0) for x in (b.k, b.v))
+        keys = k.shape[1]
+        if n and keys:
+            q = b.queries[t0:t0 + n].double().transpose(0, 1)
+            at = torch.arange(keys, device="cuda")
+            seen = at[None, :] <= keys - n + torch.arange(n, device="cuda")[:, None]
+            assert seen.any(-1).all()
+            s = (q @ k.transpose(1, 2) * scale).masked_fill(~seen, -math.inf)
+            off = (q.abs() @ k.abs().transpose(1, 2)).masked_fill(~seen, 0).nan_to_num(0, 0, 0).amax(-1) * scale * 2.0 ** -20
+            p = s.softmax(-1)
+            o, a = p @ v, p @ v.abs()
+            e = u * o.abs() + (u + 2.0 ** -16 + 2 * off[..., None]) * a
+            if b.act == "f16":
+                e = e + 2.0 ** -25 * keys * v.abs().nan_to_num(0).max()
+            out[t0:t0 + n], tol[t0:t0 + n] = o.transpose(0, 1), e.transpose(0, 1) + 1e-7
+            l = s.logsumexp(-1)
+            l = l.masked_fill(l == math.inf, math.nan)  # as its row is
+            lse[t0:t0 + n] = l.T
+            lse_tol[t0:t0 + n] = (off + 2.0 ** -20 * (1 + l.abs().nan_to_num(0, 0, 0))).T
+        t0 += n
+    return out, tol, lse, lse_tol
+
+
+def agree(b):
+    torch = _torch()
+    scale = b.d ** -0.5
+    lse = torch.full((b.t, b.hq), 7.0, device="cuda")
+    got = b.step.attend(b.cache, b.queries, lse=lse)
+    torch.cuda.synchronize()
+    ref, tol, ref_lse, lse_tol = softmax64(b, scale)
+    for name, x, r, e in (("out", got, ref, tol), ("lse", lse, ref_lse, lse_tol)):
+        assert torch.equal(x.isnan(), r.isnan()), f"{name}: {int(x.isnan().sum())} NaN, expected {int(r.isnan().sum())}"
+        low = r == -math.inf
+        assert (x[low] == -math.inf).all(), name
+        fine = r.isfinite()
+        assert ((x.double() - r).abs()[fine] <= e[fine]).all(), name
+    return got, ref
+
+
+def slot(b, seq, key):
+    """Page and slot of an own key of a sequence."""
+    return b.own_pages[seq][key // b.page], key % b.page
+
+
+@pytest.mark.parametrize("act", ["bf16", "f16"])
+@pytest.mark.parametrize("step", range(len(STEPS)))
+def test_attend_keeps_nan(cuda_device, act, step):
+    """NaN in a query, in a key or in a value that a row sees makes what a softmax makes of it, in every kernel and join."""
+    for what in ("query", "own key", "last key", "prefix key", "value"):
+        b = Batch(act=act, seed=40 + step, **STEPS[step])
+        if what == "query":
+            b.queries[0, 0, 5] = math.nan
+            b.queries[b.t - 1] = math.nan
+        elif what == "own key":  # one that all of the sequence's queries see
+            p, s = slot(b, 0, 0)
+            if b.q_lens[0] > 1 or b.own_lens[0] == 1:
+                b.k[p, 0, s, 3] = math.nan
+            else:
+                b.k[p, :, s] = math.nan
+        elif what == "last key":  # one that its last query sees
+            p, s = slot(b, len(b.q_lens) - 1, b.own_lens[-1] - 1)
+            b.k[p, 0, s, 0] = math.nan
+        elif b.prefix_lens[0] == 0:
+            continue
+        elif what == "prefix key":
+            b.k[b.prefix_pages[0][2 // b.page], 1, 2 % b.page, 1] = math.nan
+        else:
+            b.v[b.prefix_pages[0][0], 0, 1, 7] = math.nan
+        got, ref = agree(b)
+        assert ref.isnan().any()
+        assert what != "last key" or ref.isfinite().any() or b.t == 1
+
+
+@pytest.mark.parametrize("act", ["bf16", "f16"])
+@pytest.mark.parametrize("step", range(len(STEPS)))
+def test_attend_with_infinite_scores(cuda_device, act, step):
+    """Scores of -inf have no weight beside others, make NaN alone; a score of inf makes NaN."""
+    torch = _torch()
+    for what in ("one key", "prefix", "all"):
+        b = Batch(act=act, seed=50 + step, **STEPS[step])
+        if what == "one key":
+            p, s = slot(b, 0, 0)
+            b.k[p, :, s, 0] = math.inf  # scores of either sign
+        else:
+            b.queries[..., 0] = -1.0
+            for pages, n in zip(b.prefix_pages + b.own_pages * (what == "all"), b.prefix_lens + b.own_lens * (what == "all")):
+                for i, p in enumerate(pages):
+                    b.k[p, :, : min(b.page, n - i * b.page), 0] = math.inf
+        got, ref = agree(b)
+        assert ref.isnan().all() if what == "all" else ref.isfinite().any()
 
 
 # ------------------------------------------------------------------ streams
