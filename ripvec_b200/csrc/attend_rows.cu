@@ -400,18 +400,17 @@ __global__ void __launch_bounds__(kThreads, kPerSm<D>) attend_rows_kernel(const 
       const float inv = 1.f / sum;
 #pragma unroll
       for (int e = 0; e < 8; ++e) v[e] = sees ? v[e] * inv : 0.f;
-      const float ls = top + log2f(sum);
       const int tok = it.tok0 + r / p.fold, head = hg * p.fold + r % p.fold;
       const StepParts pt = pc.parts[r / p.fold];
       if (pt.count == 1) {
         *reinterpret_cast<uint4*>(static_cast<T*>(p.out) + tok * p.out_token + head * p.out_head + d) = pack8<T>(v);
-        if (p.lse && d == 0) p.lse[int64_t(tok) * p.q_heads + head] = ls * 0.6931471805599453f;
+        if (p.lse && d == 0) p.lse[int64_t(tok) * p.q_heads + head] = (top + log2f(sum)) * 0.6931471805599453f;
       } else {
         const int64_t at = int64_t(pt.first + it.part) * p.q_heads + head;
         float4* dst = reinterpret_cast<float4*>(p.part_o + at * D + d);
         dst[0] = make_float4(v[0], v[1], v[2], v[3]);
         dst[1] = make_float4(v[4], v[5], v[6], v[7]);
-        if (d == 0) p.part_l[at] = ls;
+        if (d == 0) p.part_ml[at] = make_float2(top, sum);
       }
     }
     consumers_or(false);  // read before the next piece's results are written, and this piece's place is used again

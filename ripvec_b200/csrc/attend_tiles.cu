@@ -522,14 +522,14 @@ __global__ void __launch_bounds__(kThreads, 1) attend_tiles_kernel(const __grid_
       uint8_t *dst = nullptr, *part = nullptr;
       if (fin_live) {
         const StepParts pt = p.parts ? p.parts[fin_tok] : StepParts{0, 1};
-        const float ls = none ? -INFINITY : fin_m + log2f(fin_l);
         if (pt.count == 1) {
           dst = reinterpret_cast<uint8_t*>(static_cast<T*>(p.out) + fin_tok * p.out_token + fin_head * p.out_head);
-          if (p.lse) p.lse[int64_t(fin_tok) * p.q_heads + fin_head] = ls * 0.6931471805599453f;
+          if (p.lse)
+            p.lse[int64_t(fin_tok) * p.q_heads + fin_head] = none ? -INFINITY : (fin_m + log2f(fin_l)) * 0.6931471805599453f;
         } else {
           const int64_t at = int64_t(pt.first + fin_part) * p.q_heads + fin_head;
           part = reinterpret_cast<uint8_t*>(p.part_o + at * D);
-          p.part_l[at] = ls;
+          p.part_ml[at] = make_float2(fin_m, none ? 0.f : fin_l);
         }
       }
       if (__any_sync(0xffffffffu, dst != nullptr)) {

@@ -529,7 +529,7 @@ int plan(rv_step* s, int32_t n_seqs, const int32_t* q_lens, const int32_t* own_l
   const size_t o_tiles = place_of(sc.tile_items.size() * sizeof(rv::StepItem));
   const size_t o_joined = place_of(sc.joined.size() * sizeof(int));
   const size_t o_pages = place_of(pg.size() * sizeof(int));
-  const size_t floats = size_t(sc.n_parts) * size_t(s->q_heads) * size_t(s->head_dim + 1);
+  const size_t floats = size_t(sc.n_parts) * size_t(s->q_heads) * size_t(s->head_dim + 2);
 
   // Small plans, those of decoding steps, are copied from pinned memory and leave the host at once.  The records of
   // long prompts come from pageable memory, which the copy takes over before it returns: pinned memory for them takes
@@ -768,7 +768,7 @@ int rv_step_attend(rv_step* s, const rv_kv_cache* cache, const void* q, int64_t 
     a.n_tokens = s->n_tokens;
     a.fold = s->fold;
     a.part_o = s->work;
-    a.part_l = s->work + s->n_parts * s->q_heads * s->head_dim;
+    a.part_ml = reinterpret_cast<float2*>(s->work + s->n_parts * s->q_heads * s->head_dim);
     a.num_pages = cache->num_pages;
     a.err = s->err_dev;
     a.counter = s->counter;

@@ -78,7 +78,7 @@ struct AttendArgs {
   int64_t out_token, out_head;
   float* lse;     // [tokens, q_heads] or null
   float* part_o;  // [partials, q_heads, head_dim] results of items, divided by their own sums
-  float* part_l;  // [partials, q_heads] log2 of the sums (-inf: no key)
+  float2* part_ml;  // [partials, q_heads] reference exponents m and sums l of 2^(score - m) (0: no weight)
   KvPool pool;
   int64_t num_pages;
   float scale;

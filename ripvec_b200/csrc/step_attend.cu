@@ -8,10 +8,11 @@ namespace rv {
 
 namespace {
 
-// One warp per (token, query head): out = sum_i 2^(l_i - max) o_i / sum_i 2^(l_i - max) over the partials with any
-// weight.  A partial without has l = -inf, and o = 0 where it has no key for the row, NaN where it has (scores of -inf
+// One warp per (token, query head): out = sum_i w_i o_i / sum_i w_i with w_i = l_i 2^(m_i - max), over the partials with
+// any weight.  A partial without has l = 0, and o = 0 where it has no key for the row, NaN where it has (scores of -inf
 // only); a partial with a NaN among its scores has l = NaN and so makes the row.  A row without any weight gets the sum
-// of its o: zeros, or NaN as a softmax of -inf alone; and -inf.
+// of its o: zeros, or NaN as a softmax of -inf alone; and -inf.  (The logarithm of a weight, m + log2 l, would lose l
+// beside a large m: of scores of 2^20 four bits of it are left.)
 template <typename T, int D>
 __global__ void __launch_bounds__(128) join_kernel(const int* __restrict__ tokens, int n, const AttendParams p) {
   constexpr int kPer = D / 32;  // values a lane
@@ -26,14 +27,14 @@ __global__ void __launch_bounds__(128) join_kernel(const int* __restrict__ token
   // Up to 32 partials at a time: one lane weighs each, all lanes add them, four loads in flight.
   float v[kPer] = {}, sum = 0.f, top = -INFINITY;
   for (int i0 = 0; i0 < pt.count; i0 += 32) {
-    const float ls = i0 + lane < pt.count ? p.part_l[at + int64_t(i0 + lane) * p.q_heads] : -INFINITY;
-    float mx = ls;
+    const float2 ml = i0 + lane < pt.count ? p.part_ml[at + int64_t(i0 + lane) * p.q_heads] : make_float2(-INFINITY, 0.f);
+    float mx = ml.y == 0.f ? -INFINITY : ml.x;
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
-    const unsigned weighs = __ballot_sync(0xffffffffu, ls != -INFINITY);
+    const unsigned weighs = __ballot_sync(0xffffffffu, ml.y != 0.f);
     if (!weighs) continue;
     const float now = fmaxf(top, mx), ref = now == -INFINITY ? 0.f : now;
-    const float old = ex2_approx(top - ref), f = ex2_approx(ls - ref);
+    const float old = ex2_approx(top - ref), f = ml.y * ex2_approx(ml.x - ref);
     top = now;
     sum *= old;
 #pragma unroll
@@ -115,7 +116,7 @@ cudaError_t step_attend(Act act, const AttendArgs& a, cudaStream_t st) {
   p.out_head = a.out_head;
   p.lse = a.lse;
   p.part_o = a.part_o;
-  p.part_l = a.part_l;
+  p.part_ml = a.part_ml;
   p.scale_log2 = a.scale * 1.4426950408889634f;
   p.err = a.err;
   p.counter = a.counter;

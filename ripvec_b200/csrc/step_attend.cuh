@@ -20,7 +20,8 @@ struct AttendParams {
   int page_size, box;                  // box: keys of one page copy
   void* out;
   int64_t out_token, out_head;
-  float *lse, *part_o, *part_l;
+  float *lse, *part_o;
+  float2* part_ml;
   float scale_log2;
   unsigned int* err;
   int* counter;  // [2] of the few-row kernel: work taken, CTAs done; 0 between launches

@@ -31,9 +31,9 @@ STEPS = [
 ]
 
 
-def softmax64(b, scale):
+def softmax64(b, scale, exact_scores=False):
     """out, its tolerance, lse and its tolerance by a softmax in 64 bits, NaN and infinities as they come: zeros and
-    -inf for a row that sees no key."""
+    -inf for a row that sees no key.  exact_scores: the f32 scores have no error."""
     torch = _torch()
     g, u = b.hq // b.hkv, UNIT[b.act]
     out = torch.zeros(b.t, b.hq, b.d, dtype=torch.float64, device="cuda")
@@ -51,6 +51,8 @@ def softmax64(b, scale):
             assert seen.any(-1).all()
             s = (q @ k.transpose(1, 2) * scale).masked_fill(~seen, -math.inf)
             off = (q.abs() @ k.abs().transpose(1, 2)).masked_fill(~seen, 0).nan_to_num(0, 0, 0).amax(-1) * scale * 2.0 ** -20
+            if exact_scores:
+                off = off * 0
             p = s.softmax(-1)
             o, a = p @ v, p @ v.abs()
             e = u * o.abs() + (u + 2.0 ** -16 + 2 * off[..., None]) * a
@@ -65,13 +67,13 @@ def softmax64(b, scale):
     return out, tol, lse, lse_tol
 
 
-def agree(b):
+def agree(b, exact_scores=False):
     torch = _torch()
     scale = b.d ** -0.5
     lse = torch.full((b.t, b.hq), 7.0, device="cuda")
     got = b.step.attend(b.cache, b.queries, lse=lse)
     torch.cuda.synchronize()
-    ref, tol, ref_lse, lse_tol = softmax64(b, scale)
+    ref, tol, ref_lse, lse_tol = softmax64(b, scale, exact_scores)
     for name, x, r, e in (("out", got, ref, tol), ("lse", lse, ref_lse, lse_tol)):
         assert torch.equal(x.isnan(), r.isnan()), f"{name}: {int(x.isnan().sum())} NaN, expected {int(r.isnan().sum())}"
         low = r == -math.inf
@@ -132,6 +134,25 @@ def test_attend_with_infinite_scores(cuda_device, act, step):
                     b.k[p, :, : min(b.page, n - i * b.page), 0] = math.inf
         got, ref = agree(b)
         assert ref.isnan().all() if what == "all" else ref.isfinite().any()
+
+
+@pytest.mark.parametrize("act,power", [("bf16", 10), ("bf16", 13), ("bf16", 15), ("bf16", 30), ("f16", 10),
+                                       ("f16", 12), ("f16", 14), ("f16", 15)])
+@pytest.mark.parametrize("sign", [1, -1])
+@pytest.mark.parametrize("step", range(len(STEPS)))
+def test_attend_with_large_scores(cuda_device, act, power, sign, step):
+    """Scores far beyond the range of exponents, as keys of a type's largest or lowest values make them: all powers of
+    two, so that the f32 scores are exact, and the weights are those of the largest score's keys alone."""
+    torch = _torch()
+    b = Batch(act=act, seed=60 + step, **STEPS[step])
+    b.queries.fill_(sign * 2.0 ** power)
+    for pages, n in zip(b.prefix_pages + b.own_pages, b.prefix_lens + b.own_lens):
+        for i, p in enumerate(pages):
+            fill = min(b.page, n - i * b.page)
+            at = i * b.page + torch.arange(fill, device="cuda")
+            size = torch.where(at % 7 == 4, 2.0 ** (power - 1), 2.0 ** power)
+            b.k[p, :, :fill] = size[None, :, None].to(b.k.dtype)
+    agree(b, exact_scores=True)
 
 
 # ------------------------------------------------------------------ streams
