@@ -308,7 +308,7 @@ __global__ void __launch_bounds__(kThreads, kPerSm<D>) attend_rows_kernel(const 
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
               float& v = x[n][2 * i + e];
-              v = 8 * n + e < top ? v * p.scale_log2 : -INFINITY;
+              v = 8 * n + e < top ? __fmul_rn(v, p.scale_log2) : -INFINITY;  // (rounded, as m is)
               mx = fmaxf(mx, v);
             }
           mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));

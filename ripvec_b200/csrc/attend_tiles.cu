@@ -21,6 +21,7 @@
 // that item's first P V.  A causal prompt of 8192 tokens, 32 query and 8 key/value heads of 128: 490 us, 1120
 // TFLOP/s, in a short burst.
 #include <algorithm>
+#include <cfloat>
 
 #include "step_attend.cuh"
 
@@ -492,7 +493,12 @@ __global__ void __launch_bounds__(kThreads, 1) attend_tiles_kernel(const __grid_
     const uint32_t to = tmem + lanes + 256 + i * 128;
     const int my_tok = i * per + r / p.fold, my_head = r % p.fold;
     constexpr float kRescale = 8.f;  // P stays below 2^8
-    constexpr float kNone = -1e30f;  // no key seen yet
+    constexpr float kNone = -FLT_MAX;  // no key seen yet, or scores of -inf only
+    // Beyond this m, s * scale - m is taken of the rounded product, as m is one: fused it leaves at the largest score
+    // what m lost in its rounding, up to 2^-12 here but beyond the range of 2^x for scores of 2^28 and more.  (Never
+    // fused: the products apart are one more instruction a pair.  Packed ones would not do: the compiler joins
+    // mul.rn.f32x2 and add.rn.f32x2 to a fused one.)
+    constexpr float kBig = 4096.f;
     const uint64_t sl2 = f2_pack(p.scale_log2, p.scale_log2);
     Walk wk;
     wk.init(p, total);
@@ -607,28 +613,36 @@ __global__ void __launch_bounds__(kThreads, 1) attend_tiles_kernel(const __grid_
 #pragma unroll
           for (int e = 12; e < 64; e += 2) mx[e / 2 % 6] = fmax3(mx[e / 2 % 6], s[e], s[e + 1]);
           mt = fmaxf(fmax3(mx[0], mx[1], mx[2]), fmax3(mx[3], mx[4], mx[5]));
-          mt *= p.scale_log2;
+          mt = __fmul_rn(mt, p.scale_log2);  // (m - mt below is not to be fused either)
           const bool need = m != kNone && mt > m + kRescale;
           if (m == kNone) m = fmaxf(m, mt);
-          if (__any_sync(0xffffffffu, need)) {
-            // The P V before is done, and this half's has not been issued.
-            fail = !__all_sync(0xffffffffu, mbar_wait_spin(&pv_done[2 * i + (h ^ 1)], t_ph ^ (h ^ 1), abort_flag));
-            if (fail) break;
-            tc_fence_after();
-            const float alpha = need ? ex2_approx(m - mt) : 1.f;
+          uint64_t mul = sl2;
+          if (__any_sync(0xffffffffu, need || (m != kNone && fabsf(m) > kBig))) {
+            if (__any_sync(0xffffffffu, need)) {
+              // The P V before is done, and this half's has not been issued.
+              fail = !__all_sync(0xffffffffu, mbar_wait_spin(&pv_done[2 * i + (h ^ 1)], t_ph ^ (h ^ 1), abort_flag));
+              if (fail) break;
+              tc_fence_after();
+              const float alpha = need ? ex2_approx(m - mt) : 1.f;
 #pragma unroll
-            for (int c = 0; c < D / 16; ++c) {
-              float o[16];
-              tmem_read(to + 16 * c, o);
-              uint32_t w[16];
+              for (int c = 0; c < D / 16; ++c) {
+                float o[16];
+                tmem_read(to + 16 * c, o);
+                uint32_t w[16];
 #pragma unroll
-              for (int e = 0; e < 16; ++e) w[e] = __float_as_uint(o[e] * alpha);
-              tmem_st16(to + 16 * c, w);
+                for (int e = 0; e < 16; ++e) w[e] = __float_as_uint(o[e] * alpha);
+                tmem_st16(to + 16 * c, w);
+              }
+              tc_wait_st();
+              if (need) {
+                l *= alpha;
+                m = mt;
+              }
             }
-            tc_wait_st();
-            if (need) {
-              l *= alpha;
-              m = mt;
+            if (__any_sync(0xffffffffu, m != kNone && fabsf(m) > kBig)) {
+#pragma unroll
+              for (int e = 0; e < 64; ++e) s[e] = __fmul_rn(s[e], p.scale_log2);
+              mul = f2_pack(1.f, 1.f);
             }
           }
           const uint64_t nm2 = f2_pack(-m, -m);
@@ -638,7 +652,7 @@ __global__ void __launch_bounds__(kThreads, 1) attend_tiles_kernel(const __grid_
             uint32_t w[16];
 #pragma unroll
             for (int e = 0; e < 16; ++e) {
-              const uint64_t x = f2_fma(f2_pack(s[32 * c + 2 * e], s[32 * c + 2 * e + 1]), sl2, nm2);
+              const uint64_t x = f2_fma(f2_pack(s[32 * c + 2 * e], s[32 * c + 2 * e + 1]), mul, nm2);
               float p0, p1;
               uint64_t pair;
               if ((e & 3) == 3) {

@@ -28,6 +28,7 @@ STEPS = [
     dict(q=(70, 90), own=(70, 133), prefix=(300,), hq=12, hkv=4, d=64, page=32),  # row tiles behind a prefix
     dict(q=(150,), own=(6000,), prefix=(0,), page=128),                          # row tiles, cut keys, join
     dict(q=(1,) * 48, own=tuple(1 + 7 * i for i in range(48)), prefix=(3000,)),  # packed prefix, few-row own keys, join
+    dict(q=(1, 1, 2), own=(5, 200, 64), prefix=(300,), hq=12, hkv=4, d=64, page=32),  # few rows of 64 values, join
 ]
 
 
@@ -153,6 +154,24 @@ def test_attend_with_large_scores(cuda_device, act, power, sign, step):
             size = torch.where(at % 7 == 4, 2.0 ** (power - 1), 2.0 ** power)
             b.k[p, :, :fill] = size[None, :, None].to(b.k.dtype)
     agree(b, exact_scores=True)
+
+
+@pytest.mark.parametrize("act,power", [("bf16", 10), ("bf16", 13), ("bf16", 15), ("bf16", 30), ("bf16", 50), ("f16", 10),
+                                       ("f16", 12), ("f16", 14), ("f16", 15)])
+@pytest.mark.parametrize("step", range(len(STEPS)))
+def test_attend_with_large_inexact_scores(cuda_device, act, power, step):
+    """As before with scores that the factor of the exponent rounds (1.5 times a power of two, and 0.75)."""
+    torch = _torch()
+    for sign in (1, -1):
+        b = Batch(act=act, seed=90 + step, **STEPS[step])
+        b.queries.fill_(sign * 2.0 ** power)
+        for pages, n in zip(b.prefix_pages + b.own_pages, b.prefix_lens + b.own_lens):
+            for i, p in enumerate(pages):
+                fill = min(b.page, n - i * b.page)
+                at = i * b.page + torch.arange(fill, device="cuda")
+                size = torch.where(at % 7 == 4, 0.75 * 2.0 ** power, 1.5 * 2.0 ** power)
+                b.k[p, :, :fill] = size[None, :, None].to(b.k.dtype)
+        agree(b, exact_scores=True)
 
 
 # ------------------------------------------------------------------ streams
