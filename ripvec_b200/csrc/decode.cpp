@@ -52,7 +52,6 @@ bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 
 struct StepSeq {
   int tok0, n, pg_a, len_a, pg_b, len_b, diag;
 };
-
 // The attention work of a plan.
 struct Schedule {
   std::vector<rv::StepItem> row_items, tile_items;
@@ -323,7 +322,7 @@ void schedule(const std::vector<StepSeq>& seqs, const std::vector<int>& group_fi
     it.pg_a = s.pg_a;
     it.a1 = prefix ? s.len_a : 0;
     it.pg_b = s.pg_b;
-    it.b1 = own ? std::max(0, std::min<int>(s.len_b, int(std::min<int64_t>(INT_MAX / 2, int64_t(diag) + n)))) : 0;
+    it.b1 = own ? int(std::max<int64_t>(0, std::min<int64_t>(s.len_b, int64_t(diag) + n))) : 0;
     it.diag = diag;
     if (it.a1 == 0 && it.b1 == 0) return;
     (to_rows ? rows : tiles).push_back({it, packed});

@@ -174,6 +174,32 @@ def test_attend_with_large_inexact_scores(cuda_device, act, power, step):
         agree(b, exact_scores=True)
 
 
+# ------------------------------------------------------------------ lengths
+@pytest.mark.parametrize("causal", [True, False])
+def test_attend_the_most_keys(cuda_device, causal):
+    """2^30 keys, the most that a sequence may have: the last one counts."""
+    import numpy as np
+
+    torch = _torch()
+    from ripvec_b200.decode import DecodeStep, PagedCache
+
+    keys, ps, d = 2 ** 30, 256, 64
+    k = torch.zeros(2, 1, ps, d, dtype=torch.bfloat16, device="cuda")
+    v = torch.zeros_like(k)
+    k[1, 0, -1, 0] = 320.0
+    v[1, 0, -1] = torch.randn(d, generator=torch.Generator(device="cuda").manual_seed(71), device="cuda").to(k.dtype)
+    q = torch.zeros(1, 1, d, dtype=k.dtype, device="cuda")
+    q[..., 0] = 1.0  # a score of 40 for the last key, 0 for the others
+    pages = np.zeros((1, keys // ps), np.int32)
+    pages[0, -1] = 1
+    step = DecodeStep(q_heads=1, kv_heads=1, head_dim=d, page_size=ps)
+    step.plan(q_lens=[1], own_lens=[keys], own_pages=pages, num_pages=2, causal=causal)
+    got = step.attend(PagedCache(k, v), q)[0, 0].double()
+    w = math.exp(40.0)
+    ref = v[1, 0, -1].double() * w / (w + keys - 1)
+    assert ((got - ref).abs() <= (2.0 ** -7 + 2.0 ** -16) * ref.abs()).all()
+
+
 # ------------------------------------------------------------------ streams
 @pytest.mark.parametrize("kw", [dict(q=(1,) * 30, own=(3000,) * 30, prefix=(4000,)), dict(q=(1, 2), own=(9000, 40))])
 def test_a_step_made_beside_a_busy_default_stream(cuda_device, kw):
