@@ -52,6 +52,10 @@ bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 
 struct StepSeq {
   int tok0, n, pg_a, len_a, pg_b, len_b, diag;
 };
+// diag of a sequence that is not causal.  A causal one's is its keys less its tokens: smaller where there are two
+// tokens and more.
+constexpr int kSeesAll = kMaxKeys - 1;
+
 // The attention work of a plan.
 struct Schedule {
   std::vector<rv::StepItem> row_items, tile_items;
@@ -331,7 +335,7 @@ void schedule(const std::vector<StepSeq>& seqs, const std::vector<int>& group_fi
   auto whole = [&](const StepSeq& s, bool prefix) {
     if (s.n * fold <= rv::kRowTile) return add(true, s.tok0, s.n, s, prefix, true, s.diag, false);
     for (int t = 0; t < s.n; t += 2 * per)
-      add(false, s.tok0 + t, std::min(2 * per, s.n - t), s, prefix, true, s.diag > INT_MAX / 4 ? s.diag : s.diag + t,
+      add(false, s.tok0 + t, std::min(2 * per, s.n - t), s, prefix, true, s.diag == kSeesAll ? kSeesAll : s.diag + t,
           false);
   };
   for (size_t g = 0; g + 1 < group_first.size(); ++g) {
@@ -480,7 +484,7 @@ int plan(rv_step* s, int32_t n_seqs, const int32_t* q_lens, const int32_t* own_l
   for (int g = 0; g < n_groups; ++g) {
     for (int k = 0; k < group_sizes[g]; ++k, ++b) {
       const int n = q_lens[b], own = own_lens[b];
-      sq[b] = {t, n, int(pa), prefix_lens[g], int(pb), own, causal ? own - n : INT_MAX / 2};
+      sq[b] = {t, n, int(pa), prefix_lens[g], int(pb), own, causal ? own - n : kSeesAll};
       for (int i = 0; i < n; ++i) {
         const int place = own - n + i;  // negative only when nothing can be appended
         const int page = place >= 0 ? pg[size_t(pb + place / ps)] : 0;

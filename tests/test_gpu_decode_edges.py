@@ -175,6 +175,33 @@ def test_attend_with_large_inexact_scores(cuda_device, act, power, step):
 
 
 # ------------------------------------------------------------------ lengths
+def test_attend_causal_limits_of_very_long_sequences(cuda_device):
+    """Several row tiles of new tokens after 2^29 keys (pages may be read many times): each sees its own limit."""
+    import numpy as np
+
+    torch = _torch()
+    from ripvec_b200.decode import DecodeStep, PagedCache
+
+    past, n, ps, d = 2 ** 29, 300, 256, 64
+    k = torch.zeros(3, 1, ps, d, dtype=torch.bfloat16, device="cuda")
+    v = torch.zeros_like(k)
+    g = torch.Generator(device="cuda").manual_seed(70)
+    new_v = torch.randn(n, d, generator=g, device="cuda").to(k.dtype)
+    k.view(3 * ps, d)[ps:ps + n, 0] = 320.0
+    v.view(3 * ps, d)[ps:ps + n] = new_v
+    q = torch.zeros(n, 1, d, dtype=k.dtype, device="cuda")
+    q[..., 0] = 1.0  # scores 40 for the new tokens' keys, 0 for the others
+    pages = np.zeros((1, past // ps + 2), np.int32)
+    pages[0, -2:] = 1, 2
+    step = DecodeStep(q_heads=1, kv_heads=1, head_dim=d, page_size=ps)
+    step.plan(q_lens=[n], own_lens=[past + n], own_pages=pages, num_pages=3)
+    got = step.attend(PagedCache(k, v), q)[:, 0].double()
+    w = math.exp(40.0)
+    count = torch.arange(1, n + 1, device="cuda", dtype=torch.float64)[:, None]
+    ref, a = (x.double().cumsum(0) * w / (count * w + past) for x in (new_v, new_v.abs()))
+    assert ((got - ref).abs() <= 2.0 ** -8 * ref.abs() + (2.0 ** -8 + 2.0 ** -16) * a).all()
+
+
 @pytest.mark.parametrize("causal", [True, False])
 def test_attend_the_most_keys(cuda_device, causal):
     """2^30 keys, the most that a sequence may have: the last one counts."""
