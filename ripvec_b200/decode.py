@@ -7,7 +7,9 @@ keys and values into their pages) and ``attend`` (attention of every sequence ov
 prefix and its own keys), and ``rms_norm`` is the decoder's residual norm with 16-bit or 8-bit output.
 
 Calls queue their kernels on ``stream`` (a CUDA stream handle; by default torch's current stream) and
-return.  The reference has no decoder; there is nothing of it to cite here.
+return.  An output that a call makes itself is memory of that stream, as of a tensor made under
+``torch.cuda.stream``; tensors of other streams are the caller's to order and to keep until the work is done
+(``record_stream``).  The reference has no decoder; there is nothing of it to cite here.
 """
 
 from __future__ import annotations
@@ -33,6 +35,16 @@ _norm_args = Struct("PqPqPPqPqPqiiiidiP").pack
 
 # torch's current stream of a device as a handle, without the stream object around it.
 _current_stream = torch._C._cuda_getCurrentRawStream
+
+
+def _new(stream: int | None, like, shape: tuple, strides: tuple, dtype=None):
+    """A tensor for ``stream`` to write.  torch's allocator hands out memory in the order of the stream that is
+    current: on another one an earlier owner's reads could still be to come."""
+    if stream is None or stream == _current_stream(like.get_device()):
+        return like.new_empty_strided(shape, strides, dtype=dtype)
+    other = torch.cuda.ExternalStream(stream, like.device) if stream else torch.cuda.default_stream(like.device)
+    with torch.cuda.stream(other):
+        return like.new_empty_strided(shape, strides, dtype=dtype)
 
 
 def _rows(name: str, t, shape: tuple, cache: "PagedCache") -> tuple:
@@ -160,7 +172,7 @@ class DecodeStep:
         if q is not None:
             qa = _rows("q", q, (t, self.q_heads, d), cache)
             if q_out is None:
-                q_out = q.new_empty_strided((t, self.q_heads, d), (self.q_heads * d, d, 1))
+                q_out = _new(stream, q, (t, self.q_heads, d), (self.q_heads * d, d, 1))
             qo = _rows("q_out", q_out, (t, self.q_heads, d), cache)
         elif q_out is not None:
             raise ValueError("q_out without q")
@@ -188,7 +200,7 @@ class DecodeStep:
         shape = (t, self.q_heads, d)
         qa = _rows("q", q, shape, cache)
         if out is None:
-            out = q.new_empty_strided(shape, (self.q_heads * d, d, 1))
+            out = _new(stream, q, shape, (self.q_heads * d, d, 1))
         oa = _rows("out", out, shape, cache)
         if lse is not None and (lse.shape != shape[:2] or lse.dtype is not torch.float32
                                 or lse.get_device() != cache.device_index or not lse.is_contiguous()):
@@ -234,7 +246,7 @@ def rms_norm(x, weight, *, residual=None, residual_out=None, out=None, eps: floa
         dtype, code_out = torch.float8_e4m3fn, L.RV_DTYPE_E4M3
         per_row = hidden // group if group else 1
         if scales is None:
-            scales = weight.new_empty_strided((rows, per_row), (per_row, 1))
+            scales = _new(stream, weight, (rows, per_row), (per_row, 1))
         elif scales.shape != (rows, per_row) or scales.dtype is not torch.float32 or scales.get_device() != dev \
                 or not scales.is_contiguous():
             raise ValueError(f"scales must be a contiguous {(rows, per_row)} f32 tensor on x's device")
@@ -244,7 +256,7 @@ def rms_norm(x, weight, *, residual=None, residual_out=None, out=None, eps: floa
             raise ValueError("group and scales come with out_8bit")
         code_out, sp = code, 0
     if out is None:
-        out = x.new_empty_strided(shape, (hidden, 1), dtype=dtype)
+        out = _new(stream, x, shape, (hidden, 1), dtype)
         os = hidden
     else:
         os, u = out.stride()

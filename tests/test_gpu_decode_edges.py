@@ -249,3 +249,47 @@ def test_a_step_made_beside_a_busy_default_stream(cuda_device, kw):
     assert not torch.cuda.default_stream().query()
     torch.cuda.synchronize()
     assert all(torch.equal(o, want) for o in outs)
+
+
+@pytest.mark.parametrize("call", ["append", "attend", "norm", "norm 8 bit"])
+def test_outputs_on_a_given_stream(cuda_device, call):
+    """An output that a call makes itself is the given stream's memory: what the current stream still has to read is
+    not written."""
+    torch = _torch()
+    from ripvec_b200.decode import rms_norm
+
+    b = Batch(q=(1,) * 64, own=(40,) * 64, prefix=(100,), seed=71)
+    cos, sin = torch.ones(200, 64, device="cuda"), torch.zeros(200, 64, device="cuda")
+    kn = b.randn(b.t, b.hkv, b.d)
+    x, w = b.randn(64, 4096), torch.ones(4096, device="cuda")
+    side = torch.cuda.Stream()
+
+    def run(stream):
+        if call == "append":
+            return (b.step.append(b.cache, b.queries, kn, kn, cos, sin, stream=stream),)
+        if call == "attend":
+            return (b.step.attend(b.cache, b.queries, stream=stream),)
+        return rms_norm(x, w, out_8bit=call != "norm", stream=stream)
+
+    want = [None if y is None else y.clone() for y in run(None)]
+    torch.cuda.synchronize()
+    torch.cuda.empty_cache()
+    kept = []
+    for y in want:  # blocks that the current stream's next outputs of these sizes would get
+        if y is not None:
+            old = torch.zeros_like(y)
+            kept.append((old, torch.ones_like(y)))
+    torch.cuda.synchronize()
+    torch.cuda._sleep(400_000_000)  # a fifth of a second
+    for i, (old, copy) in enumerate(kept):
+        copy.copy_(old)
+        kept[i] = copy
+    del old
+    got = run(side.cuda_stream)
+    side.synchronize()
+    assert not torch.cuda.current_stream().query()  # the copies are still to come
+    torch.cuda.synchronize()
+    for y, z in zip(want, got):
+        assert (y is None and z is None) or torch.equal(y.view(torch.uint8), z.view(torch.uint8))
+    for copy in kept:
+        assert (copy.view(torch.uint8) == 0).all()
