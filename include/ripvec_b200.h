@@ -332,7 +332,8 @@ int rv_index_find_duplicates(rv_index* idx, float threshold, int64_t max_pairs, 
  * next call. */
 
 /* One layer's key and value pools, [num_pages, kv_heads, page_size, head_dim] in any order of memory:
- * strides in elements, unit stride along head_dim; pools and strides multiples of 16 bytes. */
+ * strides in elements, unit stride along head_dim; pools and strides multiples of 16 bytes.  On the
+ * device of the step that it is used with, as are all tensors of a call. */
 typedef struct rv_kv_cache {
   void* k;
   void* v;

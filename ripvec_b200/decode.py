@@ -105,9 +105,11 @@ class DecodeStep:
         if rc != L.RV_OK:
             raise L.RvError(rc, self._lib.rv_step_last_error(self._h).decode())
 
-    def _tokens(self) -> int:
+    def _tokens(self, cache: PagedCache) -> int:
         if self.tokens is None:
             raise L.RvError(L.RV_E_NOT_READY, "no plan")
+        if cache.device_index != self.device.index:
+            raise ValueError(f"the cache's device {cache.device} is not the step's, {self.device}")
         return self.tokens
 
     def close(self) -> None:
@@ -168,7 +170,7 @@ class DecodeStep:
         by ``cos`` / ``sin [positions, rot / 2]`` (f32) and writes keys and values into the cache; returns
         the rotated queries (``q_out``, a new tensor by default; it may be ``q``).  ``q = None`` appends
         keys and values only."""
-        t, d = self._tokens(), self.head_dim
+        t, d = self._tokens(cache), self.head_dim
         if q is not None:
             qa = _rows("q", q, (t, self.q_heads, d), cache)
             if q_out is None:
@@ -196,7 +198,7 @@ class DecodeStep:
         """``rv_step_attend``: attention of every query of the step over its group's prefix and its own keys
         (``scale`` 1 / sqrt(head_dim) by default).  ``lse [tokens, q_heads]`` f32, where given, receives the
         log of the softmax's denominator.  Returns ``out [tokens, q_heads, head_dim]``."""
-        t, d = self._tokens(), self.head_dim
+        t, d = self._tokens(cache), self.head_dim
         shape = (t, self.q_heads, d)
         qa = _rows("q", q, shape, cache)
         if out is None:

@@ -131,3 +131,60 @@ def test_null_and_bad_records_are_refused():
     assert norm_record(1e-5, rows=0) == L.RV_OK
     for eps in (-1.0, math.nan, math.inf, 1e300, -1e300):
         assert norm_record(eps) == L.RV_E_INVALID
+
+
+class OnDevice:
+    """As much of a CUDA tensor as the checks look at."""
+
+    def __init__(self, shape, dtype, device):
+        import torch
+
+        self.shape, self.dtype, self.ndim, self.device = torch.Size(shape), dtype, len(shape), f"cuda:{device}"
+        self._device = device
+
+    def get_device(self):
+        return self._device
+
+    def stride(self):
+        out, n = [], 1
+        for d in reversed(self.shape):
+            out.append(n)
+            n *= d
+        return tuple(reversed(out))
+
+    def is_contiguous(self):
+        return True
+
+    def data_ptr(self):
+        return 4096
+
+
+@pytest.mark.parametrize("cache_device,step_device", [(1, 0), (0, 1)])
+def test_a_cache_of_another_device_is_refused(monkeypatch, cache_device, step_device):
+    """Nothing reaches the library: it would launch on the step's device with the other one's addresses."""
+    from types import SimpleNamespace
+
+    import torch
+
+    import ripvec_b200.decode as D
+
+    calls = []
+    fake = SimpleNamespace(rv_step_append_record=lambda *a: calls.append(a) or 0,
+                           rv_step_attend_record=lambda *a: calls.append(a) or 0, rv_step_destroy=lambda h: None)
+    monkeypatch.setattr(D, "_current_stream", lambda device: 0)
+    step = object.__new__(D.DecodeStep)
+    step._lib, step._h, step.tokens = fake, 1, 2
+    step.q_heads, step.kv_heads, step.head_dim, step.page_size = 8, 2, 64, 16
+    step.device = torch.device("cuda", step_device)
+    for device, refused in ((step_device, False), (cache_device, True)):
+        cache = SimpleNamespace(dtype=torch.bfloat16, device=f"cuda:{device}", device_index=device, _ref=4096)
+        q, out = (OnDevice((2, 8, 64), torch.bfloat16, device) for _ in range(2))
+        k = OnDevice((2, 2, 64), torch.bfloat16, device)
+        cos = OnDevice((9, 32), torch.float32, device)
+        for run in (lambda: step.append(cache, q, k, k, cos, cos, q_out=out), lambda: step.attend(cache, q, out=out)):
+            if refused:
+                with pytest.raises(ValueError, match="device"):
+                    run()
+            else:
+                run()
+        assert len(calls) == 2
