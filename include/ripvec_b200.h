@@ -328,7 +328,8 @@ int rv_index_find_duplicates(rv_index* idx, float threshold, int64_t max_pairs, 
  * serves every layer.  rv_step_append, rv_step_attend and rv_rms_norm queue their kernels on `stream`
  * (0 = the legacy default stream) and return; the tensors they are given must be ready in that
  * stream's order.  Calls on one step from different streams are ordered by the library, except while
- * a stream is being captured.  A kernel that gave up waiting (RV_E_DEVICE) is reported by the step's
+ * a stream is being captured; replays of captured calls, too, are the caller's to order against one
+ * another and against every other call on their step.  A kernel that gave up waiting (RV_E_DEVICE) is reported by the step's
  * next call. */
 
 /* One layer's key and value pools, [num_pages, kv_heads, page_size, head_dim] in any order of memory:

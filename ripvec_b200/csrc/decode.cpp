@@ -106,7 +106,7 @@ struct rv_step {
   // Calls on different streams wait for one another: plan, append and attend share the plan's device
   // records and the workspace.
   cudaEvent_t last = nullptr;
-  cudaStream_t last_stream = nullptr;
+  unsigned long long last_stream = 0;  // its id: a handle may stand for one stream a thread, or for a later stream
   bool used = false;
 };
 
@@ -143,13 +143,17 @@ bool capturing(cudaStream_t st) {
 // Makes st wait for this step's earlier work on another stream.  Under stream capture the order is the
 // caller's: an event of uncaptured work cannot be waited for there.
 cudaError_t enter(rv_step* s, cudaStream_t st) {
-  if (!s->used || st == s->last_stream || capturing(st)) return cudaSuccess;
-  return cudaStreamWaitEvent(st, s->last, 0);
+  if (!s->used || capturing(st)) return cudaSuccess;
+  unsigned long long id = 0;
+  const cudaError_t e = cudaStreamGetId(st, &id);
+  if (e != cudaSuccess) return e;
+  return id == s->last_stream ? cudaSuccess : cudaStreamWaitEvent(st, s->last, 0);
 }
 cudaError_t leave(rv_step* s, cudaStream_t st) {
   if (capturing(st)) return cudaSuccess;
+  const cudaError_t e = cudaStreamGetId(st, &s->last_stream);
+  if (e != cudaSuccess) return e;
   s->used = true;
-  s->last_stream = st;
   return cudaEventRecord(s->last, st);
 }
 

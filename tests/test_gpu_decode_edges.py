@@ -293,3 +293,66 @@ def test_outputs_on_a_given_stream(cuda_device, call):
         assert (y is None and z is None) or torch.equal(y.view(torch.uint8), z.view(torch.uint8))
     for copy in kept:
         assert (copy.view(torch.uint8) == 0).all()
+
+
+def test_one_handle_for_a_stream_of_each_thread(cuda_device):
+    """cudaStreamPerThread is one handle and, in each host thread, another stream: a call waits for the step's earlier
+    call of another thread."""
+    import threading
+    import time
+
+    torch = _torch()
+    b = Batch(q=(1,) * 30, own=(3000,) * 30, prefix=(4000,), seed=74)
+    want = b.step.attend(b.cache, b.queries)
+    outs = [torch.zeros_like(want) for _ in range(2)]
+    done = [torch.cuda.Event() for _ in range(2)]
+    torch.cuda.synchronize()
+    queued, checked = threading.Event(), threading.Event()
+
+    def first():
+        with torch.cuda.stream(torch.cuda.ExternalStream(2)):
+            torch.cuda._sleep(1_000_000_000)  # half a second
+            b.step.attend(b.cache, b.queries, out=outs[0])
+            done[0].record()
+        queued.set()
+        checked.wait(60)
+
+    thread = threading.Thread(target=first)
+    thread.start()
+    assert queued.wait(60)
+    with torch.cuda.stream(torch.cuda.ExternalStream(2)):
+        b.step.attend(b.cache, b.queries, out=outs[1])
+        done[1].record()
+    time.sleep(0.1)
+    late = done[1].query()
+    busy = not done[0].query()
+    checked.set()
+    thread.join()
+    torch.cuda.synchronize()
+    assert busy and not late
+    assert all(torch.equal(o, want) for o in outs)
+
+
+def test_one_step_in_many_threads(cuda_device):
+    """Threads that call one step, each on a stream of its own."""
+    import threading
+
+    torch = _torch()
+    b = Batch(q=(1,) * 30, own=(300,) * 30, prefix=(4000,), seed=75)
+    want = b.step.attend(b.cache, b.queries)
+    torch.cuda.synchronize()
+    wrong = []
+
+    def work():
+        stream = torch.cuda.Stream()
+        with torch.cuda.stream(stream):
+            outs = [b.step.attend(b.cache, b.queries) for _ in range(20)]
+        stream.synchronize()
+        wrong.extend(1 for o in outs if not torch.equal(o, want))
+
+    threads = [threading.Thread(target=work) for _ in range(6)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not wrong
