@@ -371,7 +371,8 @@ int rv_step_plan(rv_step* step, int32_t n_seqs, const int32_t* q_lens, const int
  * with strides in elements and unit stride along head_dim.  The first `rot` values of a head turn by
  * cos / sin [positions, rot / 2] (f32), as pairs (i, i + rot / 2), or (2i, 2i + 1) when interleaved;
  * f32 arithmetic, rounded once.  RV_E_INVALID where own_lens < q_lens, and where a page that new
- * tokens go to takes another sequence's new tokens too or is a prefix's. */
+ * tokens go to takes another sequence's new tokens too, is a prefix's, or stands among the pages of
+ * earlier keys of a sequence with new tokens. */
 int rv_step_append(rv_step* step, const rv_kv_cache* cache, const void* q, int64_t q_token_stride,
                    int64_t q_head_stride, const void* k, int64_t k_token_stride, int64_t k_head_stride, const void* v,
                    int64_t v_token_stride, int64_t v_head_stride, void* q_out, int64_t q_out_token_stride,

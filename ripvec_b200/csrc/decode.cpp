@@ -102,6 +102,7 @@ struct rv_step {
   std::vector<StepSeq> seq;
   std::vector<int> group_first, pg;
   std::vector<int> written;  // pages that new tokens go to
+  std::vector<uint64_t> written_bits;
   Schedule sched;
   // Calls on different streams wait for one another: plan, append and attend share the plan's device
   // records and the workspace.
@@ -502,11 +503,24 @@ int plan(rv_step* s, int32_t n_seqs, const int32_t* q_lens, const int32_t* own_l
     pa += count(prefix_lens[g]);
     s->group_first.push_back(b);
   }
-  // A page that new tokens go to stands in the step's lists once.  (A sequence's new tokens take consecutive places.)
+  // A page that new tokens go to is none that this step reads through another entry of its lists: another sequence's
+  // new tokens', a prefix's, or an earlier page of any sequence with queries.  (A sequence's new tokens take consecutive
+  // places, and all its entries before theirs are full of earlier keys.)  A table of 2^16 bits, by the low bits of the
+  // page, spares most entries the search.
   std::sort(written.begin(), written.end());
   if (std::adjacent_find(written.begin(), written.end()) != written.end()) can_append = false;
-  for (int64_t i = 0; i < n_prefix_pages && can_append && !written.empty(); ++i)
-    if (std::binary_search(written.begin(), written.end(), prefix_pages[i])) can_append = false;
+  if (can_append && !written.empty()) {
+    std::vector<uint64_t>& bits = s->written_bits;
+    bits.assign(1024, 0);
+    for (const int page : written) bits[page >> 6 & 1023] |= uint64_t(1) << (page & 63);
+    auto is_written = [&](int page) {
+      return (bits[page >> 6 & 1023] >> (page & 63) & 1) && std::binary_search(written.begin(), written.end(), page);
+    };
+    for (int64_t i = 0; i < n_prefix_pages && can_append; ++i) can_append = !is_written(prefix_pages[i]);
+    const int* list = own_pages;
+    for (b = 0; b < n_seqs && can_append; list += count(own_lens[b++]))
+      for (int i = 0; q_lens[b] > 0 && i < (own_lens[b] - q_lens[b]) / ps && can_append; ++i) can_append = !is_written(list[i]);
+  }
 
   Schedule& sc = s->sched;
   sc.row_items.clear();
@@ -701,7 +715,7 @@ int rv_step_append(rv_step* s, const rv_kv_cache* cache, const void* q, int64_t 
     if (!s->planned) return fail(s, RV_E_NOT_READY, "no plan");
     if (!s->can_append)
       return fail(s, RV_E_INVALID, "the plan cannot append: own_lens below q_lens, or a page that new tokens go to is "
-                                   "another sequence's or a prefix's");
+                                   "a prefix's, another sequence's or listed twice");
     rv::AppendArgs a{};
     rv::Act act;
     const std::string why = take_pool(s, cache, &a.pool, &act);

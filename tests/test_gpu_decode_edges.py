@@ -356,3 +356,31 @@ def test_one_step_in_many_threads(cuda_device):
     for t in threads:
         t.join()
     assert not wrong
+
+
+# ------------------------------------------------------------------ refusals
+def test_append_refuses_pages_that_others_read(cuda_device):
+    """New tokens would overwrite keys that the step reads: a page among another sequence's earlier ones, or twice in a
+    sequence's own list.  Without queries nothing is read, and pages that are only read may be shared."""
+    torch = _torch()
+    from ripvec_b200 import _lib as L
+
+    b = Batch(q=(2, 1), own=(20, 40), prefix=(40,), seed=72)
+    cos = torch.ones(100, 64, device="cuda")
+    k = b.randn(3, 2, 128)
+    (a0, a1), (b0, b1, b2) = b.own_pages
+
+    def plan(pages, q_lens=(2, 1)):
+        b.step.plan(q_lens=q_lens, own_lens=[20, 40], own_pages=pages, prefix_lens=[40], prefix_pages=b.prefix_pages,
+                    num_pages=b.cache.num_pages)
+
+    for pages in ([[a0, a1], [b0, a1, b2]], [[a1, a1], [b0, b1, b2]], [[a0, a1], [b2, b1, b2]], [[b2, a1], [b0, b1, b2]]):
+        plan(pages)
+        with pytest.raises(L.RvError):
+            b.step.append(b.cache, b.queries, k, k, cos, cos)
+        b.step.attend(b.cache, b.queries)
+    plan([[a0, a1], [a0, b1, b2]])  # an earlier page that both read
+    b.step.append(b.cache, b.queries, k, k, cos, cos)
+    plan([[a0, a1], [a0, a1, b2]], q_lens=(2, 0))  # a sequence that rests
+    b.step.append(b.cache, b.queries[:2], k[:2], k[:2], cos, cos)
+    torch.cuda.synchronize()
