@@ -723,6 +723,8 @@ int rv_step_append(rv_step* s, const rv_kv_cache* cache, const void* q, int64_t 
     if (rot < 0 || rot > s->head_dim || rot % 2) return fail(s, RV_E_INVALID, "rot must be even, from 0 to head_dim");
     if (s->n_tokens == 0) return RV_OK;
     if (!k || !v || !q != !q_out) return fail(s, RV_E_INVALID, "null keys or values, or queries without their output");
+    if (q && ((s->n_tokens > 1 && q_out_token == 0) || (s->q_heads > 1 && q_out_head == 0)))
+      return fail(s, RV_E_INVALID, "the rotated queries of several tokens or heads would go to one place");
     if (rot > 0 && (!cos || !sin || s->last_pos >= positions))
       return fail(s, RV_E_INVALID, "the rotation table is missing or shorter than the step's positions");
     a.tokens = s->tokens;

@@ -384,3 +384,18 @@ def test_append_refuses_pages_that_others_read(cuda_device):
     plan([[a0, a1], [a0, a1, b2]], q_lens=(2, 0))  # a sequence that rests
     b.step.append(b.cache, b.queries[:2], k[:2], k[:2], cos, cos)
     torch.cuda.synchronize()
+
+
+def test_append_refuses_outputs_that_overlap(cuda_device):
+    """As attend does: rotated queries of several tokens or heads in one place."""
+    torch = _torch()
+    from ripvec_b200 import _lib as L
+
+    b = Batch(q=(2, 1), own=(20, 40), seed=73)
+    cos = torch.ones(100, 64, device="cuda")
+    k = b.randn(3, 2, 128)
+    for shape in ((1, 8, 128), (3, 1, 128)):
+        one = torch.zeros(shape, dtype=k.dtype, device="cuda").expand(3, 8, 128)
+        with pytest.raises(L.RvError):
+            b.step.append(b.cache, b.queries, k, k, cos, cos, q_out=one)
+    torch.cuda.synchronize()
