@@ -191,7 +191,7 @@ int topk_device(rv_index* x, const float* q_dev, int nq, int k, float threshold,
     }
     IX_TRY(x, cudaStreamSynchronize(st));
     if (e) {
-      cudaMemset(x->d_err, 0, 4);
+      cudaMemsetAsync(x->d_err, 0, 4, x->stream);
       return ifail(x, RV_E_DEVICE, "scan kernel reported device error flags " + std::to_string(e));
     }
     if (ovf) {
@@ -263,7 +263,7 @@ int tq_device(rv_index* x, const float* q_dev, int nq, int top_k, float threshol
   }
   IX_TRY(x, cudaStreamSynchronize(st));
   if (e) {
-    cudaMemset(x->d_err, 0, 4);
+    cudaMemsetAsync(x->d_err, 0, 4, x->stream);
     return ifail(x, RV_E_DEVICE, "turboquant kernel reported device error flags " + std::to_string(e));
   }
   if (ovf)
@@ -296,7 +296,7 @@ int rv_index_create(int device, const void* src, int64_t n, int32_t dim, int32_t
     return code;
   };
   if (cudaStreamCreateWithFlags(&x->stream, cudaStreamNonBlocking) != cudaSuccess) return bail(RV_E_CUDA);
-  if (cudaMalloc(&x->d_err, 4) != cudaSuccess || cudaMemset(x->d_err, 0, 4) != cudaSuccess)
+  if (cudaMalloc(&x->d_err, 4) != cudaSuccess || cudaMemsetAsync(x->d_err, 0, 4, x->stream) != cudaSuccess)
     return bail(RV_E_NOMEM);
   const size_t elems = size_t(n) * dim;
   if (n > 0 && cudaMalloc(&x->db, elems * 2) != cudaSuccess) return bail(RV_E_NOMEM);
@@ -571,7 +571,7 @@ int rv_index_rank(rv_index* x, const float* query, float threshold, int64_t capa
   IX_TRY(x, cudaStreamSynchronize(st));
   x->launches++;
   if (e) {
-    cudaMemset(x->d_err, 0, 4);
+    cudaMemsetAsync(x->d_err, 0, 4, x->stream);
     return ifail(x, RV_E_DEVICE, "rank kernel reported device error flags " + std::to_string(e));
   }
   *out_count = static_cast<int64_t>(kept);
@@ -914,7 +914,7 @@ int rv_index_find_duplicates(rv_index* x, float threshold, int64_t max_pairs, in
     IX_TRY(x, cudaMemcpyAsync(&e, x->d_err, 4, cudaMemcpyDeviceToHost, st));
     IX_TRY(x, cudaStreamSynchronize(st));
     if (e) {
-      cudaMemset(x->d_err, 0, 4);
+      cudaMemsetAsync(x->d_err, 0, 4, x->stream);
       return ifail(x, RV_E_DEVICE, "duplicate search kernel reported device error flags " + std::to_string(e));
     }
     return RV_OK;

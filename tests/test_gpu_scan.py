@@ -210,3 +210,26 @@ def test_index_waits_for_rows_that_are_still_being_written(cuda_device):
         got = idx.export_rows(bf16_bits=True)
         idx.close()
         assert np.array_equal(got, rows.view(torch.int16).cpu().numpy().view(np.uint16))
+
+
+def test_index_made_beside_a_busy_default_stream(cuda_device):
+    """The index's error word is cleared in the index's own stream: what the memory held before is not taken for a
+    kernel's error while the default stream is busy."""
+    import torch
+
+    rt = pytest.importorskip("cuda.bindings.runtime")
+    query = np.ones((1, 128), np.float32)
+    first = SearchIndex(np.zeros((0, 128), np.float32))
+    assert first.topk(query, 5)[2].tolist() == [0]
+    small = [rt.cudaMalloc(4)[1] for _ in range(4096)]
+    for p in small:  # memory that the next small allocations get again
+        rt.cudaMemset(p, 255, 4)
+    torch.cuda.synchronize()
+    for p in small:
+        rt.cudaFree(p)
+    torch.cuda.synchronize()
+    torch.cuda._sleep(1_000_000_000)  # half a second of the default stream
+    idx = SearchIndex(np.zeros((0, 128), np.float32))
+    assert idx.topk(query, 5)[2].tolist() == [0]
+    assert not torch.cuda.default_stream().query()
+    torch.cuda.synchronize()
