@@ -18,8 +18,8 @@
 // S and P V of a row tile from one warp that was 2300 cycles a half tile, and the softmax waited for it.  The
 // reference maximum m moves only when a row's maximum grows by more than 2^8; then the row's O is rescaled in
 // TMEM, once the P V before is done.  An item's O is read out after the next item's first P is written, before
-// that item's first P V.  A causal prompt of 8192 tokens, 32 query and 8 key/value heads of 128: 490 us, 1120
-// TFLOP/s, in a short burst.
+// that item's first P V.  A causal prompt of 8192 tokens, 32 query and 8 key/value heads of 128: 492 to 507
+// us, 1085 to 1115 TFLOP/s, in a short burst.
 #include <algorithm>
 #include <cfloat>
 
@@ -71,8 +71,8 @@ __device__ __forceinline__ float max_nan(float a, float b) {
 // [-1/2, 1/2]; 2^f by a polynomial of degree 4, this project's own minimax fit of the relative error (2.7e-6;
 // mean 4e-8, which is what a row's sum sees); times 2^n built in the exponent field.  Below -126.5 the result is 0
 // (a masked score's weight), NaN stays NaN.  One pair in four of a tile's exponentials is computed so, beside the
-// others on the MUFU unit: 507 -> 479 us on a causal prompt of 8192 tokens, 32 heads of 128; every third or second
-// pair was slower.
+// others on the MUFU unit: 507 -> 479 us on a causal prompt of 8192 tokens, 32 heads of 128, when it was made
+// (changes of the compile since, and scores of any size, took back 3 to 5 %); every third or second pair was slower.
 __device__ __forceinline__ uint64_t f2_exp2(uint64_t x) {
   float a, b;
   f2_unpack(x, a, b);

@@ -122,12 +122,12 @@ int cuda_fail(rv_step* s, const char* what, cudaError_t e) {
   return fail(s, e == cudaErrorMemoryAllocation ? RV_E_NOMEM : RV_E_CUDA, std::string(what) + ": " + cudaGetErrorString(e));
 }
 
-// An error that an earlier call's kernels reported (without waiting for those still queued).
 // A record's double as f32; what is beyond its range becomes an infinity.
 float to_float(double v) {
   return std::fabs(v) > double(FLT_MAX) ? float(std::copysign(HUGE_VAL, v)) : float(v);
 }
 
+// An error that an earlier call's kernels reported (without waiting for those still queued).
 bool device_error(rv_step* s) {
   volatile unsigned int* w = s->err_host;
   if (!*w) return false;
@@ -318,7 +318,8 @@ double packing_saves(int64_t rows, int keys) {
 // more, up to kPackRows, do where it saves time, all of a group's or none, so that runs stay whole.  32 query and
 // 8 key/value heads of 128, packed against not: 64 sequences of 20 tokens over 32768 keys 714 and 1333 us, 16 of 30 to
 // 60 over 8000 121 and 135, 32 of 20 to 120 over 8000 334 and 368, 32 of 16 to 24 over 2000 57 and 63; over 1000 45 and
-// 42, where they walk alone.
+// 42, where they walk alone.  (Those constants are this one layout's.  Below half a row tile nothing is weighed: for 17
+// to 63 rows behind some hundred prefix keys the same formula would have each walk alone.)
 void schedule(const std::vector<StepSeq>& seqs, const std::vector<int>& group_first, int n_tokens, int fold,
               int groups, int head_dim,
               int sms, Schedule* out) {
