@@ -42,7 +42,8 @@ def _new(stream: int | None, like, shape: tuple, strides: tuple, dtype=None):
     current: on another one an earlier owner's reads could still be to come."""
     if stream is None or stream == _current_stream(like.get_device()):
         return like.new_empty_strided(shape, strides, dtype=dtype)
-    other = torch.cuda.ExternalStream(stream, like.device) if stream else torch.cuda.default_stream(like.device)
+    # (0 and 1, cudaStreamLegacy, are the default stream.)
+    other = torch.cuda.ExternalStream(stream, like.device) if stream > 1 else torch.cuda.default_stream(like.device)
     with torch.cuda.stream(other):
         return like.new_empty_strided(shape, strides, dtype=dtype)
 

@@ -295,6 +295,23 @@ def test_outputs_on_a_given_stream(cuda_device, call):
         assert (copy.view(torch.uint8) == 0).all()
 
 
+@pytest.mark.parametrize("handle", [0, 1, 2])
+def test_streams_without_an_object(cuda_device, handle):
+    """The default stream by its two handles, and the calling thread's."""
+    torch = _torch()
+    from ripvec_b200.decode import rms_norm
+
+    b = Batch(q=(1, 3), own=(40, 60), prefix=(100,), seed=76)
+    x, w = b.randn(5, 256), torch.ones(256, device="cuda")
+    for side in (torch.cuda.default_stream(), torch.cuda.Stream()):
+        torch.cuda.synchronize()
+        with torch.cuda.stream(side):
+            got = b.step.attend(b.cache, b.queries, stream=handle), *rms_norm(x, w, out_8bit=True, stream=handle)
+        torch.cuda.synchronize()
+        want = b.step.attend(b.cache, b.queries), *rms_norm(x, w, out_8bit=True)
+        assert all(torch.equal(g.view(torch.uint8), e.view(torch.uint8)) for g, e in zip(got, want))
+
+
 def test_one_handle_for_a_stream_of_each_thread(cuda_device):
     """cudaStreamPerThread is one handle and, in each host thread, another stream: a call waits for the step's earlier
     call of another thread."""
